@@ -1,0 +1,99 @@
+// Device helpers of the dense layer and layer norm: element types, activations, the column
+// sum's second stage.
+#pragma once
+#include "operators.hpp"
+#include "../lapis/launch.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace mace {
+namespace op {
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// U neighbouring elements, moved by one load or store.
+template <class T, int U> struct alignas(sizeof(T) * U) Unit {
+  T v[U];
+};
+
+// 1 / (1 + exp(-z)).  16-bit results take the fast exponential and division (a few 2^-22 of the
+// value, far below their own rounding).
+template <bool Fast> __device__ __forceinline__ float sigmoid(float z) {
+  return Fast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+}
+template <bool Fast> __device__ __forceinline__ float activate(float z, int act) {
+  if (act == Silu)
+    return Fast ? __fdividef(z, 1.f + __expf(-z)) : z / (1.f + expf(-z));
+  if (act == Gelu)
+    return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if (act == Relu)
+    return z < 0.f ? 0.f : z; // NaN stays
+  return z;
+}
+// d act / dz
+template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
+  if (act == Silu) {
+    float s = sigmoid<Fast>(z);
+    return s * (1.f + z * (1.f - s));
+  }
+  if (act == Gelu) {
+    float e = Fast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+    return 0.5f * (1.f + erff(z * 0.70710678f)) + z * e * 0.39894228f;
+  }
+  if (act == Relu)
+    return z <= 0.f ? 0.f : 1.f; // NaN passes the gradient, as a comparison that fails
+  return 1.f;
+}
+
+// Second stage of a sum over rows: out_k[c] = sum over p < parts of partial[p][k][c], k < 2
+// (out_k NULL: skipped), in a fixed order: lane group y takes p = y, y + 32, ..., then a tree.
+// 32 columns per block; the partials come from L2, so latency bounds it.
+template <class T> __global__ void __launch_bounds__(1024) column_sum_kernel(const float *partial, int parts, int planes,
+                                                                             long long width, T *out0, T *out1) {
+  __shared__ float sum[32][33];
+  int x = threadIdx.x & 31, y = threadIdx.x >> 5, k = blockIdx.y;
+  long long c = (long long)blockIdx.x * 32 + x;
+  T *out = k ? out1 : out0;
+  if (!out)
+    return;
+  float s = 0.f;
+  if (c < width)
+    for (int p = y; p < parts; p += 32)
+      s += partial[((long long)p * planes + k) * width + c];
+  sum[y][x] = s;
+  __syncthreads();
+  float v = sum[x][y]; // warp y sums column y over its lanes
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  c = (long long)blockIdx.x * 32 + y;
+  if (!x && c < width)
+    out[c] = from_float<T>(v);
+}
+
+inline int sm_count() {
+  static thread_local int device = -1, sms = 0;
+  int now = 0;
+  lapis::check(cudaGetDevice(&now));
+  if (now != device) {
+    lapis::check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, now));
+    device = now;
+  }
+  return sms;
+}
+inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+template <class F> void with_type(int type, F &&f) {
+  if (type == F32)
+    f(float{});
+  else if (type == BF16)
+    f(__nv_bfloat16{});
+  else
+    f(__half{});
+}
+} // namespace op
+} // namespace mace
