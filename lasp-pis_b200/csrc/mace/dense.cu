@@ -1,37 +1,28 @@
-// Dense layer, forward and backward: y = act(x W^T + b) + r; dx = dz W, dW = dz^T x, db = sum dz.
+// Dense layer, forward and backward: y = act(x W^T + b) + r; dx = dz W, dW = dz^T x, db = sum dz
+// with dz = dy act'(z).
 //
-// The three products are one kernel over operands with two strides each:
-//   out(i, j) = sum_k P(i, k) Q(j, k)
-//   forward  P = x (rows, inputs),  Q = W   (outputs, inputs)
-//   dx       P = dz (rows, outputs), Q = W^T (inputs, outputs)
-//   dW       P = dz^T (outputs, rows), Q = x^T (inputs, rows)
-// 64 x 64 output tiles, 4 x 4 per thread, float accumulation.
-#include "operators.cuh"
-#include <algorithm>
+// The three products are out(i, j) = sum_k P(i, k) Q(j, k):
+//   forward  P = x (rows, inputs),   Q = W (outputs, inputs)
+//   dx       P = dz (rows, outputs), Q = W turned (inputs, outputs)
+//   dW       P = dz turned (outputs, rows), Q = x turned (inputs, rows)
+// 16-bit types run on dense_gemm16.cu.  Around them: a copy of operands whose rows TMA cannot read in
+// place, and one pass over dy (and z) that writes dz and sums its columns.
+#include "dense_gemm.cuh"
 
 namespace mace {
 namespace op {
 namespace {
-struct Product {
+// ---------------- float products: 64 x 64 tiles, 4 x 4 per thread ----------------
+struct Plain {
   long long I, J, K;
-  const void *p;
-  long long pi, pk; // strides of P in elements
-  const void *q;
+  const float *p;
+  long long pi, pk; // strides of P
+  const float *q;
   long long qj, qk;
-  const void *bias; // [J]
-  int activation;
-  const void *residual;
-  long long ldr;
-  void *out;
-  long long ldo;
-  void *z;
-  long long ldz;
+  Epilogue e;
 };
-
-template <class T> __global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Product a) {
-  constexpr bool Fast = sizeof(T) == 2;
+__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Plain a) {
   __shared__ float ps[16][65], qs[16][65];
-  const T *p = static_cast<const T *>(a.p), *q = static_cast<const T *>(a.q);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long i0 = (long long)blockIdx.x * 64, j0 = (long long)blockIdx.y * 64;
   float acc[4][4] = {};
@@ -40,8 +31,8 @@ template <class T> __global__ void __launch_bounds__(256) product_kernel(const _
       // Consecutive threads walk the contiguous index.
       int kp = a.pk == 1 ? e & 15 : e >> 6, ip = a.pk == 1 ? e >> 4 : e & 63;
       int kq = a.qk == 1 ? e & 15 : e >> 6, jq = a.qk == 1 ? e >> 4 : e & 63;
-      ps[kp][ip] = i0 + ip < a.I && k0 + kp < a.K ? to_float(p[(i0 + ip) * a.pi + (k0 + kp) * a.pk]) : 0.f;
-      qs[kq][jq] = j0 + jq < a.J && k0 + kq < a.K ? to_float(q[(j0 + jq) * a.qj + (k0 + kq) * a.qk]) : 0.f;
+      ps[kp][ip] = i0 + ip < a.I && k0 + kp < a.K ? a.p[(i0 + ip) * a.pi + (k0 + kp) * a.pk] : 0.f;
+      qs[kq][jq] = j0 + jq < a.J && k0 + kq < a.K ? a.q[(j0 + jq) * a.qj + (k0 + kq) * a.qk] : 0.f;
     }
     __syncthreads();
 #pragma unroll
@@ -58,90 +49,249 @@ template <class T> __global__ void __launch_bounds__(256) product_kernel(const _
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       long long r = i0 + ty + 16 * i, c = j0 + tx + 16 * j;
-      if (r >= a.I || c >= a.J)
-        continue;
-      float v = acc[i][j] + (a.bias ? to_float(static_cast<const T *>(a.bias)[c]) : 0.f);
-      if (a.z)
-        static_cast<T *>(a.z)[r * a.ldz + c] = from_float<T>(v);
-      v = activate<Fast>(v, a.activation);
-      if (a.residual)
-        v += to_float(static_cast<const T *>(a.residual)[r * a.ldr + c]);
-      static_cast<T *>(a.out)[r * a.ldo + c] = from_float<T>(v);
+      if (r < a.I && c < a.J)
+        finish<float>(a.e, r, c, acc[i][j]);
     }
 }
+void product32(const Product &p, cudaStream_t stream) {
+  Plain a{p.I, p.J, p.K, static_cast<const float *>(p.p.p), p.p.turned ? 1 : p.p.ld, p.p.turned ? p.p.ld : 1,
+          static_cast<const float *>(p.q.p), p.q.turned ? 1 : p.q.ld, p.q.turned ? p.q.ld : 1, p.e};
+  dim3 grid(unsigned((p.I + 63) / 64), unsigned((p.J + 63) / 64));
+  lapis::launch(product_kernel, grid, 256, 0, stream, a);
+  lapis::check(cudaGetLastError());
+}
 
-// dz = dy act'(z) into dz [rows][outputs] (NULL: not written) and the partial column sums of its
-// float values, [gridDim.y][outputs] (NULL: not wanted).
-template <class T>
-__global__ void __launch_bounds__(256) gradient_kernel(const __grid_constant__ DenseBackward a, T *dz, float *partial) {
+// ---------------- one pass over dy ----------------
+// A block is `lanes` columns units wide (a power of two up to 32) and 256 / lanes rows high; it walks
+// rows by gridDim.y blocks' heights, writes dz = dy act'(z) (dz NULL: not wanted) and adds its columns:
+// partial [gridDim.y][outputs] (NULL: not wanted).  Memory-bound: every value is read once.
+template <class T, int U>
+__global__ void __launch_bounds__(256)
+    gradient_kernel(const __grid_constant__ DenseBackward a, T *dz, long long lddz, float *partial, int lanes) {
   constexpr bool Fast = sizeof(T) == 2;
-  long long c = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.outputs)
+  constexpr int kAhead = 4; // rows in flight per thread
+  using Un = Unit<T, U>;
+  __shared__ float join[256 * U];
+  const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, high = 256 / lanes;
+  const long long col = ((long long)blockIdx.x * lanes + tx) * U;
+  const bool live = col < a.outputs;
+  const long long step = (long long)gridDim.y * high;
+  float sum[U] = {};
+  if (live)
+    for (long long r0 = (long long)blockIdx.y * high + ty; r0 < a.rows; r0 += step * kAhead) {
+      Un dy[kAhead], z[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const long long r = r0 + k * step;
+        if (r < a.rows) {
+          dy[k] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.dy) + r * a.lddy + col);
+          if (a.activation != None)
+            z[k] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.z) + r * a.ldz + col);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const long long r = r0 + k * step;
+        if (r >= a.rows)
+          break;
+        Un o;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float v = to_float(dy[k].v[u]);
+          if (a.activation != None)
+            v *= slope<Fast>(to_float(z[k].v[u]), a.activation);
+          sum[u] += v;
+          o.v[u] = from_float<T>(v);
+        }
+        if (dz)
+          *reinterpret_cast<Un *>(dz + r * lddz + col) = o;
+      }
+    }
+  if (!partial)
     return;
-  float sum = 0.f;
-  for (long long r = blockIdx.y; r < a.rows; r += gridDim.y) {
-    float v = to_float(static_cast<const T *>(a.dy)[r * a.lddy + c]);
-    if (a.activation != None)
-      v *= slope<Fast>(to_float(static_cast<const T *>(a.z)[r * a.ldz + c]), a.activation);
-    sum += v;
-    if (dz)
-      dz[r * a.outputs + c] = from_float<T>(v);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    join[(ty * lanes + tx) * U + u] = sum[u];
+  __syncthreads();
+  const long long c0 = (long long)blockIdx.x * lanes * U;
+  for (int c = threadIdx.x; c < lanes * U; c += 256) {
+    float s = 0.f;
+    for (int y = 0; y < high; ++y)
+      s += join[y * lanes * U + c];
+    if (c0 + c < a.outputs)
+      partial[blockIdx.y * a.outputs + c0 + c] = s;
   }
-  if (partial)
-    partial[blockIdx.y * a.outputs + c] = sum;
 }
 
-int parts_of(long long rows) { return int(std::min<long long>(rows, 256)); }
-long long round16(long long n) { return (n + 15) / 16 * 16; }
-
-void product(int type, const Product &p, cudaStream_t stream) {
-  with_type(type, [&](auto tag) {
-    dim3 grid(unsigned((p.I + 63) / 64), unsigned((p.J + 63) / 64));
-    lapis::launch(product_kernel<decltype(tag)>, grid, 256, 0, stream, p);
-    lapis::check(cudaGetLastError());
-  });
+// Copy of a [rows][cols] array with any row distance and alignment into rows of ldo elements.
+template <class T>
+__global__ void __launch_bounds__(256) pack_kernel(const T *in, long long ldi, T *out, long long ldo, long long rows,
+                                                   long long cols) {
+  for (long long r = blockIdx.y; r < rows; r += gridDim.y)
+    for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < cols; c += 256ll * gridDim.x)
+      out[r * ldo + c] = in[r * ldi + c];
 }
+
+// The pass's grid: about 8 blocks per SM.
+struct Pass {
+  int unit, lanes, grid_x, parts;
+};
+Pass pass_of(const DenseBackward &d, bool vectors) {
+  Pass p{vectors ? 16 / bytes_of(d.type) : 1, 1, 0, 0};
+  long long units = (d.outputs + p.unit - 1) / p.unit;
+  while (p.lanes < 32 && p.lanes < units)
+    p.lanes *= 2;
+  p.grid_x = int((units + p.lanes - 1) / p.lanes);
+  long long high = 256 / p.lanes, blocks = (d.rows + 4 * high - 1) / (4 * high);
+  p.parts = int(std::min<long long>({blocks, std::max(1ll, 8ll * sm_count() / p.grid_x), 2048}));
+  return p;
+}
+bool vectors_of(const DenseBackward &d) {
+  const int U = 16 / bytes_of(d.type);
+  return d.outputs % U == 0 && aligned16(d.dy) && (d.rows <= 1 || d.lddy % U == 0) &&
+         (d.activation == None || (aligned16(d.z) && (d.rows <= 1 || d.ldz % U == 0)));
+}
+// z's alignment is not known to the workspace call: the larger of both passes.
+long long partial_bytes(const DenseBackward &d) {
+  return round_up(std::max(pass_of(d, true).parts, pass_of(d, false).parts) * d.outputs * 4, 16);
+}
+
+// Where an operand lies once TMA can read it: in place, or copied behind `used` bytes of the workspace.
+struct Place {
+  long long at = -1, ld = 0, bytes = 0;
+};
+Place place(int type, const void *p, long long rows, long long cols, long long ld, long long &used) {
+  Place w;
+  w.ld = ld;
+  if (type == F32 || tma_ready(type, p, rows, ld))
+    return w;
+  w.at = used;
+  w.ld = round_up(cols, 16 / bytes_of(type));
+  w.bytes = round_up(rows * w.ld * bytes_of(type), 16);
+  used += w.bytes;
+  return w;
+}
+Operand bring(int type, const Place &w, const void *p, long long rows, long long cols, long long ld, bool turned,
+              void *workspace, cudaStream_t stream) {
+  if (w.at < 0)
+    return {p, ld, turned};
+  void *to = static_cast<char *>(workspace) + w.at;
+  using U16 = unsigned short;
+  dim3 grid(unsigned(std::min<long long>((cols + 255) / 256, 1024)), unsigned(std::min<long long>(rows, 8192)));
+  lapis::launch(pack_kernel<U16>, grid, 256, 0, stream, static_cast<const U16 *>(p), ld, static_cast<U16 *>(to), w.ld, rows,
+                cols);
+  lapis::check(cudaGetLastError());
+  return {to, w.ld, turned};
+}
+
+Epilogue plain_out(int type, void *out, long long ldo, long long I, long long J) {
+  Epilogue e{};
+  const int U = 16 / bytes_of(type);
+  e.out = out, e.ldo = ldo;
+  e.vectors = J % U == 0 && aligned16(out) && (I <= 1 || ldo % U == 0);
+  return e;
+}
+void product(const Product &p, void *workspace, cudaStream_t stream) {
+  if (p.type == F32)
+    product32(p, stream);
+  else
+    product16(p, workspace, stream);
+}
+long long product_workspace(int type, long long I, long long J, long long K) {
+  return type == F32 ? 0 : product16_workspace(I, J, K);
+}
+
+struct ForwardLayout {
+  Place x, w;
+  long long product, total;
+  explicit ForwardLayout(const Dense &d) {
+    long long used = 0;
+    x = place(d.type, d.x, d.rows, d.inputs, d.ldx, used);
+    w = place(d.type, d.weight, d.outputs, d.inputs, d.ldw, used);
+    product = used;
+    total = used + product_workspace(d.type, d.rows, d.outputs, d.inputs);
+  }
+};
+struct BackwardLayout {
+  Place dz, x, w;
+  bool write_dz; // by the pass over dy: the activation's slope, or a copy that TMA can read
+  long long partial, product, total;
+  explicit BackwardLayout(const DenseBackward &d) {
+    long long used = 0;
+    partial = used;
+    used += partial_bytes(d);
+    write_dz = d.activation != None || !(d.type == F32 || tma_ready(d.type, d.dy, d.rows, d.lddy));
+    dz.ld = d.lddy;
+    if (write_dz) {
+      dz.at = used;
+      dz.ld = round_up(d.outputs, 16 / bytes_of(d.type));
+      used += round_up(d.rows * dz.ld * bytes_of(d.type), 16);
+    }
+    x = place(d.type, d.x, d.rows, d.inputs, d.ldx, used);
+    w = place(d.type, d.weight, d.outputs, d.inputs, d.ldw, used);
+    product = used;
+    total = used + std::max(product_workspace(d.type, d.rows, d.inputs, d.outputs),
+                            product_workspace(d.type, d.outputs, d.inputs, d.rows));
+  }
+};
 } // namespace
 
-long long dense_workspace(const Dense &) { return 0; }
-void dense(const Dense &d, void *, cudaStream_t stream) {
-  product(d.type,
-          {d.rows, d.outputs, d.inputs, d.x, d.ldx, 1, d.weight, d.ldw, 1, d.bias, d.activation, d.residual, d.ldr,
-           d.y, d.ldy, d.z, d.ldz},
-          stream);
+long long dense_workspace(const Dense &d) { return ForwardLayout(d).total; }
+void dense(const Dense &d, void *workspace, cudaStream_t stream) {
+  const ForwardLayout l(d);
+  const int U = 16 / bytes_of(d.type);
+  Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz, 0};
+  e.vectors = d.outputs % U == 0 && aligned16(d.bias) && aligned16(d.residual) && aligned16(d.y) && aligned16(d.z) &&
+              (d.rows <= 1 || (d.ldy % U == 0 && (!d.residual || d.ldr % U == 0) && (!d.z || d.ldz % U == 0)));
+  Product p{d.type, d.rows, d.outputs, d.inputs,
+            bring(d.type, l.x, d.x, d.rows, d.inputs, d.ldx, false, workspace, stream),
+            bring(d.type, l.w, d.weight, d.outputs, d.inputs, d.ldw, false, workspace, stream), e};
+  product(p, static_cast<char *>(workspace) + l.product, stream);
 }
 
-long long dense_backward_workspace(const DenseBackward &d) {
-  return round16(parts_of(d.rows) * d.outputs * 4) +
-         (d.activation != None ? round16(d.rows * d.outputs * bytes_of(d.type)) : 0);
-}
+long long dense_backward_workspace(const DenseBackward &d) { return BackwardLayout(d).total; }
 void dense_backward(const DenseBackward &d, void *workspace, cudaStream_t stream) {
-  with_type(d.type, [&](auto tag) {
-    using T = decltype(tag);
-    int parts = parts_of(d.rows);
-    float *partial = d.dbias ? static_cast<float *>(workspace) : nullptr;
-    T *dz = d.activation != None && (d.dx || d.dweight)
-                ? reinterpret_cast<T *>(static_cast<char *>(workspace) + round16(parts * d.outputs * 4))
-                : nullptr;
-    if (d.rows && (dz || partial))
-      lapis::launch(gradient_kernel<T>, dim3(unsigned((d.outputs + 255) / 256), unsigned(parts)), 256, 0, stream, d, dz,
-                    partial);
-    if (d.dbias)
-      lapis::launch(column_sum_kernel<T>, dim3(unsigned((d.outputs + 31) / 32), 1), 1024, 0, stream, partial, parts, 1,
-                    d.outputs, static_cast<T *>(d.dbias), static_cast<T *>(nullptr));
-    if (d.dbias || (d.rows && dz))
-      lapis::check(cudaGetLastError());
-    const void *g = dz ? dz : d.dy;
-    long long ldg = dz ? d.outputs : d.lddy;
-    if (d.dx && d.rows)
-      product(d.type, {d.rows, d.inputs, d.outputs, g, ldg, 1, d.weight, 1, d.ldw, nullptr, None, nullptr, 0, d.dx,
-                       d.lddx, nullptr, 0},
-              stream);
+  if (!d.rows) { // sums of nothing
     if (d.dweight)
-      product(d.type, {d.outputs, d.inputs, d.rows, g, 1, ldg, d.x, 1, d.ldx, nullptr, None, nullptr, 0, d.dweight,
-                       d.lddw, nullptr, 0},
-              stream);
-  });
+      lapis::check(cudaMemset2DAsync(d.dweight, size_t(d.lddw) * bytes_of(d.type), 0, size_t(d.inputs) * bytes_of(d.type),
+                                     size_t(d.outputs), stream));
+    if (d.dbias)
+      lapis::check(cudaMemsetAsync(d.dbias, 0, size_t(d.outputs) * bytes_of(d.type), stream));
+    return;
+  }
+  const BackwardLayout l(d);
+  char *ws = static_cast<char *>(workspace);
+  const bool products = d.dx || d.dweight, write_dz = products && l.write_dz;
+  float *partial = d.dbias ? reinterpret_cast<float *>(ws + l.partial) : nullptr;
+  void *dz = write_dz ? ws + l.dz.at : nullptr;
+  if (dz || partial)
+    with_type(d.type, [&](auto tag) {
+      using T = decltype(tag);
+      constexpr int V = 16 / int(sizeof(T));
+      const bool vectors = vectors_of(d);
+      const Pass p = pass_of(d, vectors);
+      dim3 grid(unsigned(p.grid_x), unsigned(p.parts));
+      if (vectors)
+        lapis::launch(gradient_kernel<T, V>, grid, 256, 0, stream, d, static_cast<T *>(dz), l.dz.ld, partial, p.lanes);
+      else
+        lapis::launch(gradient_kernel<T, 1>, grid, 256, 0, stream, d, static_cast<T *>(dz), l.dz.ld, partial, p.lanes);
+      if (partial)
+        lapis::launch(column_sum_kernel<T>, dim3(unsigned((d.outputs + 31) / 32), 1), 1024, 0, stream, partial, p.parts, 1,
+                      d.outputs, static_cast<T *>(d.dbias), static_cast<T *>(nullptr));
+      lapis::check(cudaGetLastError());
+    });
+  const void *g = dz ? dz : d.dy;
+  const long long ldg = dz ? l.dz.ld : d.lddy;
+  if (d.dx)
+    product({d.type, d.rows, d.inputs, d.outputs, {g, ldg, false},
+             bring(d.type, l.w, d.weight, d.outputs, d.inputs, d.ldw, true, workspace, stream),
+             plain_out(d.type, d.dx, d.lddx, d.rows, d.inputs)},
+            ws + l.product, stream);
+  if (d.dweight)
+    product({d.type, d.outputs, d.inputs, d.rows, {g, ldg, true},
+             bring(d.type, l.x, d.x, d.rows, d.inputs, d.ldx, true, workspace, stream),
+             plain_out(d.type, d.dweight, d.lddw, d.outputs, d.inputs)},
+            ws + l.product, stream);
 }
 } // namespace op
 } // namespace mace

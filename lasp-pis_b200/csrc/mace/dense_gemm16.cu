@@ -1,0 +1,362 @@
+// The dense layer's matrix products of 16-bit types on the tensor cores (tcgen05, kind::f16).
+//
+//   out(i, j) = sum_k P(i, k) Q(j, k), accumulated in float in TMEM
+//
+// An operand may be k-major ([I][K]) or turned ([K][I], the gradients' products): TMA brings 64-wide
+// slabs of k into shared memory in the layout that it has in global memory (SWIZZLE_128B), and the
+// matrix descriptor says which of the two it is.
+//
+// Persistent: one CTA per SM walks 128 x BN tiles.  10 warps: TMA producer, MMA issuer (one elected
+// thread), and eight that move a finished tile out of TMEM, through the epilogue and to global
+// memory while the next tile accumulates in TMEM's other half.  With too few tiles for the
+// device, K is cut into parts whose float products a second launch adds in order.
+#include "dense_gemm.cuh"
+
+namespace mace {
+namespace op {
+namespace {
+using namespace tc;
+constexpr int kBM = 128, kBK = 64;
+constexpr int kThreads = 320, kEpilogueThreads = 256;
+constexpr int kStageRing = 192 * 1024; // bytes of the operand ring
+constexpr int kStageFloats = 8 * 32 * 33;
+constexpr int kSmem = 1024 + kStageRing + kStageFloats * 4 + 256;
+static_assert(kSmem + 64 <= 232448, "shared memory budget");
+
+struct Gemm16 {
+  CUtensorMap p, q;
+  long long I, J;
+  int slabs, parts, p_rows, q_rows; // rows of a k-major operand's boxes
+  uint32_t idesc;
+  float *partial;
+  Epilogue e;
+};
+
+// Shared-memory descriptor of a turned operand (MN-major, SWIZZLE_128B): 64-wide blocks 8 KiB apart,
+// groups of 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t turned_desc(unsigned addr) {
+  return uint64_t((addr >> 4) & 0x3fff) | uint64_t(8192 >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
+         uint64_t(2) << 61;
+}
+
+template <class T, int BN, bool PT, bool QT>
+__global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_constant__ Gemm16 g) {
+  constexpr int kPBytes = kBM * kBK * 2, kQBytes = BN * kBK * 2, kStageBytes = kPBytes + kQBytes;
+  constexpr int kStages = kStageRing / kStageBytes;
+  constexpr int kTmemCols = 2 * BN;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float *staging = reinterpret_cast<float *>(smem + kStageRing);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kStageFloats); // full[S] | empty[S] | tfull[2] | tfree[2] | done
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int abort_flag;
+  __shared__ int mma_done_issued;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, tfull0 = empty0 + 8 * kStages,
+                 tfree0 = tfull0 + 16, done = tfree0 + 16;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mma_done_issued = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull0 + 8 * b, 1);
+      mbar_init(tfree0 + 8 * b, kEpilogueThreads);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const Tiles tiles(g.I, g.J, kBM, BN);
+  const long long units = tiles.count * g.parts;
+  // Slabs [first, last) of part s.
+  auto first_slab = [&](long long s) { return int(s * g.slabs / g.parts); };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      long long n = 0;
+      bool ok = true;
+      const unsigned bytes = (PT ? kPBytes : g.p_rows * 128) + (QT ? kQBytes : g.q_rows * 128);
+      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        long long i, j, s = u / tiles.count;
+        tiles.at(u - s * tiles.count, i, j);
+        const int i0 = int(i * kBM), j0 = int(j * BN);
+        for (int k = first_slab(s), end = first_slab(s + 1); k < end; ++k, ++n) {
+          const int st = int(n % kStages);
+          if (n >= kStages && !(ok = mbar_wait(empty0 + 8 * st, unsigned(n / kStages - 1) & 1, &abort_flag)))
+            break;
+          const unsigned base = smem_u32(smem + st * kStageBytes), full = full0 + 8 * st;
+          mbar_expect_tx(full, bytes);
+          if (PT) {
+#pragma unroll
+            for (int h = 0; h < kBM / 64; ++h)
+              tma_load_2d(base + 8192 * h, &g.p, i0 + 64 * h, k * kBK, full);
+          } else {
+            tma_load_2d(base, &g.p, k * kBK, i0, full);
+          }
+          if (QT) {
+#pragma unroll
+            for (int h = 0; h < BN / 64; ++h)
+              tma_load_2d(base + kPBytes + 8192 * h, &g.q, j0 + 64 * h, k * kBK, full);
+          } else {
+            tma_load_2d(base + kPBytes, &g.q, k * kBK, j0, full);
+          }
+        }
+      }
+      if (!ok) // copies in flight end (bounded wait) before the CTA does
+        for (long long m = n > kStages ? n - kStages : 0; m < n; ++m) {
+          long long start = clock64();
+          while (!mbar_try(full0 + 8 * int(m % kStages), unsigned(m / kStages) & 1) && clock64() - start < kWaitCycles) {
+          }
+        }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      long long n = 0;
+      int tile = 0;
+      bool ok = true;
+      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x, ++tile) {
+        const int b = tile & 1;
+        const long long s = u / tiles.count;
+        const uint32_t d = tmem + uint32_t(b * BN);
+        if (tile >= 2 && !(ok = mbar_wait(tfree0 + 8 * b, unsigned(tile / 2 - 1) & 1, &abort_flag)))
+          break;
+        tc_fence_after();
+        const int first = first_slab(s), end = first_slab(s + 1);
+        for (int k = first; k < end; ++k, ++n) {
+          const int st = int(n % kStages);
+          if (!(ok = mbar_wait(full0 + 8 * st, unsigned(n / kStages) & 1, &abort_flag)))
+            break;
+          tc_fence_after();
+          const unsigned base = smem_u32(smem + st * kStageBytes);
+          // 16-wide k steps: 32 bytes into k-major rows, two groups of 8 rows into turned ones.
+#pragma unroll
+          for (int m = 0; m < kBK / 16; ++m)
+            umma_f16_desc(d, PT ? turned_desc(base + 2048 * m) : smem_desc(base + 32 * m),
+                          QT ? turned_desc(base + kPBytes + 2048 * m) : smem_desc(base + kPBytes + 32 * m), g.idesc,
+                          k > first || m ? 1u : 0u);
+          umma_commit(empty0 + 8 * st);
+        }
+        if (ok)
+          umma_commit(tfull0 + 8 * b);
+      }
+      umma_commit(done);
+      mma_done_issued = 1;
+    }
+  } else {
+    // Two warps per TMEM lane quadrant, each with half of the columns.
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    float *stage = staging + (warp - 2) * 32 * 33;
+    bool ok = true;
+    int tile = 0;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
+      const int b = tile & 1;
+      const long long s = u / tiles.count;
+      long long i, j;
+      tiles.at(u - s * tiles.count, i, j);
+      ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(tile / 2) & 1, &abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
+      const long long row0 = i * kBM + 32 * quarter;
+#pragma unroll 1
+      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        const long long col0 = j * BN + c;
+        if (row0 >= g.I || col0 >= g.J)
+          break;
+        uint32_t r[32];
+        float v[32];
+        tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + c), r);
+        tmem_wait_ld();
+        tmem_anchor(r);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) // a wait that ran out shows as NaN
+          v[k] = ok ? __uint_as_float(r[k]) : __uint_as_float(0x7fc00000u);
+        finish_block<T>(g.e, partial, g.I, g.J, row0, col0, v, stage);
+      }
+      tc_fence_before();
+      mbar_arrive(tfree0 + 8 * b);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (abort_flag && mma_done_issued) { // bounded wait for the MMAs in flight before TMEM goes
+      long long start = clock64();
+      while (!mbar_try(done, 0) && clock64() - start < kWaitCycles) {
+      }
+    }
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) finish_parts_kernel(const __grid_constant__ Epilogue e, const float *partial,
+                                                           int parts, long long I, long long J) {
+  const long long plane = I * J;
+  if (e.vectors) {
+    constexpr int U = 16 / int(sizeof(T));
+    for (long long x = U * ((long long)blockIdx.x * 256 + threadIdx.x); x < plane; x += U * 256ll * gridDim.x) {
+      float s[U] = {};
+      for (int p = 0; p < parts; ++p)
+#pragma unroll
+        for (int k = 0; k < U; k += 4) {
+          float4 v = *reinterpret_cast<const float4 *>(partial + p * plane + x + k);
+          s[k] += v.x, s[k + 1] += v.y, s[k + 2] += v.z, s[k + 3] += v.w;
+        }
+      const long long row = x / J;
+      finish_row<T>(e, row, x - row * J, s);
+    }
+    return;
+  }
+  for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < plane; x += 256ll * gridDim.x) {
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p)
+      s += partial[p * plane + x];
+    finish<T>(e, x / J, x % J, s);
+  }
+}
+
+// Tile width and parts of K.  A tile twice as wide costs less than twice the time (P is read once);
+// few tiles are cut along K until they fill the device, parts of at least four slabs.
+struct Plan {
+  int bn, parts;
+};
+Plan plan_of(long long I, long long J, long long K) {
+  const int sms = sm_count();
+  const long long slabs = (K + kBK - 1) / kBK;
+  Plan best{0, 1};
+  double cost = 0;
+  for (int bn : {256, 128, 64}) {
+    long long tiles = Tiles(I, J, kBM, bn).count;
+    int parts = int(std::min<long long>({std::max(1ll, sms / tiles), std::max(1ll, slabs / 4), 64}));
+    long long waves = (tiles * parts + sms - 1) / sms;
+    double c = double(waves) * double((slabs + parts - 1) / parts) * (bn == 256 ? 1. : bn == 128 ? .56 : .36);
+    if (!best.bn || c < cost)
+      best = {bn, parts}, cost = c;
+  }
+  return best;
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  if (!fn)
+    throw lapis::Error("cuTensorMapEncodeTiled is unavailable");
+  return fn;
+}
+
+template <class T, int BN, bool PT, bool QT> void launch_gemm16(const Gemm16 &g, cudaStream_t stream) {
+  static thread_local int configured = -1;
+  int device = 0;
+  lapis::check(cudaGetDevice(&device));
+  if (configured != device) {
+    lapis::check(cudaFuncSetAttribute(gemm16_kernel<T, BN, PT, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    configured = device;
+  }
+  long long units = Tiles(g.I, g.J, kBM, BN).count * g.parts;
+  lapis::launch(gemm16_kernel<T, BN, PT, QT>, dim3(unsigned(std::min<long long>(units, sm_count()))), kThreads, kSmem, stream, g);
+  lapis::check(cudaGetLastError());
+}
+} // namespace
+
+CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows) {
+  const int b = bytes_of(type);
+  if (rows <= 1)
+    ld = round_up(cols, 16 / b);
+  CUtensorMap map;
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * unsigned(b)};
+  cuuint32_t box[2] = {cuuint32_t(128 / b), cuuint32_t(box_rows)}, elem[2] = {1, 1};
+  CUresult r = encoder()(&map,
+                         type == F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                         : type == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    throw lapis::Error("cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+  return map;
+}
+
+long long product16_workspace(long long I, long long J, long long K) {
+  Plan p = plan_of(I, J, K);
+  return p.parts > 1 ? round_up(p.parts * I * J * 4, 16) : 0;
+}
+
+void product16(const Product &p, void *workspace, cudaStream_t stream) {
+  const Plan plan = plan_of(p.I, p.J, p.K);
+  Gemm16 g{};
+  g.I = p.I, g.J = p.J;
+  g.slabs = int((p.K + kBK - 1) / kBK);
+  g.parts = plan.parts;
+  // Boxes of a short k-major operand end with its rows (in groups of 8): what lies behind them in
+  // shared memory reaches no output that is written.
+  g.p_rows = int(std::min<long long>(kBM, round_up(p.I, 8)));
+  g.q_rows = int(std::min<long long>(plan.bn, round_up(p.J, 8)));
+  g.p = p.p.turned ? tile_map(p.type, p.p.p, p.K, p.I, p.p.ld, kBK) : tile_map(p.type, p.p.p, p.I, p.K, p.p.ld, g.p_rows);
+  g.q = p.q.turned ? tile_map(p.type, p.q.p, p.K, p.J, p.q.ld, kBK) : tile_map(p.type, p.q.p, p.J, p.K, p.q.ld, g.q_rows);
+  const uint32_t format = p.type == BF16 ? 1 : 0;
+  g.idesc = idesc_f16(kBM, plan.bn) | format << 7 | format << 10 | uint32_t(p.p.turned) << 15 | uint32_t(p.q.turned) << 16;
+  g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
+  g.e = p.e;
+  auto run = [&](auto tag) {
+    using T = decltype(tag);
+    auto width = [&](auto bn) {
+      constexpr int BN = decltype(bn)::value;
+      if (!p.p.turned && !p.q.turned)
+        launch_gemm16<T, BN, false, false>(g, stream);
+      else if (!p.p.turned)
+        launch_gemm16<T, BN, false, true>(g, stream);
+      else
+        launch_gemm16<T, BN, true, true>(g, stream);
+    };
+    if (plan.bn == 256)
+      width(std::integral_constant<int, 256>{});
+    else if (plan.bn == 128)
+      width(std::integral_constant<int, 128>{});
+    else
+      width(std::integral_constant<int, 64>{});
+  };
+  if (p.type == BF16)
+    run(__nv_bfloat16{});
+  else
+    run(__half{});
+  if (plan.parts > 1)
+    finish_parts(p.type, p.e, g.partial, plan.parts, p.I, p.J, stream);
+}
+
+void finish_parts(int type, const Epilogue &e, const float *partial, int parts, long long I, long long J,
+                  cudaStream_t stream) {
+  with_type(type, [&](auto tag) {
+    long long blocks = (I * J + 1023) / 1024;
+    lapis::launch(finish_parts_kernel<decltype(tag)>, dim3(unsigned(std::min<long long>(blocks, 8ll * sm_count()))), 256,
+                  0, stream, e, partial, parts, I, J);
+    lapis::check(cudaGetLastError());
+  });
+}
+} // namespace op
+} // namespace mace
