@@ -5,62 +5,14 @@
 //   forward  P = x (rows, inputs),   Q = W (outputs, inputs)
 //   dx       P = dz (rows, outputs), Q = W turned (inputs, outputs)
 //   dW       P = dz turned (outputs, rows), Q = x turned (inputs, rows)
-// 16-bit types run on dense_gemm16.cu.  Around them: a copy of operands whose rows TMA cannot read in
-// place, and one pass over dy (and z) that writes dz and sums its columns.
+// 16-bit types run on dense_gemm16.cu, floats on dense_gemm32.cu.  Around them: a copy of 16-bit
+// operands whose rows TMA cannot read in place, and one pass over dy (and z) that writes dz and sums
+// its columns.
 #include "dense_gemm.cuh"
 
 namespace mace {
 namespace op {
 namespace {
-// ---------------- float products: 64 x 64 tiles, 4 x 4 per thread ----------------
-struct Plain {
-  long long I, J, K;
-  const float *p;
-  long long pi, pk; // strides of P
-  const float *q;
-  long long qj, qk;
-  Epilogue e;
-};
-__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Plain a) {
-  __shared__ float ps[16][65], qs[16][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const long long i0 = (long long)blockIdx.x * 64, j0 = (long long)blockIdx.y * 64;
-  float acc[4][4] = {};
-  for (long long k0 = 0; k0 < a.K; k0 += 16) {
-    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
-      // Consecutive threads walk the contiguous index.
-      int kp = a.pk == 1 ? e & 15 : e >> 6, ip = a.pk == 1 ? e >> 4 : e & 63;
-      int kq = a.qk == 1 ? e & 15 : e >> 6, jq = a.qk == 1 ? e >> 4 : e & 63;
-      ps[kp][ip] = i0 + ip < a.I && k0 + kp < a.K ? a.p[(i0 + ip) * a.pi + (k0 + kp) * a.pk] : 0.f;
-      qs[kq][jq] = j0 + jq < a.J && k0 + kq < a.K ? a.q[(j0 + jq) * a.qj + (k0 + kq) * a.qk] : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = fmaf(ps[k][ty + 16 * i], qs[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      long long r = i0 + ty + 16 * i, c = j0 + tx + 16 * j;
-      if (r < a.I && c < a.J)
-        finish<float>(a.e, r, c, acc[i][j]);
-    }
-}
-void product32(const Product &p, cudaStream_t stream) {
-  Plain a{p.I, p.J, p.K, static_cast<const float *>(p.p.p), p.p.turned ? 1 : p.p.ld, p.p.turned ? p.p.ld : 1,
-          static_cast<const float *>(p.q.p), p.q.turned ? 1 : p.q.ld, p.q.turned ? p.q.ld : 1, p.e};
-  dim3 grid(unsigned((p.I + 63) / 64), unsigned((p.J + 63) / 64));
-  lapis::launch(product_kernel, grid, 256, 0, stream, a);
-  lapis::check(cudaGetLastError());
-}
-
 // ---------------- one pass over dy ----------------
 // A block is `lanes` columns units wide (a power of two up to 32) and 256 / lanes rows high; it walks
 // rows by gridDim.y blocks' heights, writes dz = dy act'(z) (dz NULL: not wanted) and adds its columns:
@@ -184,21 +136,14 @@ Operand bring(int type, const Place &w, const void *p, long long rows, long long
   return {to, w.ld, turned};
 }
 
-Epilogue plain_out(int type, void *out, long long ldo, long long I, long long J) {
-  Epilogue e{};
-  const int U = 16 / bytes_of(type);
-  e.out = out, e.ldo = ldo;
-  e.vectors = J % U == 0 && aligned16(out) && (I <= 1 || ldo % U == 0);
-  return e;
-}
 void product(const Product &p, void *workspace, cudaStream_t stream) {
   if (p.type == F32)
-    product32(p, stream);
+    product32(p, workspace, stream);
   else
     product16(p, workspace, stream);
 }
 long long product_workspace(int type, long long I, long long J, long long K) {
-  return type == F32 ? 0 : product16_workspace(I, J, K);
+  return parts_workspace(type == F32 ? plan32(I, J, K) : plan16(I, J, K), I, J);
 }
 
 struct ForwardLayout {
@@ -239,10 +184,7 @@ struct BackwardLayout {
 long long dense_workspace(const Dense &d) { return ForwardLayout(d).total; }
 void dense(const Dense &d, void *workspace, cudaStream_t stream) {
   const ForwardLayout l(d);
-  const int U = 16 / bytes_of(d.type);
-  Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz, 0};
-  e.vectors = d.outputs % U == 0 && aligned16(d.bias) && aligned16(d.residual) && aligned16(d.y) && aligned16(d.z) &&
-              (d.rows <= 1 || (d.ldy % U == 0 && (!d.residual || d.ldr % U == 0) && (!d.z || d.ldz % U == 0)));
+  const Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz};
   Product p{d.type, d.rows, d.outputs, d.inputs,
             bring(d.type, l.x, d.x, d.rows, d.inputs, d.ldx, false, workspace, stream),
             bring(d.type, l.w, d.weight, d.outputs, d.inputs, d.ldw, false, workspace, stream), e};
@@ -285,12 +227,12 @@ void dense_backward(const DenseBackward &d, void *workspace, cudaStream_t stream
   if (d.dx)
     product({d.type, d.rows, d.inputs, d.outputs, {g, ldg, false},
              bring(d.type, l.w, d.weight, d.outputs, d.inputs, d.ldw, true, workspace, stream),
-             plain_out(d.type, d.dx, d.lddx, d.rows, d.inputs)},
+             Epilogue{nullptr, None, nullptr, 0, d.dx, d.lddx}},
             ws + l.product, stream);
   if (d.dweight)
     product({d.type, d.outputs, d.inputs, d.rows, {g, ldg, true},
              bring(d.type, l.x, d.x, d.rows, d.inputs, d.ldx, true, workspace, stream),
-             plain_out(d.type, d.dweight, d.lddw, d.outputs, d.inputs)},
+             Epilogue{nullptr, None, nullptr, 0, d.dweight, d.lddw}},
             ws + l.product, stream);
 }
 } // namespace op

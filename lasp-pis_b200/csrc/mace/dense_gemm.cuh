@@ -24,7 +24,12 @@ struct Epilogue {
   long long ldo;
   void *z;
   long long ldz;
-  int vectors; // every array's rows start on 16-byte boundaries and J is a multiple of 16 bytes
+};
+// How the finished blocks reach memory.  on: as boxes of 32 rows through TMA, where y, z and the
+// residual (or the parts) have 16-byte aligned rows; columns past J are clipped.
+struct Boxes {
+  CUtensorMap y, z, residual; // y: the parts, when K is cut
+  int on;
 };
 struct Product {
   int type;
@@ -60,90 +65,140 @@ __device__ __forceinline__ void finish(const Epilogue &e, long long row, long lo
     v += to_float(static_cast<const T *>(e.residual)[row * e.ldr + col]);
   static_cast<T *>(e.out)[row * e.ldo + col] = from_float<T>(v);
 }
-// N neighbouring values (N a multiple of a 16-byte unit), for arrays that allow vectors.
-template <class T, int N>
-__device__ __forceinline__ void finish_row(const Epilogue &e, long long row, long long col, float (&v)[N]) {
-  constexpr bool Fast = sizeof(T) == 2;
-  constexpr int U = 16 / int(sizeof(T));
-  using Un = Unit<T, U>;
-#pragma unroll
-  for (int k = 0; k < N; k += U) {
-    if (e.bias) {
-      Un b = *reinterpret_cast<const Un *>(static_cast<const T *>(e.bias) + col + k);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        v[k + u] += to_float(b.v[u]);
-    }
-    if (e.z) {
-      Un z;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        z.v[u] = from_float<T>(v[k + u]);
-      *reinterpret_cast<Un *>(static_cast<T *>(e.z) + row * e.ldz + col + k) = z;
-    }
-    if (e.activation != None)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        v[k + u] = activate<Fast>(v[k + u], e.activation);
-    if (e.residual) {
-      Un r = *reinterpret_cast<const Un *>(static_cast<const T *>(e.residual) + row * e.ldr + col + k);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        v[k + u] += to_float(r.v[u]);
-    }
-    Un o;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      o.v[u] = from_float<T>(v[k + u]);
-    *reinterpret_cast<Un *>(static_cast<T *>(e.out) + row * e.ldo + col + k) = o;
-  }
-}
+// A warp's part of the epilogue: its shared memory, and the mbarrier of its residual boxes.
+struct Warp {
+  unsigned char *box; // 32 rows of a box, 1024-byte aligned
+  float *bias;        // 32 floats
+  unsigned bar, phase;
+};
 
-// A warp's 32 x 32 block of the product: lane = row, v = its columns from col0.  Rows that allow
-// no vectors go through `stage` (32 x 33 floats), so that neighbouring lanes write neighbouring
-// columns.  partial != NULL: the float values go to partial[row * J + col] instead.
-template <class T>
-__device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
-                                             long long row0, long long col0, float (&v)[32], float *stage) {
+// 32 rows by RB (64 or 128) bytes of the result from (row0, col0), rows = lanes.  get(c, v) gives the
+// product's columns col0 + c .. (as many as v holds).  T float with `part` >= 0: the values as they
+// are, to plane `part`.  Rows are swizzled in shared memory, so that neither side has bank
+// conflicts; TMA writes whole sectors.
+template <class T, int RB, class Get>
+__device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, long long J, long long row0,
+                                           long long col0, int part, Warp &w, Get &&get) {
+  constexpr bool Fast = sizeof(T) == 2;
+  constexpr int U = 16 / int(sizeof(T)), W = RB / int(sizeof(T)), N = W < 32 ? W : 32;
+  using Un = Unit<T, U>;
   const int lane = threadIdx.x & 31;
-  if (partial ? J % 4 == 0 : e.vectors) {
-    long long row = row0 + lane;
-    if (row < I) {
-      if (partial) {
+  unsigned char *mine = w.box + lane * RB;
+  const int swizzle = RB == 128 ? lane & 7 : (lane >> 1) & 3; // SWIZZLE_128B, SWIZZLE_64B
+  const bool plain = part >= 0;
+  auto block = [&](int c, float (&v)[N]) {
+    get(c, v);
+    if (plain || !e.bias)
+      return;
+    const long long col = col0 + c + lane;
+    __syncwarp();
+    w.bias[lane] = lane < N && col < J ? to_float(static_cast<const T *>(e.bias)[col]) : 0.f;
+    __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 32; k += 4)
-          if (col0 + k < J)
-            *reinterpret_cast<float4 *>(partial + row * J + col0 + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-      } else if (col0 + 32 <= J) {
-        finish_row<T>(e, row, col0, v);
-      } else {
-        constexpr int U = 16 / int(sizeof(T));
+    for (int k = 0; k < N; k += 4) {
+      const float4 b = *reinterpret_cast<const float4 *>(w.bias + k);
+      v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
+    }
+  };
+  auto free_box = [&] { // the box's last store has read it
+    if (lane == 0)
+      tc::bulk_wait_read();
+    __syncwarp();
+  };
+  auto send = [&](const CUtensorMap &map, int plane) {
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store_3d(&map, tc::smem_u32(w.box), int(col0), int(row0), plane);
+      tc::bulk_commit();
+    }
+  };
+  if (!plain && e.z) {
+    free_box();
 #pragma unroll
-        for (int k = 0; k < 32; k += U)
-          if (col0 + k < J) {
-            float w[U];
+    for (int c = 0; c < W; c += N) {
+      float v[N];
+      block(c, v);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-              w[u] = v[k + u];
-            finish_row<T>(e, row, col0 + k, w);
-          }
+      for (int k = 0; k < N; k += U) {
+        Un o;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          o.v[u] = from_float<T>(v[k + u]);
+        *reinterpret_cast<Un *>(mine + ((((c + k) / U) ^ swizzle) << 4)) = o;
       }
     }
-    return;
+    send(m.z, 0);
+  }
+  free_box();
+  const bool residual = !plain && e.residual;
+  if (residual && lane == 0) {
+    tc::mbar_expect_tx(w.bar, 32 * RB);
+    tc::tma_load_3d(tc::smem_u32(w.box), &m.residual, int(col0), int(row0), 0, w.bar);
   }
 #pragma unroll
-  for (int k = 0; k < 32; ++k)
-    stage[lane * 33 + k] = v[k];
-  __syncwarp();
-  long long col = col0 + lane;
-  int rows = int(min(32ll, I - row0));
-  if (col < J)
-    for (int r = 0; r < rows; ++r) {
-      if (partial)
-        partial[(row0 + r) * J + col] = stage[r * 33 + lane];
-      else
-        finish<T>(e, row0 + r, col, stage[r * 33 + lane]);
+  for (int c = 0; c < W; c += N) {
+    float v[N];
+    block(c, v);
+    if (!plain && e.activation != None)
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        v[k] = activate<Fast>(v[k], e.activation);
+    if (residual && c == 0) {
+      const long long start = clock64();
+      bool there = false;
+      while (!(there = tc::mbar_try(w.bar, w.phase)) && clock64() - start < tc::kWaitCycles) {
+      }
+      w.phase ^= 1;
+      if (!there) // shows as NaN
+        col0 = J;
     }
+#pragma unroll
+    for (int k = 0; k < N; k += U) {
+      Un *at = reinterpret_cast<Un *>(mine + ((((c + k) / U) ^ swizzle) << 4));
+      Un o;
+      if (residual) {
+        o = *at;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          v[k + u] += to_float(o.v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        o.v[u] = from_float<T>(v[k + u]);
+      *at = o;
+    }
+  }
+  send(m.y, plain ? part : 0);
+}
+
+// A warp's 32 x 32 block where rows allow no boxes: through 32 rows of 16 floats
+// (2 KiB, their columns permuted by row), so that
+// neighbouring lanes write neighbouring columns.  partial != NULL: the float values go to
+// partial[row * J + col] instead.
+template <class T>
+__device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
+                                             long long row0, long long col0, float *v, float *stage) {
+  const int lane = threadIdx.x & 31;
+  const int rows = int(min(32ll, I - row0));
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      stage[lane * 16 + (k ^ (lane & 15))] = v[h + k];
+    __syncwarp();
+    const long long col = col0 + h + (lane & 15);
+    if (col < J)
+#pragma unroll 4
+      for (int r = lane >> 4; r < rows; r += 2) {
+        const float x = stage[r * 16 + ((lane ^ r) & 15)];
+        if (partial)
+          partial[(row0 + r) * J + col] = x;
+        else
+          finish<T>(e, row0 + r, col, x);
+      }
+  }
   __syncwarp();
 }
 
@@ -151,17 +206,31 @@ __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, 
 inline long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 // Tensor map of a [rows][cols] array of 16-bit or float elements with row distance ld, in boxes of
-// box_rows rows by 128 bytes, SWIZZLE_128B; elements outside the array read as zero.
-CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows);
+// box_rows rows by box_bytes, swizzled by as much; elements outside the array read as zero.
+// planes: a third dimension of `rows` rows each (0: a map of two dimensions).
+CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows,
+                     int planes = 0, int box_bytes = 128);
+// The boxes of a product's results, or of its parts.
+Boxes boxes_of(const Product &, float *partial, int parts, int box_bytes);
 // Whether TMA can read the array in place: 16-byte aligned rows.
 inline bool tma_ready(int type, const void *p, long long rows, long long ld) {
   return aligned16(p) && (rows <= 1 || ld * bytes_of(type) % 16 == 0);
 }
 
-// The products of 16-bit types (dense_gemm16.cu): operands that TMA can read; workspace of
-// product16_workspace bytes.
-long long product16_workspace(long long I, long long J, long long K);
+// Tile width and parts of K of a product.
+struct Plan {
+  int bn, parts;
+};
+// Workspace of a product: the float values of its parts.
+inline long long parts_workspace(const Plan &p, long long I, long long J) {
+  return p.parts > 1 ? round_up(p.parts * I * J * 4, 16) : 0;
+}
+// The products of 16-bit types (dense_gemm16.cu; operands that TMA can read) and of floats
+// (dense_gemm32.cu; any operands).
+Plan plan16(long long I, long long J, long long K);
 void product16(const Product &, void *workspace, cudaStream_t);
+Plan plan32(long long I, long long J, long long K);
+void product32(const Product &, void *workspace, cudaStream_t);
 // Sum of `parts` float products [parts][I][J], through the epilogue.
 void finish_parts(int type, const Epilogue &, const float *partial, int parts, long long I, long long J, cudaStream_t);
 } // namespace op

@@ -19,8 +19,8 @@ using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 320, kEpilogueThreads = 256;
 constexpr int kStageRing = 192 * 1024; // bytes of the operand ring
-constexpr int kStageFloats = 8 * 32 * 33;
-constexpr int kSmem = 1024 + kStageRing + kStageFloats * 4 + 256;
+constexpr int kBoxBytes = 32 * 128;
+constexpr int kSmem = 1024 + kStageRing + 8 * kBoxBytes + 8 * 128 + 256;
 static_assert(kSmem + 64 <= 232448, "shared memory budget");
 
 struct Gemm16 {
@@ -30,6 +30,7 @@ struct Gemm16 {
   uint32_t idesc;
   float *partial;
   Epilogue e;
+  Boxes boxes;
 };
 
 // Shared-memory descriptor of a turned operand (MN-major, SWIZZLE_128B): 64-wide blocks 8 KiB apart,
@@ -46,14 +47,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   constexpr int kTmemCols = 2 * BN;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float *staging = reinterpret_cast<float *>(smem + kStageRing);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kStageFloats); // full[S] | empty[S] | tfull[2] | tfree[2] | done
+  unsigned char *staging = smem + kStageRing; // a box per epilogue warp, then its bias
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes + 8 * 128);
+  // full[S] | empty[S] | tfull[2] | tfree[2] | done | residual[8]
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
   __shared__ int mma_done_issued;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, tfull0 = empty0 + 8 * kStages,
-                 tfree0 = tfull0 + 16, done = tfree0 + 16;
+                 tfree0 = tfull0 + 16, done = tfree0 + 16, residual0 = done + 8;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     mma_done_issued = 0;
@@ -66,6 +68,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
       mbar_init(tfree0 + 8 * b, kEpilogueThreads);
     }
     mbar_init(done, 1);
+    for (int x = 0; x < 8; ++x)
+      mbar_init(residual0 + 8 * x, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
   }
@@ -157,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   } else {
     // Two warps per TMEM lane quadrant, each with half of the columns.
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    float *stage = staging + (warp - 2) * 32 * 33;
+    const int me = warp - 2;
+    Warp w{staging + me * kBoxBytes, reinterpret_cast<float *>(staging + 8 * kBoxBytes + me * 128), residual0 + 8 * me, 0};
     bool ok = true;
     int tile = 0;
     for (long long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
@@ -168,26 +173,46 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
       ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(tile / 2) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
       const long long row0 = i * kBM + 32 * quarter;
-#pragma unroll 1
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        const long long col0 = j * BN + c;
-        if (row0 >= g.I || col0 >= g.J)
-          break;
+      const uint32_t d = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN);
+      auto get = [&](int c, float (&v)[32]) { // the tile's columns c ..
         uint32_t r[32];
-        float v[32];
-        tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + c), r);
+        tmem_ld32_async(d + uint32_t(c), r);
         tmem_wait_ld();
         tmem_anchor(r);
 #pragma unroll
         for (int k = 0; k < 32; ++k) // a wait that ran out shows as NaN
           v[k] = ok ? __uint_as_float(r[k]) : __uint_as_float(0x7fc00000u);
-        finish_block<T>(g.e, partial, g.I, g.J, row0, col0, v, stage);
+      };
+      const int first = half * (BN / 2), end = first + BN / 2;
+      if (row0 < g.I) {
+        if (g.boxes.on && g.partial) {
+#pragma unroll 1
+          for (int c = first; c < end && j * BN + c < g.J; c += 32)
+            finish_box<float, 128>(g.e, g.boxes, g.J, row0, j * BN + c, int(s), w,
+                              [&](int k, float (&v)[32]) { get(c + k, v); });
+        } else if (g.boxes.on && BN >= 128) {
+#pragma unroll 1
+          for (int c = first; c < end && j * BN + c < g.J; c += 64)
+            finish_box<T, 128>(g.e, g.boxes, g.J, row0, j * BN + c, -1, w, [&](int k, float (&v)[32]) { get(c + k, v); });
+        } else if (g.boxes.on) { // one box per row quarter: the first of its two warps
+          if (!half)
+            finish_box<T, 128>(g.e, g.boxes, g.J, row0, j * BN, -1, w, get);
+        } else {
+          float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
+#pragma unroll 1
+          for (int c = first; c < end && j * BN + c < g.J; c += 32) {
+            float v[32];
+            get(c, v);
+            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, reinterpret_cast<float *>(w.box));
+          }
+        }
       }
       tc_fence_before();
       mbar_arrive(tfree0 + 8 * b);
     }
+    if (lane == 0)
+      bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -206,18 +231,17 @@ template <class T>
 __global__ void __launch_bounds__(256) finish_parts_kernel(const __grid_constant__ Epilogue e, const float *partial,
                                                            int parts, long long I, long long J) {
   const long long plane = I * J;
-  if (e.vectors) {
-    constexpr int U = 16 / int(sizeof(T));
-    for (long long x = U * ((long long)blockIdx.x * 256 + threadIdx.x); x < plane; x += U * 256ll * gridDim.x) {
-      float s[U] = {};
-      for (int p = 0; p < parts; ++p)
-#pragma unroll
-        for (int k = 0; k < U; k += 4) {
-          float4 v = *reinterpret_cast<const float4 *>(partial + p * plane + x + k);
-          s[k] += v.x, s[k + 1] += v.y, s[k + 2] += v.z, s[k + 3] += v.w;
-        }
-      const long long row = x / J;
-      finish_row<T>(e, row, x - row * J, s);
+  if (J % 4 == 0) {
+    for (long long x = 4 * ((long long)blockIdx.x * 256 + threadIdx.x); x < plane; x += 1024ll * gridDim.x) {
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int p = 0; p < parts; ++p) {
+        const float4 v = *reinterpret_cast<const float4 *>(partial + p * plane + x);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      const long long row = x / J, col = x - row * J;
+      finish<T>(e, row, col, s.x), finish<T>(e, row, col + 1, s.y);
+      finish<T>(e, row, col + 2, s.z), finish<T>(e, row, col + 3, s.w);
     }
     return;
   }
@@ -229,12 +253,10 @@ __global__ void __launch_bounds__(256) finish_parts_kernel(const __grid_constant
   }
 }
 
-// Tile width and parts of K.  A tile twice as wide costs less than twice the time (P is read once);
+// A tile twice as wide costs less than twice the time (P is read once);
 // few tiles are cut along K until they fill the device, parts of at least four slabs.
-struct Plan {
-  int bn, parts;
-};
-Plan plan_of(long long I, long long J, long long K) {
+} // namespace
+Plan plan16(long long I, long long J, long long K) {
   const int sms = sm_count();
   const long long slabs = (K + kBK - 1) / kBK;
   Plan best{0, 1};
@@ -249,6 +271,7 @@ Plan plan_of(long long I, long long J, long long K) {
   }
   return best;
 }
+namespace {
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -282,33 +305,51 @@ template <class T, int BN, bool PT, bool QT> void launch_gemm16(const Gemm16 &g,
 }
 } // namespace
 
-CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows) {
+CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows,
+                     int planes, int box_bytes) {
   const int b = bytes_of(type);
   if (rows <= 1)
     ld = round_up(cols, 16 / b);
   CUtensorMap map;
-  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(ld) * unsigned(b)};
-  cuuint32_t box[2] = {cuuint32_t(128 / b), cuuint32_t(box_rows)}, elem[2] = {1, 1};
+  cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(planes)};
+  cuuint64_t strides[2] = {cuuint64_t(ld) * unsigned(b), cuuint64_t(ld) * cuuint64_t(rows) * unsigned(b)};
+  cuuint32_t box[3] = {cuuint32_t(box_bytes / b), cuuint32_t(box_rows), 1}, elem[3] = {1, 1, 1};
   CUresult r = encoder()(&map,
                          type == F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                          : type == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                         2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         planes ? 3 : 2, const_cast<void *>(base), dims, strides, box, elem,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     throw lapis::Error("cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
   return map;
 }
 
-long long product16_workspace(long long I, long long J, long long K) {
-  Plan p = plan_of(I, J, K);
-  return p.parts > 1 ? round_up(p.parts * I * J * 4, 16) : 0;
+Boxes boxes_of(const Product &p, float *partial, int parts, int box_bytes) {
+  Boxes b{};
+  const Epilogue &e = p.e;
+  if (partial) {
+    b.on = p.J % 4 == 0;
+    if (b.on)
+      b.y = tile_map(F32, partial, p.I, p.J, p.J, 32, parts, box_bytes);
+    return b;
+  }
+  b.on = tma_ready(p.type, e.out, p.I, e.ldo) && (!e.z || tma_ready(p.type, e.z, p.I, e.ldz)) &&
+         (!e.residual || tma_ready(p.type, e.residual, p.I, e.ldr));
+  if (!b.on)
+    return b;
+  b.y = tile_map(p.type, e.out, p.I, p.J, e.ldo, 32, 1, box_bytes);
+  if (e.z)
+    b.z = tile_map(p.type, e.z, p.I, p.J, e.ldz, 32, 1, box_bytes);
+  if (e.residual)
+    b.residual = tile_map(p.type, e.residual, p.I, p.J, e.ldr, 32, 1, box_bytes);
+  return b;
 }
 
 void product16(const Product &p, void *workspace, cudaStream_t stream) {
-  const Plan plan = plan_of(p.I, p.J, p.K);
+  const Plan plan = plan16(p.I, p.J, p.K);
   Gemm16 g{};
   g.I = p.I, g.J = p.J;
   g.slabs = int((p.K + kBK - 1) / kBK);
@@ -323,6 +364,7 @@ void product16(const Product &p, void *workspace, cudaStream_t stream) {
   g.idesc = idesc_f16(kBM, plan.bn) | format << 7 | format << 10 | uint32_t(p.p.turned) << 15 | uint32_t(p.q.turned) << 16;
   g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
   g.e = p.e;
+  g.boxes = boxes_of(p, g.partial, plan.parts, 128);
   auto run = [&](auto tag) {
     using T = decltype(tag);
     auto width = [&](auto bn) {
