@@ -5,7 +5,7 @@
 //   forward  P = x (rows, inputs),   Q = W (outputs, inputs)
 //   dx       P = dz (rows, outputs), Q = W turned (inputs, outputs)
 //   dW       P = dz turned (outputs, rows), Q = x turned (inputs, rows)
-// 16-bit types run on dense_gemm16.cu, floats on dense_gemm32.cu.  Around them: a copy of 16-bit
+// 16-bit types run on dense_gemm16.cu, floats on dense_gemm32.cu.  Around them: a copy of
 // operands whose rows TMA cannot read in place, and one pass over dy (and z) that writes dz and sums
 // its columns.
 #include "dense_gemm.cuh"
@@ -115,7 +115,7 @@ struct Place {
 Place place(int type, const void *p, long long rows, long long cols, long long ld, long long &used) {
   Place w;
   w.ld = ld;
-  if (type == F32 || tma_ready(type, p, rows, ld))
+  if (tma_ready(type, p, rows, ld))
     return w;
   w.at = used;
   w.ld = round_up(cols, 16 / bytes_of(type));
@@ -128,10 +128,15 @@ Operand bring(int type, const Place &w, const void *p, long long rows, long long
   if (w.at < 0)
     return {p, ld, turned};
   void *to = static_cast<char *>(workspace) + w.at;
-  using U16 = unsigned short;
   dim3 grid(unsigned(std::min<long long>((cols + 255) / 256, 1024)), unsigned(std::min<long long>(rows, 8192)));
-  lapis::launch(pack_kernel<U16>, grid, 256, 0, stream, static_cast<const U16 *>(p), ld, static_cast<U16 *>(to), w.ld, rows,
-                cols);
+  auto copy = [&](auto tag) {
+    using U = decltype(tag);
+    lapis::launch(pack_kernel<U>, grid, 256, 0, stream, static_cast<const U *>(p), ld, static_cast<U *>(to), w.ld, rows, cols);
+  };
+  if (type == F32)
+    copy(0u);
+  else
+    copy((unsigned short)0);
   lapis::check(cudaGetLastError());
   return {to, w.ld, turned};
 }
@@ -165,7 +170,7 @@ struct BackwardLayout {
     long long used = 0;
     partial = used;
     used += partial_bytes(d);
-    write_dz = d.activation != None || !(d.type == F32 || tma_ready(d.type, d.dy, d.rows, d.lddy));
+    write_dz = d.activation != None || !tma_ready(d.type, d.dy, d.rows, d.lddy);
     dz.ld = d.lddy;
     if (write_dz) {
       dz.at = used;

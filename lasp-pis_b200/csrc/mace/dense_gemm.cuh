@@ -65,42 +65,42 @@ __device__ __forceinline__ void finish(const Epilogue &e, long long row, long lo
     v += to_float(static_cast<const T *>(e.residual)[row * e.ldr + col]);
   static_cast<T *>(e.out)[row * e.ldo + col] = from_float<T>(v);
 }
-// A warp's part of the epilogue: its shared memory, and the mbarrier of its residual boxes.
+// A warp's part of the epilogue: a box of 32 rows by 128 bytes in shared memory, and the mbarrier of
+// its residual.
+constexpr int kBoxBytes = 32 * 128;
 struct Warp {
-  unsigned char *box; // 32 rows of a box, 1024-byte aligned
-  float *bias;        // 32 floats
+  unsigned char *box; // 1024-byte aligned
   unsigned bar, phase;
 };
+// Starts the load of a residual box (one lane; the box's last store has read it).
+__device__ __forceinline__ void fetch_residual(const Boxes &m, const Warp &w, long long row0, long long col0) {
+  tc::mbar_expect_tx(w.bar, kBoxBytes);
+  tc::tma_load_3d(tc::smem_u32(w.box), &m.residual, int(col0), int(row0), 0, w.bar);
+}
 
-// 32 rows by RB (64 or 128) bytes of the result from (row0, col0), rows = lanes.  get(c, v) gives the
-// product's columns col0 + c .. (as many as v holds).  T float with `part` >= 0: the values as they
-// are, to plane `part`.  Rows are swizzled in shared memory, so that neither side has bank
-// conflicts; TMA writes whole sectors.
-template <class T, int RB, class Get>
-__device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, long long J, long long row0,
-                                           long long col0, int part, Warp &w, Get &&get) {
+// 32 rows by 128 bytes of the result from (row0, col0), rows = lanes.  get(c, v) gives the product's
+// columns col0 + c .. + 31, and bias(c) the lane's (col0 + c + lane) bias.  part >= 0 (T float): the
+// values as they are, to plane `part`.  fetched: the residual is on its way already.  Rows are
+// swizzled in shared memory, so that neither side has bank conflicts; TMA writes whole lines.
+template <class T, class Get, class Bias>
+__device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, long long row0, long long col0, int part,
+                                           Warp &w, bool fetched, Get &&get, Bias &&bias) {
   constexpr bool Fast = sizeof(T) == 2;
-  constexpr int U = 16 / int(sizeof(T)), W = RB / int(sizeof(T)), N = W < 32 ? W : 32;
+  constexpr int U = 16 / int(sizeof(T)), W = 128 / int(sizeof(T));
   using Un = Unit<T, U>;
   const int lane = threadIdx.x & 31;
-  unsigned char *mine = w.box + lane * RB;
-  const int swizzle = RB == 128 ? lane & 7 : (lane >> 1) & 3; // SWIZZLE_128B, SWIZZLE_64B
+  unsigned char *mine = w.box + lane * 128;
   const bool plain = part >= 0;
-  auto block = [&](int c, float (&v)[N]) {
+  auto block = [&](int c, float (&v)[32]) {
     get(c, v);
     if (plain || !e.bias)
       return;
-    const long long col = col0 + c + lane;
-    __syncwarp();
-    w.bias[lane] = lane < N && col < J ? to_float(static_cast<const T *>(e.bias)[col]) : 0.f;
-    __syncwarp();
+    const float b = bias(c);
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      const float4 b = *reinterpret_cast<const float4 *>(w.bias + k);
-      v[k] += b.x, v[k + 1] += b.y, v[k + 2] += b.z, v[k + 3] += b.w;
-    }
+    for (int i = 0; i < 32; ++i)
+      v[i] += __shfl_sync(0xffffffffu, b, i);
   };
-  auto free_box = [&] { // the box's last store has read it
+  auto free_box = [&] { // its last store has read it
     if (lane == 0)
       tc::bulk_wait_read();
     __syncwarp();
@@ -116,66 +116,63 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
   if (!plain && e.z) {
     free_box();
 #pragma unroll
-    for (int c = 0; c < W; c += N) {
-      float v[N];
+    for (int c = 0; c < W; c += 32) {
+      float v[32];
       block(c, v);
 #pragma unroll
-      for (int k = 0; k < N; k += U) {
+      for (int i = 0; i < 32; i += U) {
         Un o;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          o.v[u] = from_float<T>(v[k + u]);
-        *reinterpret_cast<Un *>(mine + ((((c + k) / U) ^ swizzle) << 4)) = o;
+          o.v[u] = from_float<T>(v[i + u]);
+        *reinterpret_cast<Un *>(mine + ((((c + i) / U) ^ (lane & 7)) << 4)) = o;
       }
     }
     send(m.z, 0);
   }
-  free_box();
   const bool residual = !plain && e.residual;
-  if (residual && lane == 0) {
-    tc::mbar_expect_tx(w.bar, 32 * RB);
-    tc::tma_load_3d(tc::smem_u32(w.box), &m.residual, int(col0), int(row0), 0, w.bar);
+  if (!fetched) {
+    free_box();
+    if (residual && lane == 0)
+      fetch_residual(m, w, row0, col0);
   }
+  bool there = true;
 #pragma unroll
-  for (int c = 0; c < W; c += N) {
-    float v[N];
+  for (int c = 0; c < W; c += 32) {
+    float v[32];
     block(c, v);
     if (!plain && e.activation != None)
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        v[k] = activate<Fast>(v[k], e.activation);
+      for (int i = 0; i < 32; ++i)
+        v[i] = activate<Fast>(v[i], e.activation);
     if (residual && c == 0) {
       const long long start = clock64();
-      bool there = false;
       while (!(there = tc::mbar_try(w.bar, w.phase)) && clock64() - start < tc::kWaitCycles) {
       }
       w.phase ^= 1;
-      if (!there) // shows as NaN
-        col0 = J;
     }
 #pragma unroll
-    for (int k = 0; k < N; k += U) {
-      Un *at = reinterpret_cast<Un *>(mine + ((((c + k) / U) ^ swizzle) << 4));
+    for (int i = 0; i < 32; i += U) {
+      Un *at = reinterpret_cast<Un *>(mine + ((((c + i) / U) ^ (lane & 7)) << 4));
       Un o;
       if (residual) {
         o = *at;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          v[k + u] += to_float(o.v[u]);
+        for (int u = 0; u < U; ++u) // a wait that ran out shows as NaN
+          v[i + u] = there ? v[i + u] + to_float(o.v[u]) : __uint_as_float(0x7fc00000u);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        o.v[u] = from_float<T>(v[k + u]);
+        o.v[u] = from_float<T>(v[i + u]);
       *at = o;
     }
   }
   send(m.y, plain ? part : 0);
 }
 
-// A warp's 32 x 32 block where rows allow no boxes: through 32 rows of 16 floats
-// (2 KiB, their columns permuted by row), so that
-// neighbouring lanes write neighbouring columns.  partial != NULL: the float values go to
-// partial[row * J + col] instead.
+// A warp's 32 x 32 block where rows allow no boxes: through 32 rows of 16 floats (their columns
+// permuted by row), so that neighbouring lanes write neighbouring columns.  partial != NULL: the
+// float values go to partial[row * J + col] instead.
 template <class T>
 __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
                                              long long row0, long long col0, float *v, float *stage) {
@@ -206,12 +203,12 @@ __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, 
 inline long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 // Tensor map of a [rows][cols] array of 16-bit or float elements with row distance ld, in boxes of
-// box_rows rows by box_bytes, swizzled by as much; elements outside the array read as zero.
+// box_rows rows by 128 bytes, SWIZZLE_128B; elements outside the array read as zero.
 // planes: a third dimension of `rows` rows each (0: a map of two dimensions).
 CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows,
-                     int planes = 0, int box_bytes = 128);
+                     int planes = 0);
 // The boxes of a product's results, or of its parts.
-Boxes boxes_of(const Product &, float *partial, int parts, int box_bytes);
+Boxes boxes_of(const Product &, float *partial, int parts);
 // Whether TMA can read the array in place: 16-byte aligned rows.
 inline bool tma_ready(int type, const void *p, long long rows, long long ld) {
   return aligned16(p) && (rows <= 1 || ld * bytes_of(type) % 16 == 0);
@@ -225,8 +222,8 @@ struct Plan {
 inline long long parts_workspace(const Plan &p, long long I, long long J) {
   return p.parts > 1 ? round_up(p.parts * I * J * 4, 16) : 0;
 }
-// The products of 16-bit types (dense_gemm16.cu; operands that TMA can read) and of floats
-// (dense_gemm32.cu; any operands).
+// The products of 16-bit types (dense_gemm16.cu) and of floats
+// (dense_gemm32.cu); the operands are as TMA can read them.
 Plan plan16(long long I, long long J, long long K);
 void product16(const Product &, void *workspace, cudaStream_t);
 Plan plan32(long long I, long long J, long long K);

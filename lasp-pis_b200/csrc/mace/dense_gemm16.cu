@@ -19,8 +19,7 @@ using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 320, kEpilogueThreads = 256;
 constexpr int kStageRing = 192 * 1024; // bytes of the operand ring
-constexpr int kBoxBytes = 32 * 128;
-constexpr int kSmem = 1024 + kStageRing + 8 * kBoxBytes + 8 * 128 + 256;
+constexpr int kSmem = 1024 + kStageRing + 8 * kBoxBytes + 256;
 static_assert(kSmem + 64 <= 232448, "shared memory budget");
 
 struct Gemm16 {
@@ -47,8 +46,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   constexpr int kTmemCols = 2 * BN;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *staging = smem + kStageRing; // a box per epilogue warp, then its bias
-  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes + 8 * 128);
+  unsigned char *staging = smem + kStageRing; // a box per epilogue warp
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes);
   // full[S] | empty[S] | tfull[2] | tfree[2] | done | residual[8]
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
     // Two warps per TMEM lane quadrant, each with half of the columns.
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int me = warp - 2;
-    Warp w{staging + me * kBoxBytes, reinterpret_cast<float *>(staging + 8 * kBoxBytes + me * 128), residual0 + 8 * me, 0};
+    Warp w{staging + me * kBoxBytes, residual0 + 8 * me, 0};
     bool ok = true;
     int tile = 0;
     for (long long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
@@ -170,6 +169,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
       const long long s = u / tiles.count;
       long long i, j;
       tiles.at(u - s * tiles.count, i, j);
+      // The lane's bias of this warp's columns, before the wait for the product.
+      float bias[BN / 64 < 2 ? 2 : BN / 64] = {};
+      if (g.e.bias)
+#pragma unroll
+        for (int k = 0; k < int(sizeof(bias) / 4); ++k) {
+          const long long col = j * BN + half * (BN / 2) + 32 * k + lane;
+          bias[k] = col < g.J ? to_float(static_cast<const T *>(g.e.bias)[col]) : 0.f;
+        }
       ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(tile / 2) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -189,15 +196,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
         if (g.boxes.on && g.partial) {
 #pragma unroll 1
           for (int c = first; c < end && j * BN + c < g.J; c += 32)
-            finish_box<float, 128>(g.e, g.boxes, g.J, row0, j * BN + c, int(s), w,
-                              [&](int k, float (&v)[32]) { get(c + k, v); });
-        } else if (g.boxes.on && BN >= 128) {
-#pragma unroll 1
-          for (int c = first; c < end && j * BN + c < g.J; c += 64)
-            finish_box<T, 128>(g.e, g.boxes, g.J, row0, j * BN + c, -1, w, [&](int k, float (&v)[32]) { get(c + k, v); });
-        } else if (g.boxes.on) { // one box per row quarter: the first of its two warps
-          if (!half)
-            finish_box<T, 128>(g.e, g.boxes, g.J, row0, j * BN, -1, w, get);
+            finish_box<float>(g.e, g.boxes, row0, j * BN + c, int(s), w, false,
+                              [&](int k, float (&v)[32]) { get(c + k, v); }, [](int) { return 0.f; });
+        } else if (g.boxes.on) {
+          // 64 columns to a box: where the tile has no more, the first of a quarter's two warps has it.
+          const int step = BN >= 128 ? 1 : 2;
+#pragma unroll
+          for (int x = 0; x < (BN + 127) / 128; ++x) {
+            const int c = first * step + 64 * x;
+            if (c < end && j * BN + c < g.J)
+              finish_box<T>(g.e, g.boxes, row0, j * BN + c, -1, w, false,
+                            [&](int k, float (&v)[32]) { get(c + k, v); },
+                            [&](int k) { return bias[2 * x + k / 32]; });
+          }
         } else {
           float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
 #pragma unroll 1
@@ -306,45 +317,44 @@ template <class T, int BN, bool PT, bool QT> void launch_gemm16(const Gemm16 &g,
 } // namespace
 
 CUtensorMap tile_map(int type, const void *base, long long rows, long long cols, long long ld, int box_rows,
-                     int planes, int box_bytes) {
+                     int planes) {
   const int b = bytes_of(type);
   if (rows <= 1)
     ld = round_up(cols, 16 / b);
   CUtensorMap map;
   cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(planes)};
   cuuint64_t strides[2] = {cuuint64_t(ld) * unsigned(b), cuuint64_t(ld) * cuuint64_t(rows) * unsigned(b)};
-  cuuint32_t box[3] = {cuuint32_t(box_bytes / b), cuuint32_t(box_rows), 1}, elem[3] = {1, 1, 1};
+  cuuint32_t box[3] = {cuuint32_t(128 / b), cuuint32_t(box_rows), 1}, elem[3] = {1, 1, 1};
   CUresult r = encoder()(&map,
                          type == F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                          : type == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                          planes ? 3 : 2, const_cast<void *>(base), dims, strides, box, elem,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     throw lapis::Error("cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
   return map;
 }
 
-Boxes boxes_of(const Product &p, float *partial, int parts, int box_bytes) {
+Boxes boxes_of(const Product &p, float *partial, int parts) {
   Boxes b{};
   const Epilogue &e = p.e;
   if (partial) {
     b.on = p.J % 4 == 0;
     if (b.on)
-      b.y = tile_map(F32, partial, p.I, p.J, p.J, 32, parts, box_bytes);
+      b.y = tile_map(F32, partial, p.I, p.J, p.J, 32, parts);
     return b;
   }
   b.on = tma_ready(p.type, e.out, p.I, e.ldo) && (!e.z || tma_ready(p.type, e.z, p.I, e.ldz)) &&
          (!e.residual || tma_ready(p.type, e.residual, p.I, e.ldr));
   if (!b.on)
     return b;
-  b.y = tile_map(p.type, e.out, p.I, p.J, e.ldo, 32, 1, box_bytes);
+  b.y = tile_map(p.type, e.out, p.I, p.J, e.ldo, 32, 1);
   if (e.z)
-    b.z = tile_map(p.type, e.z, p.I, p.J, e.ldz, 32, 1, box_bytes);
+    b.z = tile_map(p.type, e.z, p.I, p.J, e.ldz, 32, 1);
   if (e.residual)
-    b.residual = tile_map(p.type, e.residual, p.I, p.J, e.ldr, 32, 1, box_bytes);
+    b.residual = tile_map(p.type, e.residual, p.I, p.J, e.ldr, 32, 1);
   return b;
 }
 
@@ -364,7 +374,7 @@ void product16(const Product &p, void *workspace, cudaStream_t stream) {
   g.idesc = idesc_f16(kBM, plan.bn) | format << 7 | format << 10 | uint32_t(p.p.turned) << 15 | uint32_t(p.q.turned) << 16;
   g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
   g.e = p.e;
-  g.boxes = boxes_of(p, g.partial, plan.parts, 128);
+  g.boxes = boxes_of(p, g.partial, plan.parts);
   auto run = [&](auto tag) {
     using T = decltype(tag);
     auto width = [&](auto bn) {

@@ -11,13 +11,16 @@
 // must not add up over long k.  A slab's result is first moved one ulp away from zero, which
 // cancels the mean of that truncation (the same measure as in tc_gemm.cu).
 //
-// Operands are read by plain coalesced loads, so any row distance and alignment will do, and the
-// split turns a [K][I] operand for free: the slab in shared memory is always k-major.  16 warps (128
-// registers each; a 17th for the MMAs would leave 96 and spill):
-//   0..7    load and split: four for P, four for Q; the loads of the next slab are issued as the
-//           registers of this one are split.  Warp 0 also issues the MMAs of a slab, after its
-//           own part of the next one, when the other warps' parts are long there.
-//   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each
+// TMA brings the slab's floats into the place of the split (128 rows of 64 floats are as large as two
+// fp16 planes), whichever index is contiguous; the split reads a row per thread and leaves it k-major,
+// hi over the first half and lo over the second.  16 warps, 128 registers each:
+//   0..7    split, a row per thread: four warps P, four Q (two in 64-wide tiles).  The warp that
+//           finishes a slab last issues its MMAs.
+//   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
+//           epilogue.  A slab that has reached TMEM has left its stage: warp 8 then starts the
+//           loads of the slab three ahead.
+// (Loading by plain loads straight into the registers of the split was 5 times slower: the loads of
+// 64 KB per slab stalled the split warps.)
 // Infinities and NaN make every result of their row (of P or Q) NaN in this scheme; results that
 // are not finite are summed again, one product at a time.
 #include "dense_gemm.cuh"
@@ -27,17 +30,17 @@ namespace op {
 namespace {
 using namespace tc;
 constexpr int kBM = 128, kBK = 64, kStages = 3;
-constexpr int kThreads = 512, kSplitThreads = 256, kDrainThreads = 256;
+constexpr int kThreads = 512, kDrainThreads = 256;
 // The split of slab g runs after the MMAs of g - 3, which waited for the drain of g - 5.
 constexpr int kSlots = 6;
-constexpr int kBoxBytes = 32 * 64; // a third stage leaves room for no more
 template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2; }
 template <int BN> constexpr int smem_bytes() {
-  return 1024 + kStages * stage_bytes<BN>() + 8 * kBoxBytes + 8 * 128 + kSlots * (kBM + BN) * 4 + 256;
+  return 1024 + kStages * stage_bytes<BN>() + 8 * kBoxBytes + kSlots * (kBM + BN) + 256;
 }
-static_assert(smem_bytes<128>() + 64 <= 232448, "shared memory budget");
+static_assert(smem_bytes<128>() + 128 <= 232448, "shared memory budget");
 
 struct Gemm32 {
+  CUtensorMap mp, mq;
   long long I, J, K;
   const float *p, *q;
   long long ldp, ldq;
@@ -56,37 +59,20 @@ __device__ __forceinline__ int split_power(uint32_t bits) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// Two neighbouring values: hi and lo halves.
-__device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &hi, uint32_t &lo) {
-  a *= scale, b *= scale;
-  __half2 h = __floats2half2_rn(a, b);
-  float2 f = __half22float2(h);
-  __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-  hi = *reinterpret_cast<uint32_t *>(&h);
-  lo = *reinterpret_cast<uint32_t *>(&l);
-}
-
-// Predicated loads that leave zero where they are off.  Written out, so that each lands in its own
-// register and none waits for another: a load under a branch is waited for where the branches join,
-// and a second load into the same register waits for the first even if only one of them is on.
-__device__ __forceinline__ float load_if(const float *p, bool on) {
-  float v;
-  asm volatile("{\n\t.reg .pred a;\n\tsetp.ne.u32 a, %2, 0;\n\tmov.b32 %0, 0;\n\t@a ld.global.nc.f32 %0, [%1];\n\t}"
-               : "=f"(v)
-               : "l"(p), "r"(unsigned(on)));
-  return v;
-}
-__device__ __forceinline__ void load_pair_if(const float *p, bool on, float &x, float &y) {
-  asm volatile("{\n\t.reg .pred a;\n\tsetp.ne.u32 a, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
-               "@a ld.global.nc.v2.f32 {%0, %1}, [%2];\n\t}"
-               : "=f"(x), "=f"(y)
-               : "l"(p), "r"(unsigned(on)));
+// Two neighbouring values: hi and lo halves (the remainder v 2^e - hi is exact).
+__device__ __forceinline__ void split2(float2 v, float2 scale, uint32_t &hi, uint32_t &lo) {
+  const float2 x = __fmul2_rn(v, scale);
+  const __half2 h = __float22half2_rn(x);
+  const __half2 l = __float22half2_rn(__ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x));
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
 // The walk over (tile, slab): the same for all warps.
 struct Walk {
   long long u, units, tiles;
   int k, end, slabs, parts;
+  Walk() = default;
   __device__ Walk(const Gemm32 &g, const Tiles &t)
       : u(blockIdx.x), units(t.count * g.parts), tiles(t.count), k(0), end(0), slabs(g.slabs), parts(g.parts) {
     open();
@@ -107,94 +93,55 @@ struct Walk {
   }
 };
 
-// 16 rows of an operand's slab in a warp's registers, 32 values per lane.  k-major: lane = two
-// neighbouring k, v[2 r], v[2 r + 1] of row r; a row's largest magnitude by one warp reduction.
-// Turned: lane = row lane % 16 and half of the slab's k, v[k].  A warp keeps two batches: one is
-// split while the other's loads are in flight, and each batch's loads are issued together (loads
-// interleaved with the split would share the few scoreboards that it waits on: 9x slower).
-template <bool Turned> struct Batch {
-  float v[32];
-  __device__ __forceinline__ void load(const float *base, long long ld, bool pairs, long long row0, long long rows,
-                                       long long k0, long long K) {
-    const int lane = threadIdx.x & 31;
-    if (Turned) {
-      const long long row = row0 + (lane & 15), kf = k0 + 32 * (lane >> 4);
-      const float *p = base + kf * ld + row;
-      const int most = row < rows ? int(min(32ll, max(0ll, K - kf))) : 0;
+// Splits row r of an operand's slab (ROWS rows, floats at `base`) in place.  k-major: two boxes of
+// ROWS rows by 32 k; a thread's row is its own.  Turned: boxes of 64 k by 32 rows; the rows of a box
+// are read by a warp's lanes together, and all of the operand's threads have read before any
+// writes (named barrier `id` of ROWS threads).  Returns the power of two that scales back, biased.
+template <int ROWS, bool Turned>
+__device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id) {
+  float v[64];
+  if (Turned) {
+    const unsigned char *box = base + (r >> 5) * 8192 + (r & 3) * 4;
+    const int chunk = r >> 2 & 7;
 #pragma unroll
-      for (int i = 0; i < 32; ++i, p += ld)
-        v[i] = load_if(p, i < most);
-    } else {
-      const long long k = k0 + 2 * lane;
-      const float *p = base + row0 * ld + k;
-      const int most = int(min(16ll, max(0ll, rows - row0)));
-      if (pairs) {
+    for (int k = 0; k < 64; ++k)
+      v[k] = *reinterpret_cast<const float *>(box + k * 128 + ((chunk ^ (k & 7)) << 4));
+  } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r, p += ld)
-          load_pair_if(p, k < K && r < most, v[2 * r], v[2 * r + 1]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r, p += ld) {
-          v[2 * r] = load_if(p, k < K && r < most);
-          v[2 * r + 1] = load_if(p + 1, k + 1 < K && r < most);
-        }
-      }
+    for (int c = 0; c < 16; ++c) {
+      const float4 x = *reinterpret_cast<const float4 *>(base + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
     }
   }
-  // Splits into hi and lo (k-major, SWIZZLE_128B; the batch's first row at `row` of the tile) and
-  // writes the rows' 2^-e.
-  __device__ __forceinline__ void split(unsigned char *hi, unsigned char *lo, int row, float *unscale) {
-    const int lane = threadIdx.x & 31;
-    if (Turned) {
-      uint32_t m[8];
+  uint32_t m[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        m[k] = magnitude(v[k]);
+  for (int k = 0; k < 8; ++k)
+    m[k] = magnitude(v[k]);
 #pragma unroll
-      for (int k = 8; k < 32; ++k)
-        m[k & 7] = max(m[k & 7], magnitude(v[k]));
+  for (int k = 8; k < 64; ++k)
+    m[k & 7] = max(m[k & 7], magnitude(v[k]));
 #pragma unroll
-      for (int w = 4; w; w >>= 1)
+  for (int w = 4; w; w >>= 1)
 #pragma unroll
-        for (int j = 0; j < w; ++j)
-          m[j] = max(m[j], m[j + w]);
-      const int e = split_power(max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 16))), r = row + (lane & 15);
-      const float scale = pow2(e);
+    for (int j = 0; j < w; ++j)
+      m[j] = max(m[j], m[j + w]);
+  const int e = split_power(m[0]);
+  const float2 scale = make_float2(pow2(e), pow2(e));
+  if (Turned)
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(ROWS) : "memory");
+  unsigned char *hi = base + r * 128, *lo = hi + ROWS * 128;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t h[4], l[4];
+  for (int c = 0; c < 8; ++c) {
+    uint32_t h[4], l[4];
 #pragma unroll
-        for (int p = 0; p < 4; ++p)
-          split2(v[8 * c + 2 * p], v[8 * c + 2 * p + 1], scale, h[p], l[p]);
-        const int at = r * 128 + (((c + 4 * (lane >> 4)) ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4 *>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-      }
-      if (lane < 16)
-        unscale[r] = pow2(-e);
-    } else {
-      // All maxima before the first of them is used: the reductions' latencies overlap.
-      uint32_t m[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        m[r] = __reduce_max_sync(0xffffffffu, max(magnitude(v[2 * r]), magnitude(v[2 * r + 1])));
-      float mine = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int e = split_power(m[r]);
-        uint32_t h, l;
-        split2(v[2 * r], v[2 * r + 1], pow2(e), h, l);
-        const int at = (row + r) * 128 + (((lane >> 2) ^ ((row + r) & 7)) << 4) + ((lane & 3) << 2);
-        *reinterpret_cast<uint32_t *>(hi + at) = h;
-        *reinterpret_cast<uint32_t *>(lo + at) = l;
-        if (lane == r)
-          mine = pow2(-e);
-      }
-      if (lane < 16)
-        unscale[row + lane] = mine;
-    }
+    for (int p = 0; p < 4; ++p)
+      split2(make_float2(v[8 * c + 2 * p], v[8 * c + 2 * p + 1]), scale, h[p], l[p]);
+    const int at = (c ^ (r & 7)) << 4;
+    *reinterpret_cast<uint4 *>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
-};
+  return unsigned(127 - e);
+}
 
 // sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time; ends early at NaN.
 __device__ __noinline__ float plain_sum(const float *p, long long pk, const float *q, long long qk, long long k0,
@@ -222,30 +169,29 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   constexpr int kTmemCols = 2 * BN;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *staging = smem + kStages * kStageBytes; // a box per drain warp, then its bias
-  float *scales = reinterpret_cast<float *>(staging + 8 * kBoxBytes + 8 * 128); // [kSlots][kBM + BN]: 2^-e of P's rows, then of Q's
+  unsigned char *staging = smem + kStages * kStageBytes; // a box per drain warp
+  unsigned char *scales = staging + 8 * kBoxBytes;       // [kSlots][kBM + BN]: 127 - e of P's rows, then of Q's
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kSlots * (kBM + BN));
-  // ready[S] | empty[S] | tfull[2] | tfree[2] | done | scaled[kSlots] | residual[8]
+  // full[S] | tfull[2] | tfree[2] | scaled[kSlots] | residual[8]
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
-  __shared__ int mma_done_issued;
+  __shared__ int arrived[kSlots]; // split warps that are through with a slab
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned ready0 = smem_u32(bars), empty0 = ready0 + 8 * kStages, tfull0 = empty0 + 8 * kStages,
-                 tfree0 = tfull0 + 16, done = tfree0 + 16, scaled0 = done + 8, residual0 = scaled0 + 8 * kSlots;
+  const unsigned full0 = smem_u32(bars), tfull0 = full0 + 8 * kStages, tfree0 = tfull0 + 16, scaled0 = tfree0 + 16,
+                 residual0 = scaled0 + 8 * kSlots;
+  constexpr int kSplitWarps = 4 + BN / 32;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    mma_done_issued = 0;
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(ready0 + 8 * s, kSplitThreads);
-      mbar_init(empty0 + 8 * s, 1);
-    }
+    for (int s = 0; s < kStages; ++s)
+      mbar_init(full0 + 8 * s, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull0 + 8 * b, 1);
       mbar_init(tfree0 + 8 * b, kDrainThreads);
     }
-    mbar_init(done, 1);
-    for (int x = 0; x < kSlots; ++x)
-      mbar_init(scaled0 + 8 * x, 8);
+    for (int x = 0; x < kSlots; ++x) {
+      mbar_init(scaled0 + 8 * x, kSplitWarps);
+      arrived[x] = 0;
+    }
     for (int x = 0; x < 8; ++x)
       mbar_init(residual0 + 8 * x, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -264,12 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
 
   // The MMAs of slab n (one thread).
   auto multiply = [&](int n) {
-    const int st = n % kStages, b = n & 1;
-    if (!mbar_wait(ready0 + 8 * st, unsigned(n / kStages) & 1, &abort_flag) ||
-        (n >= 2 && !mbar_wait(tfree0 + 8 * b, unsigned(n / 2 - 1) & 1, &abort_flag)))
-      return false;
+    const int b = n & 1;
+    if (n >= 2 && !mbar_wait(tfree0 + 8 * b, unsigned(n / 2 - 1) & 1, &abort_flag))
+      return;
     tc_fence_after();
-    const unsigned ph = smem_u32(smem + st * kStageBytes), pl = ph + kPBytes, qh = pl + kPBytes, ql = qh + kQBytes;
+    const unsigned ph = smem_u32(smem + n % kStages * kStageBytes), pl = ph + kPBytes, qh = pl + kPBytes, ql = qh + kQBytes;
     const uint32_t d = tmem + uint32_t(b * BN);
 #pragma unroll
     for (int m = 0; m < kBK / 16; ++m) { // the small terms first
@@ -279,92 +224,79 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
 #pragma unroll
     for (int m = 0; m < kBK / 16; ++m)
       umma_f16_desc(d, smem_desc(ph + 32 * m), smem_desc(qh + 32 * m), g.idesc, 1u);
-    umma_commit(empty0 + 8 * st);
     umma_commit(tfull0 + 8 * b);
-    return true;
   };
-  // A split warp: `high` (16 or 32) rows of every tile's P or Q from row `first` of the tile.
-  auto split_warp = [&](auto turned, auto high, int first, bool of_q) {
-    constexpr bool Turned = decltype(turned)::value;
-    constexpr int kHigh = decltype(high)::value;
-    const float *base = of_q ? g.q : g.p;
-    const long long ld = of_q ? g.ldq : g.ldp, rows = of_q ? g.J : g.I;
-    // 8-byte loads: aligned, and none crosses the end of a row.
-    const bool pairs = reinterpret_cast<uintptr_t>(base) % 8 == 0 && (rows <= 1 || ld % 2 == 0) && g.K % 2 == 0;
-    Batch<Turned> batch[2];
-    // The walk of the loads, and the first row of its tile; it leads by the two batches.
-    Walk ahead(g, tiles);
-    long long row0 = 0, row_u = -1;
-    auto load = [&](Batch<Turned> &b, int row) {
-      if (!ahead.live())
-        return;
-      if (ahead.u != row_u) {
-        long long i, j;
-        tiles.at(ahead.u % tiles.count, i, j);
-        row0 = (of_q ? j * BN : i * kBM) + first;
-        row_u = ahead.u;
-      }
-      b.load(base, ld, pairs, row0 + row, rows, (long long)ahead.k * kBK, g.K);
-      if (row + 16 == kHigh)
-        ahead.next();
-    };
-    load(batch[0], 0);
-    load(batch[1], kHigh == 32 ? 16 : 0);
-    bool ok = true, issued = true; // ok: the same in the whole warp
-    int n = 0;
-    auto slab = [&](auto one) { // slab n from both batches (32 rows) or from batch[one]
-      const int st = n % kStages;
-      ok = issued && (n < kStages || mbar_wait(empty0 + 8 * st, unsigned(n / kStages - 1) & 1, &abort_flag));
-      if (!(ok = __all_sync(0xffffffffu, ok)))
-        return;
-      unsigned char *hi = smem + st * kStageBytes + (of_q ? 2 * kPBytes : 0), *lo = hi + (of_q ? kQBytes : kPBytes);
-      float *unscale = scales + n % kSlots * (kBM + BN) + (of_q ? kBM : 0);
-      if (kHigh == 32) {
-        batch[0].split(hi, lo, first, unscale);
-        load(batch[0], 0);
-        batch[1].split(hi, lo, first + 16, unscale);
-        load(batch[1], 16);
-      } else {
-        constexpr int k = decltype(one)::value;
-        batch[k].split(hi, lo, first, unscale);
-        load(batch[k], 0);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(ready0 + 8 * st);
-      __syncwarp();
-      if (lane == 0) // this warp's scales, for the drain
-        mbar_arrive(scaled0 + 8 * (n % kSlots));
-      if (warp == 0 && lane == 0 && n)
-        issued = multiply(n - 1);
-      ++n;
-    };
-    Walk w(g, tiles);
-    while (w.live() && ok) {
-      slab(std::integral_constant<int, 0>{});
-      w.next();
-      if (kHigh == 16 && w.live() && ok) {
-        slab(std::integral_constant<int, 1>{});
-        w.next();
-      }
+  // The loads of slab n at walk w (one thread; the MMAs of slab n - 3 are done).
+  auto fetch = [&](int n, const Walk &w) {
+    long long i, j;
+    tiles.at(w.u % tiles.count, i, j);
+    const int i0 = int(i * kBM), j0 = int(j * BN), k0 = w.k * kBK;
+    const unsigned base = smem_u32(smem + n % kStages * kStageBytes), full = full0 + 8 * (n % kStages);
+    mbar_expect_tx(full, kStageBytes);
+    if (PT) {
+#pragma unroll
+      for (int h = 0; h < kBM / 32; ++h)
+        tma_load_2d(base + 8192 * h, &g.mp, i0 + 32 * h, k0, full);
+    } else {
+      tma_load_2d(base, &g.mp, k0, i0, full);
+      tma_load_2d(base + kPBytes, &g.mp, k0 + 32, i0, full);
     }
-    if (warp == 0 && lane == 0) {
-      if (ok && issued && n)
-        multiply(n - 1);
-      umma_commit(done);
-      mma_done_issued = 1;
+    if (QT) {
+#pragma unroll
+      for (int h = 0; h < BN / 32; ++h)
+        tma_load_2d(base + 2 * kPBytes + 8192 * h, &g.mq, j0 + 32 * h, k0, full);
+    } else {
+      tma_load_2d(base + 2 * kPBytes, &g.mq, k0, j0, full);
+      tma_load_2d(base + 2 * kPBytes + kQBytes, &g.mq, k0 + 32, j0, full);
     }
   };
 
-  using std::integral_constant;
-  if (warp < 4)
-    split_warp(integral_constant<bool, PT>{}, integral_constant<int, 32>{}, 32 * warp, false);
-  else if (warp < 8)
-    split_warp(integral_constant<bool, QT>{}, integral_constant<int, BN / 4>{}, BN / 4 * (warp - 4), true);
-  else {
+  if (warp < kSplitWarps) {
+    const bool of_q = warp >= 4;
+    const int r = threadIdx.x & 127;
+    bool ok = true; // the same in the whole warp
+    int n = 0;
+    for (Walk w(g, tiles); w.live(); w.next(), ++n) {
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &abort_flag));
+      if (!ok) { // the other warps of the operand may wait at this slab's barrier
+        if (of_q ? QT : PT)
+          asm volatile("bar.sync %0, %1;" ::"r"(of_q ? 2 : 1), "r"(of_q ? BN : kBM) : "memory");
+        continue;
+      }
+      unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * (kBM + BN);
+      if (of_q)
+        scale[kBM + r] = static_cast<unsigned char>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2));
+      else
+        scale[r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1));
+      // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
+      // last to arrive sees all of them.
+      fence_proxy_async_smem();
+      __threadfence_block();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
+        if (atomicAdd(&arrived[n % kSlots], 1) == kSplitWarps - 1) {
+          arrived[n % kSlots] = 0;
+          __threadfence_block();
+          fence_proxy_async_smem();
+          multiply(n);
+        }
+      }
+    }
+  } else if (warp >= 8) {
     constexpr int kCols = BN / 2;
     const int quarter = warp & 3, half = (warp - 8) >> 2;
     const int me = warp - 8;
-    Warp box{staging + me * kBoxBytes, reinterpret_cast<float *>(staging + 8 * kBoxBytes + me * 128), residual0 + 8 * me, 0};
+    Warp box{staging + me * kBoxBytes, residual0 + 8 * me, 0};
+    // The residual of a tile's first box is on its way while the tile accumulates (a kept z needs the
+    // box first).
+    const bool early = g.boxes.on && !g.partial && g.e.residual && !g.e.z;
+    __shared__ Walk ahead; // of the loads: warp 8's first lane
+    if (me == 0 && lane == 0) {
+      ahead = Walk(g, tiles);
+      for (int x = 0; x < kStages && ahead.live(); ++x, ahead.next())
+        fetch(x, ahead);
+    }
     float acc[kCols];
     bool ok = true;
     int n = 0;
@@ -373,6 +305,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       const long long k0 = (long long)w.k * kBK, k1 = min(g.K, (long long)w.end * kBK);
       long long i, j;
       tiles.at(u - s * tiles.count, i, j);
+      const long long row0 = i * kBM + 32 * quarter, row = row0 + lane, cols0 = j * BN + half * kCols;
+      const bool any = row0 < g.I && cols0 < g.J;
+      float bias[kCols / 32];
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c)
+        bias[c] = g.e.bias && cols0 + 32 * c + lane < g.J ? static_cast<const float *>(g.e.bias)[cols0 + 32 * c + lane] : 0.f;
+      if (early && any && lane == 0) {
+        bulk_wait_read();
+        fetch_residual(g.boxes, box, row0, cols0);
+      }
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
         acc[c] = 0.f;
@@ -383,10 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
           continue;
+        if (me == 0 && lane == 0 && ahead.live()) {
+          fetch(n + kStages, ahead);
+          ahead.next();
+        }
         tc_fence_after();
-        const float *scale = scales + n % kSlots * (kBM + BN);
-        const float fp = scale[32 * quarter + lane];
-        const float *fq = scale + kBM + half * kCols;
+        const unsigned char *scale = scales + n % kSlots * (kBM + BN);
+        const float fp = __uint_as_float(uint32_t(scale[32 * quarter + lane]) << 23);
+        const unsigned char *fq = scale + kBM + half * kCols;
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32) {
           uint32_t r[32];
@@ -399,24 +345,27 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           }
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(fq + c0 + c);
-            const float fs[4] = {f.x, f.y, f.z, f.w};
+            const uint32_t f = *reinterpret_cast<const uint32_t *>(fq + c0 + c);
+            float x[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const uint32_t bits = r[c + x];
-              // One ulp away from zero (not zero itself, infinities and NaN); then the two exact
-              // scalings.
-              const uint32_t away = bits + ((bits << 1) - 1u < 0xfeffffffu);
-              acc[c0 + c + x] = fmaf(__uint_as_float(away) * fs[x], fp, acc[c0 + c + x]);
+            for (int y = 0; y < 4; ++y) { // one ulp away from zero (not zero itself, infinities and NaN)
+              const uint32_t bits = r[c + y];
+              x[y] = __uint_as_float(bits + ((bits << 1) - 1u < 0xfeffffffu));
+            }
+#pragma unroll
+            for (int y = 0; y < 4; y += 2) { // the two exact scalings, and the float sum
+              const float2 s = make_float2(__uint_as_float((f >> 8 * y & 0xffu) << 23), __uint_as_float((f >> 8 * (y + 1) & 0xffu) << 23));
+              const float2 a = __ffma2_rn(__fmul2_rn(make_float2(x[y], x[y + 1]), s), make_float2(fp, fp),
+                                          make_float2(acc[c0 + c + y], acc[c0 + c + y + 1]));
+              acc[c0 + c + y] = a.x, acc[c0 + c + y + 1] = a.y;
             }
           }
         }
       }
       float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
-      const long long row0 = i * kBM + 32 * quarter, row = row0 + lane;
 #pragma unroll
       for (int c0 = 0; c0 < kCols; c0 += 32) {
-        const long long col0 = j * BN + half * kCols + c0;
+        const long long col0 = cols0 + c0;
         if (row0 >= g.I || col0 >= g.J)
           continue;
         bool odd = false;
@@ -441,16 +390,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           }
         }
         if (g.boxes.on)
+          finish_box<float>(
+              g.e, g.boxes, row0, col0, g.partial ? int(s) : -1, box, early && c0 == 0,
+              [&](int, float (&v)[32]) {
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            if (col0 + h < g.J)
-              finish_box<float, 64>(g.e, g.boxes, g.J, row0, col0 + h, g.partial ? int(s) : -1, box,
-                                    [&](int, float (&v)[16]) {
-#pragma unroll
-                                      for (int c = 0; c < 16; ++c)
-                                        v[c] = acc[c0 + h + c];
-                                    });
-          }
+                for (int c = 0; c < 32; ++c)
+                  v[c] = acc[c0 + c];
+              },
+              [&](int) { return bias[c0 / 32]; });
         else
           finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, reinterpret_cast<float *>(box.box));
       }
@@ -461,9 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
-    if (abort_flag && mma_done_issued) { // bounded wait for the MMAs in flight before TMEM goes
+    if (abort_flag) { // bounded pause for copies and MMAs in flight before TMEM and the CTA go
       long long start = clock64();
-      while (!mbar_try(done, 0) && clock64() - start < kWaitCycles) {
+      while (clock64() - start < kWaitCycles / 100) {
       }
     }
     tc_fence_after();
@@ -498,13 +445,18 @@ Plan plan32(long long I, long long J, long long K) {
 
 void product32(const Product &p, void *workspace, cudaStream_t stream) {
   const Plan plan = plan32(p.I, p.J, p.K);
-  Gemm32 g{p.I, p.J, p.K, static_cast<const float *>(p.p.p), static_cast<const float *>(p.q.p), p.p.ld, p.q.ld};
+  Gemm32 g{};
+  g.I = p.I, g.J = p.J, g.K = p.K;
+  g.p = static_cast<const float *>(p.p.p), g.ldp = p.p.ld;
+  g.q = static_cast<const float *>(p.q.p), g.ldq = p.q.ld;
+  g.mp = p.p.turned ? tile_map(F32, p.p.p, p.K, p.I, p.p.ld, kBK) : tile_map(F32, p.p.p, p.I, p.K, p.p.ld, kBM);
+  g.mq = p.q.turned ? tile_map(F32, p.q.p, p.K, p.J, p.q.ld, kBK) : tile_map(F32, p.q.p, p.J, p.K, p.q.ld, plan.bn);
   g.slabs = int((p.K + kBK - 1) / kBK);
   g.parts = plan.parts;
   g.idesc = idesc_f16(kBM, plan.bn);
   g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
   g.e = p.e;
-  g.boxes = boxes_of(p, g.partial, plan.parts, 64);
+  g.boxes = boxes_of(p, g.partial, plan.parts);
   auto width = [&](auto bn) {
     constexpr int BN = decltype(bn)::value;
     if (!p.p.turned && !p.q.turned)

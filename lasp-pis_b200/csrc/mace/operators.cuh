@@ -21,14 +21,15 @@ template <class T, int U> struct alignas(sizeof(T) * U) Unit {
   T v[U];
 };
 
-// 1 / (1 + exp(-z)).  16-bit results take the fast exponential and division (a few 2^-22 of the
-// value, far below their own rounding).
-template <bool Fast> __device__ __forceinline__ float sigmoid(float z) {
-  return Fast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+// 1 + exp(-z).  16-bit results take the fast exponential (2^-21 of the value and a little more for
+// large |z|, far below their own rounding).  The quotients below take the fast division (2 ulp): the
+// exact one branches for every value.
+template <bool Fast> __device__ __forceinline__ float exp_plus_one(float z) {
+  return 1.f + (Fast ? __expf(-z) : expf(-z));
 }
 template <bool Fast> __device__ __forceinline__ float activate(float z, int act) {
   if (act == Silu)
-    return Fast ? __fdividef(z, 1.f + __expf(-z)) : z / (1.f + expf(-z));
+    return __fdividef(z, exp_plus_one<Fast>(z));
   if (act == Gelu)
     return 0.5f * z * (1.f + erff(z * 0.70710678f));
   if (act == Relu)
@@ -38,7 +39,7 @@ template <bool Fast> __device__ __forceinline__ float activate(float z, int act)
 // d act / dz
 template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
   if (act == Silu) {
-    float s = sigmoid<Fast>(z);
+    float s = __fdividef(1.f, exp_plus_one<Fast>(z));
     return s * (1.f + z * (1.f - s));
   }
   if (act == Gelu) {
