@@ -141,10 +141,8 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
   for (int c = 0; c < W; c += 32) {
     float v[32];
     block(c, v);
-    if (!plain && e.activation != None)
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        v[i] = activate<Fast>(v[i], e.activation);
+    if (!plain)
+      activate_all<Fast>(v, e.activation);
     if (residual && c == 0) {
       const long long start = clock64();
       while (!(there = tc::mbar_try(w.bar, w.phase)) && clock64() - start < tc::kWaitCycles) {

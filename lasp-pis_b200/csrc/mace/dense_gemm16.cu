@@ -19,8 +19,8 @@ using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 320, kEpilogueThreads = 256;
 constexpr int kStageRing = 192 * 1024; // bytes of the operand ring
-constexpr int kSmem = 1024 + kStageRing + 8 * kBoxBytes + 256;
-static_assert(kSmem + 64 <= 232448, "shared memory budget");
+constexpr int kSmem = kStageRing + 8 * kBoxBytes + 256;
+static_assert(kSmem <= 232448, "shared memory budget");
 
 struct Gemm16 {
   CUtensorMap p, q;
@@ -44,14 +44,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   constexpr int kPBytes = kBM * kBK * 2, kQBytes = BN * kBK * 2, kStageBytes = kPBytes + kQBytes;
   constexpr int kStages = kStageRing / kStageBytes;
   constexpr int kTmemCols = 2 * BN;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *staging = smem + kStageRing; // a box per epilogue warp
   uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes);
   // full[S] | empty[S] | tfull[2] | tfree[2] | done | residual[8]
-  __shared__ uint32_t tmem_base;
-  __shared__ volatile int abort_flag;
-  __shared__ int mma_done_issued;
+  constexpr int kBars = 2 * kStages + 5 + 8;
+  static_assert(kBars * 8 + 12 <= 256, "barriers and state");
+  uint32_t &tmem_base = *reinterpret_cast<uint32_t *>(bars + kBars);
+  volatile int &abort_flag = *reinterpret_cast<volatile int *>(&tmem_base + 1);
+  int &mma_done_issued = *reinterpret_cast<int *>(&tmem_base + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, tfull0 = empty0 + 8 * kStages,
                  tfree0 = tfull0 + 16, done = tfree0 + 16, residual0 = done + 8;

@@ -8,8 +8,8 @@
 // rounded to nearest (22 significant bits for values down to 2^-18 of the largest).  A slab's
 // products lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22) accumulate fresh in TMEM, are scaled back
 // by the two exact powers of two and added to float registers: the tensor pipe truncates, which
-// must not add up over long k.  A slab's result is first moved one ulp away from zero, which
-// cancels the mean of that truncation (the same measure as in tc_gemm.cu).
+// must not add up over long k.  A slab's result comes out 8.7e-8 too small in the mean (tc_gemm.cu),
+// so three slabs of four are scaled by 1 + 2^-23: 8.9e-8.
 //
 // TMA brings the slab's floats into the place of the split (128 rows of 64 floats are as large as two
 // fp16 planes), whichever index is contiguous; the split reads a row per thread and leaves it k-major,
@@ -32,12 +32,12 @@ using namespace tc;
 constexpr int kBM = 128, kBK = 64, kStages = 3;
 constexpr int kThreads = 512, kDrainThreads = 256;
 // The split of slab g runs after the MMAs of g - 3, which waited for the drain of g - 5.
-constexpr int kSlots = 6;
+constexpr int kSlots = 5;
 template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2; }
 template <int BN> constexpr int smem_bytes() {
-  return 1024 + kStages * stage_bytes<BN>() + 8 * kBoxBytes + kSlots * (kBM + BN) + 256;
+  return kStages * stage_bytes<BN>() + 8 * kBoxBytes + kSlots * (kBM + 2 * BN) + 384;
 }
-static_assert(smem_bytes<128>() + 128 <= 232448, "shared memory budget");
+static_assert(smem_bytes<128>() <= 232448, "shared memory budget");
 
 struct Gemm32 {
   CUtensorMap mp, mq;
@@ -53,12 +53,11 @@ struct Gemm32 {
 
 // 2^e for the split of a row whose largest magnitude has these bits, e within normal powers.
 __device__ __forceinline__ int split_power(uint32_t bits) {
-  int ex = int(bits >> 23); // sign is clear
+  int ex = int(bits >> 23) & 0xff;
   int e = ex ? 141 - ex : (bits ? 126 : 0);
   return min(max(e, -126), 126);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 // Two neighbouring values: hi and lo halves (the remainder v 2^e - hi is exact).
 __device__ __forceinline__ void split2(float2 v, float2 scale, uint32_t &hi, uint32_t &lo) {
   const float2 x = __fmul2_rn(v, scale);
@@ -93,6 +92,14 @@ struct Walk {
   }
 };
 
+// The walk's state of the loads, and what the warps share.
+struct Shared {
+  Walk ahead;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+  int arrived[kSlots]; // split warps that are through with a slab
+};
+
 // Splits row r of an operand's slab (ROWS rows, floats at `base`) in place.  k-major: two boxes of
 // ROWS rows by 32 k; a thread's row is its own.  Turned: boxes of 64 k by 32 rows; the rows of a box
 // are read by a warp's lanes together, and all of the operand's threads have read before any
@@ -113,19 +120,20 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
       v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
     }
   }
-  uint32_t m[8];
+  // The largest magnitude; NaN does not count, and stays NaN in the split.
+  float m[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    m[k] = magnitude(v[k]);
+    m[k] = fabsf(v[k]);
 #pragma unroll
   for (int k = 8; k < 64; ++k)
-    m[k & 7] = max(m[k & 7], magnitude(v[k]));
+    m[k & 7] = fmaxf(m[k & 7], fabsf(v[k]));
 #pragma unroll
   for (int w = 4; w; w >>= 1)
 #pragma unroll
     for (int j = 0; j < w; ++j)
-      m[j] = max(m[j], m[j + w]);
-  const int e = split_power(m[0]);
+      m[j] = fmaxf(m[j], m[j + w]);
+  const int e = split_power(__float_as_uint(m[0]));
   const float2 scale = make_float2(pow2(e), pow2(e));
   if (Turned)
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(ROWS) : "memory");
@@ -167,15 +175,17 @@ template <int BN, bool PT, bool QT>
 __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_constant__ Gemm32 g) {
   constexpr int kPBytes = kBM * kBK * 2, kQBytes = BN * kBK * 2, kStageBytes = stage_bytes<BN>();
   constexpr int kTmemCols = 2 * BN;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *staging = smem + kStages * kStageBytes; // a box per drain warp
-  unsigned char *scales = staging + 8 * kBoxBytes;       // [kSlots][kBM + BN]: 127 - e of P's rows, then of Q's
-  uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kSlots * (kBM + BN));
+  // [kSlots][2 BN + kBM]: 2^-e of Q's rows (the upper halves of floats), then 127 - e of P's
+  unsigned char *scales = staging + 8 * kBoxBytes;
+  constexpr int kSlotBytes = 2 * BN + kBM;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kSlots * kSlotBytes);
   // full[S] | tfull[2] | tfree[2] | scaled[kSlots] | residual[8]
-  __shared__ uint32_t tmem_base;
-  __shared__ volatile int abort_flag;
-  __shared__ int arrived[kSlots]; // split warps that are through with a slab
+  constexpr int kBars = kStages + 4 + kSlots + 8;
+  static_assert(kBars * 8 + sizeof(Shared) <= 384, "barriers and state");
+  Shared &sh = *reinterpret_cast<Shared *>(bars + kBars);
+  volatile int &abort_flag = sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned full0 = smem_u32(bars), tfull0 = full0 + 8 * kStages, tfree0 = tfull0 + 16, scaled0 = tfree0 + 16,
                  residual0 = scaled0 + 8 * kSlots;
@@ -190,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     }
     for (int x = 0; x < kSlots; ++x) {
       mbar_init(scaled0 + 8 * x, kSplitWarps);
-      arrived[x] = 0;
+      sh.arrived[x] = 0;
     }
     for (int x = 0; x < 8; ++x)
       mbar_init(residual0 + 8 * x, 1);
@@ -198,20 +208,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     fence_proxy_async_smem();
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = sh.tmem_base;
   const Tiles tiles(g.I, g.J, kBM, BN);
 
   // The MMAs of slab n (one thread).
   auto multiply = [&](int n) {
     const int b = n & 1;
-    if (n >= 2 && !mbar_wait(tfree0 + 8 * b, unsigned(n / 2 - 1) & 1, &abort_flag))
+    if (n >= 2 && !mbar_wait(tfree0 + 8 * b, unsigned(n / 2 - 1) & 1, &sh.abort_flag))
       return;
     tc_fence_after();
     const unsigned ph = smem_u32(smem + n % kStages * kStageBytes), pl = ph + kPBytes, qh = pl + kPBytes, ql = qh + kQBytes;
@@ -257,17 +267,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     bool ok = true; // the same in the whole warp
     int n = 0;
     for (Walk w(g, tiles); w.live(); w.next(), ++n) {
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &abort_flag));
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
       if (!ok) { // the other warps of the operand may wait at this slab's barrier
         if (of_q ? QT : PT)
           asm volatile("bar.sync %0, %1;" ::"r"(of_q ? 2 : 1), "r"(of_q ? BN : kBM) : "memory");
         continue;
       }
-      unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * (kBM + BN);
+      unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
       if (of_q)
-        scale[kBM + r] = static_cast<unsigned char>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2));
+        reinterpret_cast<unsigned short *>(scale)[r] =
+            static_cast<unsigned short>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2) << 7);
       else
-        scale[r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1));
+        scale[2 * BN + r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1));
       // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
       // last to arrive sees all of them.
       fence_proxy_async_smem();
@@ -275,8 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
-        if (atomicAdd(&arrived[n % kSlots], 1) == kSplitWarps - 1) {
-          arrived[n % kSlots] = 0;
+        if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
+          sh.arrived[n % kSlots] = 0;
           __threadfence_block();
           fence_proxy_async_smem();
           multiply(n);
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     // The residual of a tile's first box is on its way while the tile accumulates (a kept z needs the
     // box first).
     const bool early = g.boxes.on && !g.partial && g.e.residual && !g.e.z;
-    __shared__ Walk ahead; // of the loads: warp 8's first lane
+    Walk &ahead = sh.ahead; // of the loads: warp 8's first lane
     if (me == 0 && lane == 0) {
       ahead = Walk(g, tiles);
       for (int x = 0; x < kStages && ahead.live(); ++x, ahead.next())
@@ -320,8 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         acc[c] = 0.f;
       for (; w.live() && w.u == u; w.next(), ++n) {
         const int b = n & 1;
-        ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(n / 2) & 1, &abort_flag) &&
-             mbar_wait(scaled0 + 8 * (n % kSlots), unsigned(n / kSlots) & 1, &abort_flag);
+        ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(n / 2) & 1, &sh.abort_flag) &&
+             mbar_wait(scaled0 + 8 * (n % kSlots), unsigned(n / kSlots) & 1, &sh.abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
           continue;
@@ -330,9 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           ahead.next();
         }
         tc_fence_after();
-        const unsigned char *scale = scales + n % kSlots * (kBM + BN);
-        const float fp = __uint_as_float(uint32_t(scale[32 * quarter + lane]) << 23);
-        const unsigned char *fq = scale + kBM + half * kCols;
+        const unsigned char *scale = scales + n % kSlots * kSlotBytes;
+        const unsigned char *fq = scale + 2 * (half * kCols);
+        // 2^-e of P's row, one ulp more in three slabs of four.
+        const float fp = __uint_as_float((uint32_t(scale[2 * BN + 32 * quarter + lane]) << 23) + ((n & 3) != 3));
+        const float2 fp2 = make_float2(fp, fp);
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32) {
           uint32_t r[32];
@@ -345,19 +358,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           }
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            const uint32_t f = *reinterpret_cast<const uint32_t *>(fq + c0 + c);
-            float x[4];
+            const uint2 f = *reinterpret_cast<const uint2 *>(fq + 2 * (c0 + c));
+            const uint32_t fs[2] = {f.x, f.y};
 #pragma unroll
-            for (int y = 0; y < 4; ++y) { // one ulp away from zero (not zero itself, infinities and NaN)
-              const uint32_t bits = r[c + y];
-              x[y] = __uint_as_float(bits + ((bits << 1) - 1u < 0xfeffffffu));
-            }
-#pragma unroll
-            for (int y = 0; y < 4; y += 2) { // the two exact scalings, and the float sum
-              const float2 s = make_float2(__uint_as_float((f >> 8 * y & 0xffu) << 23), __uint_as_float((f >> 8 * (y + 1) & 0xffu) << 23));
-              const float2 a = __ffma2_rn(__fmul2_rn(make_float2(x[y], x[y + 1]), s), make_float2(fp, fp),
-                                          make_float2(acc[c0 + c + y], acc[c0 + c + y + 1]));
-              acc[c0 + c + y] = a.x, acc[c0 + c + y + 1] = a.y;
+            for (int y = 0; y < 2; ++y) { // the two scalings, and the float sum
+              const int x = c0 + c + 2 * y;
+              const float2 s = make_float2(__uint_as_float(fs[y] << 16), __uint_as_float(fs[y] & 0xffff0000u));
+              const float2 a = __ffma2_rn(
+                  __fmul2_rn(make_float2(__uint_as_float(r[c + 2 * y]), __uint_as_float(r[c + 2 * y + 1])), s), fp2,
+                  make_float2(acc[x], acc[x + 1]));
+              acc[x] = a.x, acc[x + 1] = a.y;
             }
           }
         }

@@ -36,6 +36,22 @@ template <bool Fast> __device__ __forceinline__ float activate(float z, int act)
     return z < 0.f ? 0.f : z; // NaN stays
   return z;
 }
+// N values at once: one branch on the activation, so that the values' arithmetic interleaves.
+template <bool Fast, int N> __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
+  if (act == Silu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = activate<Fast>(v[i], Silu);
+  } else if (act == Gelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = activate<Fast>(v[i], Gelu);
+  } else if (act == Relu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = activate<Fast>(v[i], Relu);
+  }
+}
 // d act / dz
 template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
   if (act == Silu) {
