@@ -38,19 +38,26 @@ struct Product {
   Epilogue e;
 };
 
-// Output tiles in groups of kBand rows of tiles, column by column within a group: the tiles that
-// run together share their operands in L2.
+// Output tiles in bands of kBand rows of tiles, column by column within a band: the tiles that run
+// together share their operands in L2.  32-bit indices: products that large in memory have fewer
+// than 2^31 tiles and parts of tiles (checked on the host).
 struct Tiles {
-  long long nI, nJ, count;
-  __host__ __device__ Tiles(long long I, long long J, int bi, int bj)
-      : nI((I + bi - 1) / bi), nJ((J + bj - 1) / bj), count(nI * nJ) {}
-  __device__ __forceinline__ void at(long long t, long long &i, long long &j) const {
-    constexpr long long kBand = 16;
-    long long band = t / (kBand * nJ), first = band * kBand, rows = min(kBand, nI - first), r = t - first * nJ;
-    i = first + r % rows;
-    j = r / rows;
+  unsigned nI, nJ, count;
+  Tiles() = default;
+  Tiles(long long I, long long J, int bi, int bj)
+      : nI(unsigned((I + bi - 1) / bi)), nJ(unsigned((J + bj - 1) / bj)), count(nI * nJ) {}
+  __device__ __forceinline__ void at(unsigned t, long long &i, long long &j) const {
+    constexpr unsigned kBand = 16;
+    const unsigned band = t / (kBand * nJ), first = band * kBand, rows = min(kBand, nI - first), r = t - first * nJ;
+    const unsigned c = r / rows;
+    i = first + (r - c * rows);
+    j = c;
   }
 };
+inline void check_tiles(long long I, long long J, int bi, int bj, long long parts) {
+  if (double((I + bi - 1) / bi) * double((J + bj - 1) / bj) * double(parts) > 2e9)
+    throw lapis::Error("The product has too many tiles");
+}
 
 // One value of the product through the epilogue: z, then the output value.
 template <class T>
@@ -65,40 +72,54 @@ __device__ __forceinline__ void finish(const Epilogue &e, long long row, long lo
     v += to_float(static_cast<const T *>(e.residual)[row * e.ldr + col]);
   static_cast<T *>(e.out)[row * e.ldo + col] = from_float<T>(v);
 }
-// A warp's part of the epilogue: a box of 32 rows by 128 bytes in shared memory, and the mbarrier of
-// its residual.
+// A box of 32 rows by 128 bytes in shared memory, a warp's, and the mbarrier of its residual.
 constexpr int kBoxBytes = 32 * 128;
-struct Warp {
-  unsigned char *box; // 1024-byte aligned
-  unsigned bar, phase;
+struct Box {
+  unsigned char *at; // 1024-byte aligned
+  unsigned bar;
 };
 // Starts the load of a residual box (one lane; the box's last store has read it).
-__device__ __forceinline__ void fetch_residual(const Boxes &m, const Warp &w, long long row0, long long col0) {
+__device__ __forceinline__ void fetch_residual(const Boxes &m, const Box &w, long long row0, long long col0) {
   tc::mbar_expect_tx(w.bar, kBoxBytes);
-  tc::tma_load_3d(tc::smem_u32(w.box), &m.residual, int(col0), int(row0), 0, w.bar);
+  tc::tma_load_3d(tc::smem_u32(w.at), &m.residual, int(col0), int(row0), 0, w.bar);
+}
+
+// `count` (a multiple of 32) values of the bias from column col0 into a warp's shared memory.
+template <class T>
+__device__ __forceinline__ void fetch_bias(const Epilogue &e, long long J, long long col0, int count, T *to) {
+  if (!e.bias)
+    return;
+  __syncwarp();
+  for (int c = threadIdx.x & 31; c < count; c += 32)
+    to[c] = col0 + c < J ? static_cast<const T *>(e.bias)[col0 + c] : T(0.f);
+  __syncwarp();
 }
 
 // 32 rows by 128 bytes of the result from (row0, col0), rows = lanes.  get(c, v) gives the product's
-// columns col0 + c .. + 31, and bias(c) the lane's (col0 + c + lane) bias.  part >= 0 (T float): the
-// values as they are, to plane `part`.  fetched: the residual is on its way already.  Rows are
-// swizzled in shared memory, so that neither side has bank conflicts; TMA writes whole lines.
-template <class T, class Get, class Bias>
+// columns col0 + c .. + 31, bias their bias in shared memory.  part >= 0 (T float): the
+// values as they are, to plane `part`.  ready: the box's last store has read it, and the residual is on
+// its way; phase: of its barrier.  Rows are swizzled in shared memory, so that neither side has bank
+// conflicts; TMA writes whole lines.
+template <class T, class Get>
 __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, long long row0, long long col0, int part,
-                                           Warp &w, bool fetched, Get &&get, Bias &&bias) {
+                                           const Box &w, unsigned &phase, bool ready, const T *bias, Get &&get) {
   constexpr bool Fast = sizeof(T) == 2;
   constexpr int U = 16 / int(sizeof(T)), W = 128 / int(sizeof(T));
   using Un = Unit<T, U>;
   const int lane = threadIdx.x & 31;
-  unsigned char *mine = w.box + lane * 128;
+  unsigned char *mine = w.at + lane * 128;
   const bool plain = part >= 0;
   auto block = [&](int c, float (&v)[32]) {
     get(c, v);
     if (plain || !e.bias)
       return;
-    const float b = bias(c);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      v[i] += __shfl_sync(0xffffffffu, b, i);
+    for (int i = 0; i < 32; i += U) {
+      const Un b = *reinterpret_cast<const Un *>(bias + c + i);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[i + u] += to_float(b.v[u]);
+    }
   };
   auto free_box = [&] { // its last store has read it
     if (lane == 0)
@@ -109,7 +130,7 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
     tc::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tc::tma_store_3d(&map, tc::smem_u32(w.box), int(col0), int(row0), plane);
+      tc::tma_store_3d(&map, tc::smem_u32(w.at), int(col0), int(row0), plane);
       tc::bulk_commit();
     }
   };
@@ -131,7 +152,7 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
     send(m.z, 0);
   }
   const bool residual = !plain && e.residual;
-  if (!fetched) {
+  if (!ready) {
     free_box();
     if (residual && lane == 0)
       fetch_residual(m, w, row0, col0);
@@ -145,9 +166,9 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
       activate_all<Fast>(v, e.activation);
     if (residual && c == 0) {
       const long long start = clock64();
-      while (!(there = tc::mbar_try(w.bar, w.phase)) && clock64() - start < tc::kWaitCycles) {
+      while (!(there = tc::mbar_try(w.bar, phase)) && clock64() - start < tc::kWaitCycles) {
       }
-      w.phase ^= 1;
+      phase ^= 1;
     }
 #pragma unroll
     for (int i = 0; i < 32; i += U) {

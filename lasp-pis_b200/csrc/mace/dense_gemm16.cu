@@ -19,12 +19,15 @@ using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 320, kEpilogueThreads = 256;
 constexpr int kStageRing = 192 * 1024; // bytes of the operand ring
-constexpr int kSmem = kStageRing + 8 * kBoxBytes + 256;
+constexpr int kBiasBytes = 8 * 128 * 2; // each epilogue warp's columns
+constexpr int kSmem = kStageRing + 8 * kBoxBytes + kBiasBytes + 256;
 static_assert(kSmem <= 232448, "shared memory budget");
 
 struct Gemm16 {
   CUtensorMap p, q;
   long long I, J;
+  Tiles tiles;
+  unsigned units; // tiles x parts
   int slabs, parts, p_rows, q_rows; // rows of a k-major operand's boxes
   uint32_t idesc;
   float *partial;
@@ -45,8 +48,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   constexpr int kStages = kStageRing / kStageBytes;
   constexpr int kTmemCols = 2 * BN;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char *staging = smem + kStageRing; // a box per epilogue warp
-  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes);
+  unsigned char *staging = smem + kStageRing; // a box per epilogue warp, then its bias
+  uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 8 * kBoxBytes + kBiasBytes);
   // full[S] | empty[S] | tfull[2] | tfree[2] | done | residual[8]
   constexpr int kBars = 2 * kStages + 5 + 8;
   static_assert(kBars * 8 + 12 <= 256, "barriers and state");
@@ -82,18 +85,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  const Tiles tiles(g.I, g.J, kBM, BN);
-  const long long units = tiles.count * g.parts;
-  // Slabs [first, last) of part s.
-  auto first_slab = [&](long long s) { return int(s * g.slabs / g.parts); };
+  const Tiles &tiles = g.tiles;
+  const unsigned units = g.units;
+  // Unit u is part s = u / tiles of tile u % tiles: slabs [first_slab(s), first_slab(s + 1)).
+  auto first_slab = [&](unsigned s) { return g.parts > 1 ? int((long long)s * g.slabs / g.parts) : s ? g.slabs : 0; };
+  auto part_of = [&](unsigned u) { return g.parts > 1 ? u / tiles.count : 0u; };
 
   if (warp == 0) {
     if (lane == 0) {
-      long long n = 0;
+      unsigned n = 0;
       bool ok = true;
       const unsigned bytes = (PT ? kPBytes : g.p_rows * 128) + (QT ? kQBytes : g.q_rows * 128);
-      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        long long i, j, s = u / tiles.count;
+      for (unsigned u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const unsigned s = part_of(u);
+        long long i, j;
         tiles.at(u - s * tiles.count, i, j);
         const int i0 = int(i * kBM), j0 = int(j * BN);
         for (int k = first_slab(s), end = first_slab(s + 1); k < end; ++k, ++n) {
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
         }
       }
       if (!ok) // copies in flight end (bounded wait) before the CTA does
-        for (long long m = n > kStages ? n - kStages : 0; m < n; ++m) {
+        for (unsigned m = n > kStages ? n - kStages : 0; m < n; ++m) {
           long long start = clock64();
           while (!mbar_try(full0 + 8 * int(m % kStages), unsigned(m / kStages) & 1) && clock64() - start < kWaitCycles) {
           }
@@ -127,12 +132,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      long long n = 0;
+      unsigned n = 0;
       int tile = 0;
       bool ok = true;
-      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x, ++tile) {
+      for (unsigned u = blockIdx.x; u < units && ok; u += gridDim.x, ++tile) {
         const int b = tile & 1;
-        const long long s = u / tiles.count;
+        const unsigned s = part_of(u);
         const uint32_t d = tmem + uint32_t(b * BN);
         if (tile >= 2 && !(ok = mbar_wait(tfree0 + 8 * b, unsigned(tile / 2 - 1) & 1, &abort_flag)))
           break;
@@ -162,22 +167,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
     // Two warps per TMEM lane quadrant, each with half of the columns.
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int me = warp - 2;
-    Warp w{staging + me * kBoxBytes, residual0 + 8 * me, 0};
+    const Box w{staging + me * kBoxBytes, residual0 + 8 * me};
+    T *bias = reinterpret_cast<T *>(staging + 8 * kBoxBytes) + me * 128;
+    unsigned phase = 0;
     bool ok = true;
     int tile = 0;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
+    for (unsigned u = blockIdx.x; u < units; u += gridDim.x, ++tile) {
       const int b = tile & 1;
-      const long long s = u / tiles.count;
+      const unsigned s = part_of(u);
       long long i, j;
       tiles.at(u - s * tiles.count, i, j);
-      // The lane's bias of this warp's columns, before the wait for the product.
-      float bias[BN / 64 < 2 ? 2 : BN / 64] = {};
-      if (g.e.bias)
-#pragma unroll
-        for (int k = 0; k < int(sizeof(bias) / 4); ++k) {
-          const long long col = j * BN + half * (BN / 2) + 32 * k + lane;
-          bias[k] = col < g.J ? to_float(static_cast<const T *>(g.e.bias)[col]) : 0.f;
-        }
+      if (!g.partial)
+        fetch_bias<T>(g.e, g.J, j * BN + (BN >= 128 ? half * (BN / 2) : 0), BN >= 128 ? BN / 2 : 64, bias);
       ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(tile / 2) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -197,8 +198,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
         if (g.boxes.on && g.partial) {
 #pragma unroll 1
           for (int c = first; c < end && j * BN + c < g.J; c += 32)
-            finish_box<float>(g.e, g.boxes, row0, j * BN + c, int(s), w, false,
-                              [&](int k, float (&v)[32]) { get(c + k, v); }, [](int) { return 0.f; });
+            finish_box<float>(g.e, g.boxes, row0, j * BN + c, int(s), w, phase, false,
+                              nullptr, [&](int k, float (&v)[32]) { get(c + k, v); });
         } else if (g.boxes.on) {
           // 64 columns to a box: where the tile has no more, the first of a quarter's two warps has it.
           const int step = BN >= 128 ? 1 : 2;
@@ -206,9 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int x = 0; x < (BN + 127) / 128; ++x) {
             const int c = first * step + 64 * x;
             if (c < end && j * BN + c < g.J)
-              finish_box<T>(g.e, g.boxes, row0, j * BN + c, -1, w, false,
-                            [&](int k, float (&v)[32]) { get(c + k, v); },
-                            [&](int k) { return bias[2 * x + k / 32]; });
+              finish_box<T>(g.e, g.boxes, row0, j * BN + c, -1, w, phase, false,
+                            bias + 64 * x, [&](int k, float (&v)[32]) { get(c + k, v); });
           }
         } else {
           float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int c = first; c < end && j * BN + c < g.J; c += 32) {
             float v[32];
             get(c, v);
-            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, reinterpret_cast<float *>(w.box));
+            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, reinterpret_cast<float *>(w.at));
           }
         }
       }
@@ -274,7 +274,7 @@ Plan plan16(long long I, long long J, long long K) {
   Plan best{0, 1};
   double cost = 0;
   for (int bn : {256, 128, 64}) {
-    long long tiles = Tiles(I, J, kBM, bn).count;
+    long long tiles = (I + kBM - 1) / kBM * ((J + bn - 1) / bn);
     int parts = int(std::min<long long>({std::max(1ll, sms / tiles), std::max(1ll, slabs / 4), 64}));
     long long waves = (tiles * parts + sms - 1) / sms;
     double c = double(waves) * double((slabs + parts - 1) / parts) * (bn == 256 ? 1. : bn == 128 ? .56 : .36);
@@ -311,8 +311,7 @@ template <class T, int BN, bool PT, bool QT> void launch_gemm16(const Gemm16 &g,
     lapis::check(cudaFuncSetAttribute(gemm16_kernel<T, BN, PT, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     configured = device;
   }
-  long long units = Tiles(g.I, g.J, kBM, BN).count * g.parts;
-  lapis::launch(gemm16_kernel<T, BN, PT, QT>, dim3(unsigned(std::min<long long>(units, sm_count()))), kThreads, kSmem, stream, g);
+  lapis::launch(gemm16_kernel<T, BN, PT, QT>, dim3(std::min(g.units, unsigned(sm_count()))), kThreads, kSmem, stream, g);
   lapis::check(cudaGetLastError());
 }
 } // namespace
@@ -365,6 +364,9 @@ void product16(const Product &p, void *workspace, cudaStream_t stream) {
   g.I = p.I, g.J = p.J;
   g.slabs = int((p.K + kBK - 1) / kBK);
   g.parts = plan.parts;
+  check_tiles(p.I, p.J, kBM, plan.bn, plan.parts);
+  g.tiles = Tiles(p.I, p.J, kBM, plan.bn);
+  g.units = g.tiles.count * unsigned(plan.parts);
   // Boxes of a short k-major operand end with its rows (in groups of 8): what lies behind them in
   // shared memory reaches no output that is written.
   g.p_rows = int(std::min<long long>(kBM, round_up(p.I, 8)));

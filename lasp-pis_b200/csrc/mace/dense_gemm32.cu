@@ -18,7 +18,7 @@
 //           finishes a slab last issues its MMAs.
 //   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
 //           epilogue.  A slab that has reached TMEM has left its stage: warp 8 then starts the
-//           loads of the slab three ahead.
+//           loads of the slab two ahead.
 // (Loading by plain loads straight into the registers of the split was 5 times slower: the loads of
 // 64 KB per slab stalled the split warps.)
 // Infinities and NaN make every result of their row (of P or Q) NaN in this scheme; results that
@@ -29,21 +29,28 @@ namespace mace {
 namespace op {
 namespace {
 using namespace tc;
-constexpr int kBM = 128, kBK = 64, kStages = 3;
+constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 512, kDrainThreads = 256;
-// The split of slab g runs after the MMAs of g - 3, which waited for the drain of g - 5.
-constexpr int kSlots = 5;
+constexpr int kBuffers = 4; // TMEM accumulators
 template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2; }
+// 64-wide tiles: three stages, and a box of results per drain warp; 128-wide ones: two and two.
+template <int BN> constexpr int stages() { return BN == 64 ? 3 : 2; }
+// The split of slab g runs after the MMAs of g - stages, which waited for the drain of the slab
+// kBuffers before that.
+template <int BN> constexpr int slots() { return kBuffers + stages<BN>(); }
+template <int BN> constexpr int slot_bytes() { return 2 * BN + kBM; }
 template <int BN> constexpr int smem_bytes() {
-  return kStages * stage_bytes<BN>() + 8 * kBoxBytes + kSlots * (kBM + 2 * BN) + 384;
+  return stages<BN>() * stage_bytes<BN>() + 8 * (BN / 64) * kBoxBytes + 8 * (BN / 2) * 4 + slots<BN>() * slot_bytes<BN>() + 512;
 }
-static_assert(smem_bytes<128>() <= 232448, "shared memory budget");
+static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory budget");
 
 struct Gemm32 {
   CUtensorMap mp, mq;
   long long I, J, K;
   const float *p, *q;
   long long ldp, ldq;
+  Tiles tiles;
+  unsigned units; // tiles x parts
   int slabs, parts;
   uint32_t idesc;
   float *partial;
@@ -67,37 +74,43 @@ __device__ __forceinline__ void split2(float2 v, float2 scale, uint32_t &hi, uin
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// The walk over (tile, slab): the same for all warps.
+// The walk over (part of a tile, slab): the same for all warps.  Unit u is part u / tiles of tile
+// u % tiles, slabs [k, end).
 struct Walk {
-  long long u, units, tiles;
-  int k, end, slabs, parts;
+  unsigned u, tile;
+  int k, end, part;
   Walk() = default;
-  __device__ Walk(const Gemm32 &g, const Tiles &t)
-      : u(blockIdx.x), units(t.count * g.parts), tiles(t.count), k(0), end(0), slabs(g.slabs), parts(g.parts) {
-    open();
-  }
-  __device__ __forceinline__ void open() {
-    if (u < units) {
-      const long long s = u / tiles;
-      k = int(s * slabs / parts);
-      end = int((s + 1) * slabs / parts);
+  __device__ __forceinline__ explicit Walk(const Gemm32 &g) : u(blockIdx.x) { open(g); }
+  __device__ __forceinline__ void open(const Gemm32 &g) {
+    part = 0;
+    tile = u;
+    k = 0;
+    end = g.slabs;
+    if (g.parts > 1) {
+      part = int(u / g.tiles.count);
+      tile = u - unsigned(part) * g.tiles.count;
+      k = int((long long)part * g.slabs / g.parts);
+      end = int((part + 1ll) * g.slabs / g.parts);
     }
   }
-  __device__ __forceinline__ bool live() const { return u < units; }
-  __device__ __forceinline__ void next() {
-    if (++k >= end) {
-      u += gridDim.x;
-      open();
-    }
+  __device__ __forceinline__ bool live(const Gemm32 &g) const { return u < g.units; }
+  // Whether the next slab opens another unit.
+  __device__ __forceinline__ bool next(const Gemm32 &g) {
+    if (++k < end)
+      return false;
+    u += gridDim.x;
+    open(g);
+    return true;
   }
 };
 
 // The walk's state of the loads, and what the warps share.
 struct Shared {
   Walk ahead;
+  int i0, j0; // its tile
   uint32_t tmem_base;
   volatile int abort_flag;
-  int arrived[kSlots]; // split warps that are through with a slab
+  int arrived[8]; // per slot: split warps that are through with a slab
 };
 
 // Splits row r of an operand's slab (ROWS rows, floats at `base`) in place.  k-major: two boxes of
@@ -152,18 +165,15 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
 }
 
 // sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time; ends early at NaN.
-__device__ __noinline__ float plain_sum(const float *p, long long pk, const float *q, long long qk, long long k0,
+__device__ __forceinline__ float plain_sum(const float *p, long long pk, const float *q, long long qk, long long k0,
                                         long long k1) {
   float s = 0.f;
-  for (long long k = k0; k < k1; k += 128) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long kk = k + 32 * i + (threadIdx.x & 31);
-      if (kk < k1)
-        s = fmaf(p[kk * pk], q[kk * qk], s);
-    }
+#pragma unroll 1
+  for (long long k = k0 + (threadIdx.x & 31); k - (threadIdx.x & 31) < k1; k += 32) {
+    if (k < k1)
+      s = fmaf(p[k * pk], q[k * qk], s);
     if (__any_sync(0xffffffffu, s != s))
-      return __uint_as_float(0x7fc00000u);
+      break;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1)
@@ -174,27 +184,28 @@ __device__ __noinline__ float plain_sum(const float *p, long long pk, const floa
 template <int BN, bool PT, bool QT>
 __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_constant__ Gemm32 g) {
   constexpr int kPBytes = kBM * kBK * 2, kQBytes = BN * kBK * 2, kStageBytes = stage_bytes<BN>();
-  constexpr int kTmemCols = 2 * BN;
+  constexpr int kStages = stages<BN>(), kSlots = slots<BN>(), kSlotBytes = slot_bytes<BN>(), kBoxes = BN / 64;
+  constexpr int kTmemCols = kBuffers * BN;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char *staging = smem + kStages * kStageBytes; // a box per drain warp
+  unsigned char *staging = smem + kStages * kStageBytes; // the drain warps' boxes, then their bias
+  float *biases = reinterpret_cast<float *>(staging + 8 * kBoxes * kBoxBytes);
   // [kSlots][2 BN + kBM]: 2^-e of Q's rows (the upper halves of floats), then 127 - e of P's
-  unsigned char *scales = staging + 8 * kBoxBytes;
-  constexpr int kSlotBytes = 2 * BN + kBM;
+  unsigned char *scales = reinterpret_cast<unsigned char *>(biases + 8 * (BN / 2));
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kSlots * kSlotBytes);
-  // full[S] | tfull[2] | tfree[2] | scaled[kSlots] | residual[8]
-  constexpr int kBars = kStages + 4 + kSlots + 8;
-  static_assert(kBars * 8 + sizeof(Shared) <= 384, "barriers and state");
+  // full[S] | tfull[B] | tfree[B] | scaled[kSlots] | residual[8 x boxes]
+  constexpr int kBars = kStages + 2 * kBuffers + kSlots + 8 * kBoxes;
+  static_assert(kBars * 8 + sizeof(Shared) <= 512 && kSlots <= 8, "barriers and state");
   Shared &sh = *reinterpret_cast<Shared *>(bars + kBars);
   volatile int &abort_flag = sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned full0 = smem_u32(bars), tfull0 = full0 + 8 * kStages, tfree0 = tfull0 + 16, scaled0 = tfree0 + 16,
+  const unsigned full0 = smem_u32(bars), tfull0 = full0 + 8 * kStages, tfree0 = tfull0 + 8 * kBuffers, scaled0 = tfree0 + 8 * kBuffers,
                  residual0 = scaled0 + 8 * kSlots;
   constexpr int kSplitWarps = 4 + BN / 32;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kStages; ++s)
       mbar_init(full0 + 8 * s, 1);
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBuffers; ++b) {
       mbar_init(tfull0 + 8 * b, 1);
       mbar_init(tfree0 + 8 * b, kDrainThreads);
     }
@@ -202,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       mbar_init(scaled0 + 8 * x, kSplitWarps);
       sh.arrived[x] = 0;
     }
-    for (int x = 0; x < 8; ++x)
+    for (int x = 0; x < 8 * kBoxes; ++x)
       mbar_init(residual0 + 8 * x, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -216,12 +227,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
-  const Tiles tiles(g.I, g.J, kBM, BN);
 
   // The MMAs of slab n (one thread).
   auto multiply = [&](int n) {
-    const int b = n & 1;
-    if (n >= 2 && !mbar_wait(tfree0 + 8 * b, unsigned(n / 2 - 1) & 1, &sh.abort_flag))
+    const int b = n % kBuffers;
+    if (n >= kBuffers && !mbar_wait(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, &sh.abort_flag))
       return;
     tc_fence_after();
     const unsigned ph = smem_u32(smem + n % kStages * kStageBytes), pl = ph + kPBytes, qh = pl + kPBytes, ql = qh + kQBytes;
@@ -236,11 +246,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       umma_f16_desc(d, smem_desc(ph + 32 * m), smem_desc(qh + 32 * m), g.idesc, 1u);
     umma_commit(tfull0 + 8 * b);
   };
-  // The loads of slab n at walk w (one thread; the MMAs of slab n - 3 are done).
-  auto fetch = [&](int n, const Walk &w) {
+  // The loads of slab n at sh.ahead, which moves on (one thread; the MMAs of slab n - 2 are done).
+  auto open_ahead = [&] {
     long long i, j;
-    tiles.at(w.u % tiles.count, i, j);
-    const int i0 = int(i * kBM), j0 = int(j * BN), k0 = w.k * kBK;
+    g.tiles.at(sh.ahead.tile, i, j);
+    sh.i0 = int(i * kBM), sh.j0 = int(j * BN);
+  };
+  auto fetch = [&](int n) {
+    const int i0 = sh.i0, j0 = sh.j0, k0 = sh.ahead.k * kBK;
     const unsigned base = smem_u32(smem + n % kStages * kStageBytes), full = full0 + 8 * (n % kStages);
     mbar_expect_tx(full, kStageBytes);
     if (PT) {
@@ -259,14 +272,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       tma_load_2d(base + 2 * kPBytes, &g.mq, k0, j0, full);
       tma_load_2d(base + 2 * kPBytes + kQBytes, &g.mq, k0 + 32, j0, full);
     }
+    if (sh.ahead.next(g) && sh.ahead.live(g))
+      open_ahead();
   };
 
-  if (warp < kSplitWarps) {
+  // Registers: 128 each at launch; 256 threads give 32 to the other 256 (96 + 160 = 2 x 128).
+  if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const bool of_q = warp >= 4;
     const int r = threadIdx.x & 127;
     bool ok = true; // the same in the whole warp
     int n = 0;
-    for (Walk w(g, tiles); w.live(); w.next(), ++n) {
+    if (warp < kSplitWarps)
+    for (Walk w(g); w.live(g); w.next(g), ++n) {
       ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
       if (!ok) { // the other warps of the operand may wait at this slab's barrier
         if (of_q ? QT : PT)
@@ -294,81 +312,82 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         }
       }
     }
-  } else if (warp >= 8) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     constexpr int kCols = BN / 2;
     const int quarter = warp & 3, half = (warp - 8) >> 2;
     const int me = warp - 8;
-    Warp box{staging + me * kBoxBytes, residual0 + 8 * me, 0};
-    // The residual of a tile's first box is on its way while the tile accumulates (a kept z needs the
-    // box first).
+    Box boxes[kBoxes];
+    unsigned phase[kBoxes] = {};
+#pragma unroll
+    for (int x = 0; x < kBoxes; ++x)
+      boxes[x] = {staging + (kBoxes * me + x) * kBoxBytes, residual0 + 8 * (kBoxes * me + x)};
+    float *bias = biases + me * kCols;
+    // A tile's residual is on its way while the tile accumulates (a kept z needs the boxes first).
     const bool early = g.boxes.on && !g.partial && g.e.residual && !g.e.z;
-    Walk &ahead = sh.ahead; // of the loads: warp 8's first lane
     if (me == 0 && lane == 0) {
-      ahead = Walk(g, tiles);
-      for (int x = 0; x < kStages && ahead.live(); ++x, ahead.next())
-        fetch(x, ahead);
+      sh.ahead = Walk(g);
+      open_ahead();
+      for (int x = 0; x < kStages && sh.ahead.live(g); ++x)
+        fetch(x);
     }
     float acc[kCols];
     bool ok = true;
     int n = 0;
-    for (Walk w(g, tiles); w.live();) {
-      const long long u = w.u, s = u / tiles.count;
-      const long long k0 = (long long)w.k * kBK, k1 = min(g.K, (long long)w.end * kBK);
+    for (Walk w(g); w.live(g);) {
+      const int s = w.part;
       long long i, j;
-      tiles.at(u - s * tiles.count, i, j);
+      g.tiles.at(w.tile, i, j);
       const long long row0 = i * kBM + 32 * quarter, row = row0 + lane, cols0 = j * BN + half * kCols;
       const bool any = row0 < g.I && cols0 < g.J;
-      float bias[kCols / 32];
-#pragma unroll
-      for (int c = 0; c < kCols / 32; ++c)
-        bias[c] = g.e.bias && cols0 + 32 * c + lane < g.J ? static_cast<const float *>(g.e.bias)[cols0 + 32 * c + lane] : 0.f;
+      if (!g.partial)
+        fetch_bias<float>(g.e, g.J, cols0, kCols, bias);
       if (early && any && lane == 0) {
         bulk_wait_read();
-        fetch_residual(g.boxes, box, row0, cols0);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c)
+          if (cols0 + 32 * c < g.J)
+            fetch_residual(g.boxes, boxes[c], row0, cols0 + 32 * c);
       }
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
         acc[c] = 0.f;
-      for (; w.live() && w.u == u; w.next(), ++n) {
-        const int b = n & 1;
-        ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(n / 2) & 1, &sh.abort_flag) &&
+      for (bool same = true; same; same = !w.next(g), ++n) {
+        const int b = n % kBuffers;
+        ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(n / kBuffers) & 1, &sh.abort_flag) &&
              mbar_wait(scaled0 + 8 * (n % kSlots), unsigned(n / kSlots) & 1, &sh.abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
           continue;
-        if (me == 0 && lane == 0 && ahead.live()) {
-          fetch(n + kStages, ahead);
-          ahead.next();
-        }
+        if (me == 0 && lane == 0 && sh.ahead.live(g))
+          fetch(n + kStages);
         tc_fence_after();
         const unsigned char *scale = scales + n % kSlots * kSlotBytes;
         const unsigned char *fq = scale + 2 * (half * kCols);
         // 2^-e of P's row, one ulp more in three slabs of four.
         const float fp = __uint_as_float((uint32_t(scale[2 * BN + 32 * quarter + lane]) << 23) + ((n & 3) != 3));
         const float2 fp2 = make_float2(fp, fp);
+        uint32_t r[kCols / 32][32];
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + half * kCols + c0), r);
-          tmem_wait_ld();
-          tmem_anchor(r);
-          if (c0 + 32 == kCols) {
-            tc_fence_before();
-            mbar_arrive(tfree0 + 8 * b);
-          }
+        for (int h = 0; h < kCols / 32; ++h)
+          tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + half * kCols + 32 * h), r[h]);
+        tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const uint2 f = *reinterpret_cast<const uint2 *>(fq + 2 * (c0 + c));
-            const uint32_t fs[2] = {f.x, f.y};
+        for (int h = 0; h < kCols / 32; ++h)
+          tmem_anchor(r[h]);
+        tc_fence_before();
+        mbar_arrive(tfree0 + 8 * b);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) { // the two scalings, and the float sum
-              const int x = c0 + c + 2 * y;
-              const float2 s = make_float2(__uint_as_float(fs[y] << 16), __uint_as_float(fs[y] & 0xffff0000u));
-              const float2 a = __ffma2_rn(
-                  __fmul2_rn(make_float2(__uint_as_float(r[c + 2 * y]), __uint_as_float(r[c + 2 * y + 1])), s), fp2,
-                  make_float2(acc[x], acc[x + 1]));
-              acc[x] = a.x, acc[x + 1] = a.y;
-            }
+        for (int c = 0; c < kCols; c += 4) {
+          const uint2 f = *reinterpret_cast<const uint2 *>(fq + 2 * c);
+          const uint32_t fs[2] = {f.x, f.y};
+#pragma unroll
+          for (int y = 0; y < 2; ++y) { // the two scalings, and the float sum
+            const int x = c + 2 * y;
+            const float2 s = make_float2(__uint_as_float(fs[y] << 16), __uint_as_float(fs[y] & 0xffff0000u));
+            const float2 v = make_float2(__uint_as_float(r[x / 32][x % 32]), __uint_as_float(r[x / 32][x % 32 + 1]));
+            const float2 a = __ffma2_rn(__fmul2_rn(v, s), fp2, make_float2(acc[x], acc[x + 1]));
+            acc[x] = a.x, acc[x + 1] = a.y;
           }
         }
       }
@@ -378,38 +397,48 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         const long long col0 = cols0 + c0;
         if (row0 >= g.I || col0 >= g.J)
           continue;
-        bool odd = false;
+        if (!ok) { // a wait that ran out shows as NaN
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (!ok) // a wait that ran out shows as NaN
+          for (int c = 0; c < 32; ++c)
             acc[c0 + c] = __uint_as_float(0x7fc00000u);
-          odd |= !(fabsf(acc[c0 + c]) < INFINITY);
         }
-        if (__any_sync(0xffffffffu, odd && ok)) {
+        // 0 x: NaN where x is not finite.
+        float2 probe[4] = {};
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            unsigned todo = __ballot_sync(0xffffffffu, !(fabsf(acc[c0 + c]) < INFINITY) && row < g.I && col0 + c < g.J);
-            while (todo) {
-              const int at = __ffs(todo) - 1;
-              todo &= todo - 1;
-              const float x = plain_sum(g.p + (row0 + at) * (PT ? 1 : g.ldp), PT ? g.ldp : 1,
-                                        g.q + (col0 + c) * (QT ? 1 : g.ldq), QT ? g.ldq : 1, k0, k1);
-              if (lane == at)
-                acc[c0 + c] = x;
-            }
+        for (int c = 0; c < 32; c += 2)
+          probe[c / 2 & 3] = __ffma2_rn(make_float2(acc[c0 + c], acc[c0 + c + 1]), make_float2(0.f, 0.f), probe[c / 2 & 3]);
+        const float2 p01 = __fadd2_rn(__fadd2_rn(probe[0], probe[1]), __fadd2_rn(probe[2], probe[3]));
+        uint32_t odd = 0; // this lane's columns that are not finite
+        if (__any_sync(0xffffffffu, p01.x + p01.y != 0.f) && ok) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!(fabsf(acc[c0 + c]) < INFINITY) && row < g.I && col0 + c < g.J)
+              odd |= 1u << c;
+        }
+        while (const unsigned lanes = __ballot_sync(0xffffffffu, odd != 0)) {
+          const int at = __ffs(lanes) - 1, c = __ffs(__shfl_sync(0xffffffffu, odd, at)) - 1;
+          const float x = plain_sum(g.p + (row0 + at) * (PT ? 1 : g.ldp), PT ? g.ldp : 1,
+                                    g.q + (col0 + c) * (QT ? 1 : g.ldq), QT ? g.ldq : 1,
+                                    (long long)s * g.slabs / g.parts * kBK,
+                                    min(g.K, (s + 1ll) * g.slabs / g.parts * kBK));
+          if (lane == at) {
+            odd &= odd - 1;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == c)
+                acc[c0 + i] = x;
           }
         }
         if (g.boxes.on)
           finish_box<float>(
-              g.e, g.boxes, row0, col0, g.partial ? int(s) : -1, box, early && c0 == 0,
+              g.e, g.boxes, row0, col0, g.partial ? s : -1, boxes[c0 / 32], phase[c0 / 32], early || (c0 && !g.e.z), bias + c0,
               [&](int, float (&v)[32]) {
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
                   v[c] = acc[c0 + c];
-              },
-              [&](int) { return bias[c0 / 32]; });
+              });
         else
-          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, reinterpret_cast<float *>(box.box));
+          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, reinterpret_cast<float *>(boxes[0].at));
       }
     }
     if (lane == 0)
@@ -437,9 +466,8 @@ template <int BN, bool PT, bool QT> void launch_gemm32(const Gemm32 &g, cudaStre
                                       smem_bytes<BN>()));
     configured = device;
   }
-  long long units = Tiles(g.I, g.J, kBM, BN).count * g.parts;
-  lapis::launch(gemm32_kernel<BN, PT, QT>, dim3(unsigned(std::min<long long>(units, sm_count()))), kThreads,
-                smem_bytes<BN>(), stream, g);
+  lapis::launch(gemm32_kernel<BN, PT, QT>, dim3(std::min(g.units, unsigned(sm_count()))), kThreads, smem_bytes<BN>(),
+                stream, g);
   lapis::check(cudaGetLastError());
 }
 } // namespace
@@ -448,7 +476,7 @@ template <int BN, bool PT, bool QT> void launch_gemm32(const Gemm32 &g, cudaStre
 // device, parts of at least two slabs.
 Plan plan32(long long I, long long J, long long K) {
   Plan p{J <= 64 ? 64 : 128, 1};
-  const long long tiles = Tiles(I, J, kBM, p.bn).count, slabs = (K + kBK - 1) / kBK;
+  const long long tiles = (I + kBM - 1) / kBM * ((J + p.bn - 1) / p.bn), slabs = (K + kBK - 1) / kBK;
   p.parts = int(std::min<long long>({std::max(1ll, sm_count() / tiles), std::max(1ll, slabs / 2), 148}));
   return p;
 }
@@ -463,6 +491,9 @@ void product32(const Product &p, void *workspace, cudaStream_t stream) {
   g.mq = p.q.turned ? tile_map(F32, p.q.p, p.K, p.J, p.q.ld, kBK) : tile_map(F32, p.q.p, p.J, p.K, p.q.ld, plan.bn);
   g.slabs = int((p.K + kBK - 1) / kBK);
   g.parts = plan.parts;
+  check_tiles(p.I, p.J, kBM, plan.bn, plan.parts);
+  g.tiles = Tiles(p.I, p.J, kBM, plan.bn);
+  g.units = g.tiles.count * unsigned(plan.parts);
   g.idesc = idesc_f16(kBM, plan.bn);
   g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
   g.e = p.e;
