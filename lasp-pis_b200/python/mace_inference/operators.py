@@ -19,13 +19,15 @@ TypeError), a failed call RuntimeError.
 from __future__ import annotations
 
 import ctypes as ct
+import math
 
 from .native import _error, load
 
 ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "relu": 3}
 
-_bound = None
-_types = {}
+_bound = None   # (library, torch, the current stream's handle of a device index)
+_types = {}     # torch type -> element type of the C interface
+_sizes = {}     # workspace bytes by what they depend on: shapes, row distances, 16-byte alignment
 
 
 def _library():
@@ -45,7 +47,10 @@ def _library():
         lib.mace_layer_norm_backward_workspace.argtypes = [i, n, n]
         lib.mace_layer_norm_backward_workspace.restype = n
         _types.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-        _bound = lib, torch
+        # The stream's handle without a stream object (2 us a call), where torch has it.
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _bound = lib, torch, stream
     return _bound
 
 
@@ -69,32 +74,31 @@ def _type(t, name, torch):
     return code
 
 
-def _like(t, x, name, torch, shape, dtype=None):
-    """Checks a tensor that goes with `x`."""
+def _like(t, name, torch, shape, dtype, device):
+    """Checks a tensor that goes with others; returns it."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} is a torch tensor, not {type(t).__name__}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != (dtype or x.dtype):
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype or x.dtype}")
-    if t.device != x.device:
-        raise ValueError(f"{name} is on {t.device}, the other tensors on {x.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    return t
 
 
 def _rows(t):
     """`t` as rows with a contiguous last index: (tensor that keeps the memory alive, address, row distance)."""
-    if t.dim() == 2:
-        width = t.shape[1]
-        s0, s1 = t.stride()
-        if (s1 == 1 or width == 1) and (s0 >= width or t.shape[0] <= 1):
-            return t, t.data_ptr(), max(s0, width)
-    elif t.is_contiguous():
-        return t, t.data_ptr(), t.shape[-1]
-    else:
-        two = t.reshape(-1, t.shape[-1])  # a view where the leading indices collapse
-        return _rows(two) if two.dim() == 2 else _rows(two.contiguous())
+    if t.dim() != 2:
+        if t.is_contiguous():
+            return t, t.data_ptr(), t.shape[-1]
+        t = t.reshape(-1, t.shape[-1])  # a view where the leading indices collapse
+    rows, width = t.shape
+    s0, s1 = t.stride()
+    if (s1 == 1 or width == 1) and (s0 >= width or rows <= 1):
+        return t, t.data_ptr(), s0 if s0 > width else width
     t = t.contiguous()
-    return t, t.data_ptr(), t.shape[1]
+    return t, t.data_ptr(), width
 
 
 def _flat(t):
@@ -105,72 +109,60 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """Makes a device current for a call (and back)."""
-
-    def __init__(self, torch, device):
-        self.guard = None
-        if torch.cuda.current_device() != device.index:
-            self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *args):
-        if self.guard is not None:
-            self.guard.__exit__(*args)
+def _on(torch, device, call, *args, **kwargs):
+    """call(...) with `device` current."""
+    with torch.cuda.device(device):
+        return call(*args, **kwargs)
 
 
-def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _size(lib, key, call, *args):
+    """Workspace bytes, asked once for each `key`."""
+    size = _sizes.get(key)
+    if size is None:
+        size = call(*args)
+        if size < 0:
+            raise RuntimeError(_error(lib))
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        _sizes[key] = size
+    return size
 
 
-def _workspace(torch, lib, size, device):
-    if size < 0:
-        raise RuntimeError(_error(lib))
+def _workspace(torch, size, device):
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
-def _count(shape):
-    n = 1
-    for v in shape:
-        n *= v
-    return n
 
 
 def dense(x, weight, bias=None, activation=None, residual=None, keep=False):
     """``activation(x weight^T + bias) + residual`` for x (..., inputs), weight (outputs, inputs),
     bias (outputs,) and residual (..., outputs).  ``keep=True`` returns (y, z) with
     z = x weight^T + bias, which ``dense_backward`` takes where there is an activation."""
-    lib, torch = _library()
+    lib, torch, stream = _bound or _library()
     act = _activation(activation)
     code = _type(x, "x", torch)
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if torch.cuda.current_device() != device.index:
+        return _on(torch, device, dense, x, weight, bias, activation, residual, keep)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight is a matrix (outputs, inputs)")
-    inputs, outputs = x.shape[-1], weight.shape[0]
-    _like(weight, x, "weight", torch, (outputs, inputs))
-    shape = x.shape[:-1] + (outputs,)
+    outputs, inputs = weight.shape[0], shape[-1]
+    _like(weight, "weight", torch, (outputs, inputs), dtype, device)
+    shape = (*shape[:-1], outputs)
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
     if bias is not None:
-        _like(bias, x, "bias", torch, (outputs,))
-        bias = _flat(bias)
+        bias = _flat(_like(bias, "bias", torch, (outputs,), dtype, device))
+    pr, ldr = None, 0
     if residual is not None:
-        _like(residual, x, "residual", torch, shape)
-    device = x.device
-    with _On(torch, device):
-        y = torch.empty(shape, dtype=x.dtype, device=device)
-        z = torch.empty(shape, dtype=x.dtype, device=device) if keep else None
-        rows = _count(shape[:-1])
-        x, px, ldx = _rows(x)
-        weight, pw, ldw = _rows(weight)
-        pr, ldr = None, 0
-        if residual is not None:
-            residual, pr, ldr = _rows(residual)
-        size = lib.mace_dense_workspace(code, rows, inputs, outputs, px, ldx, pw, ldw)
-        ws = _workspace(torch, lib, size, device)
-        if lib.mace_dense(code, rows, inputs, outputs, px, ldx, pw, ldw, _address(bias), act, pr, ldr, y.data_ptr(),
-                          outputs, _address(z), outputs, _address(ws), size, _stream(torch, device)):
-            raise RuntimeError(_error(lib))
+        residual, pr, ldr = _rows(_like(residual, "residual", torch, shape, dtype, device))
+    x, px, ldx = _rows(x)
+    weight, pw, ldw = _rows(weight)
+    y = x.new_empty(shape)
+    z = x.new_empty(shape) if keep else None
+    size = _size(lib, (0, code, rows, inputs, outputs, px & 15, ldx, pw & 15, ldw, device.index),
+                 lib.mace_dense_workspace, code, rows, inputs, outputs, px, ldx, pw, ldw)
+    ws = _workspace(torch, size, device)
+    if lib.mace_dense(code, rows, inputs, outputs, px, ldx, pw, ldw, _address(bias), act, pr, ldr, y.data_ptr(), outputs,
+                      _address(z), outputs, _address(ws), size, stream(device.index)):
+        raise RuntimeError(_error(lib))
     return (y, z) if keep else y
 
 
@@ -178,65 +170,61 @@ def dense_backward(dy, x, weight, activation=None, z=None, need=(True, True, Tru
     """(dx, dweight, dbias) of ``dense`` for the output gradient dy (..., outputs); z is what
     ``dense(..., keep=True)`` gave (not needed without an activation).  The residual's gradient
     is dy itself.  ``need`` leaves gradients out: None comes back in their place."""
-    lib, torch = _library()
+    lib, torch, stream = _bound or _library()
     act = _activation(activation)
     code = _type(x, "x", torch)
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if torch.cuda.current_device() != device.index:
+        return _on(torch, device, dense_backward, dy, x, weight, activation, z, need)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight is a matrix (outputs, inputs)")
-    inputs, outputs = x.shape[-1], weight.shape[0]
-    _like(weight, x, "weight", torch, (outputs, inputs))
-    shape = x.shape[:-1] + (outputs,)
-    _like(dy, x, "dy", torch, shape)
+    outputs, inputs = weight.shape[0], shape[-1]
+    _like(weight, "weight", torch, (outputs, inputs), dtype, device)
+    out = (*shape[:-1], outputs)
+    rows = out[0] if len(out) == 2 else math.prod(out[:-1])
+    dy, pd, ldd = _rows(_like(dy, "dy", torch, out, dtype, device))
+    pz, ldz = None, 0
     if act:
         if z is None:
             raise ValueError(f"the gradient of {activation} needs z")
-        _like(z, x, "z", torch, shape)
-    device = x.device
-    with _On(torch, device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need[0] else None
-        dweight = torch.empty((outputs, inputs), dtype=x.dtype, device=device) if need[1] else None
-        dbias = torch.empty(outputs, dtype=x.dtype, device=device) if need[2] else None
-        rows = _count(shape[:-1])
-        x, px, ldx = _rows(x)
-        weight, pw, ldw = _rows(weight)
-        dy, pd, ldd = _rows(dy)
-        pz, ldz = None, 0
-        if act:
-            z, pz, ldz = _rows(z)
-        size = lib.mace_dense_backward_workspace(code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act)
-        ws = _workspace(torch, lib, size, device)
-        if lib.mace_dense_backward(code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act, pz, ldz, _address(dx),
-                                   inputs, _address(dweight), inputs, _address(dbias), _address(ws), size,
-                                   _stream(torch, device)):
-            raise RuntimeError(_error(lib))
+        z, pz, ldz = _rows(_like(z, "z", torch, out, dtype, device))
+    x, px, ldx = _rows(x)
+    weight, pw, ldw = _rows(weight)
+    dx = x.new_empty(shape) if need[0] else None
+    dweight = x.new_empty((outputs, inputs)) if need[1] else None
+    dbias = x.new_empty((outputs,)) if need[2] else None
+    size = _size(lib, (1, code, rows, inputs, outputs, pd & 15, ldd, px & 15, ldx, pw & 15, ldw, act, device.index),
+                 lib.mace_dense_backward_workspace, code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act)
+    ws = _workspace(torch, size, device)
+    if lib.mace_dense_backward(code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act, pz, ldz, _address(dx), inputs,
+                               _address(dweight), inputs, _address(dbias), _address(ws), size, stream(device.index)):
+        raise RuntimeError(_error(lib))
     return dx, dweight, dbias
-
-
-def _parameters(x, gamma, beta, torch):
-    width = x.shape[-1]
-    if gamma is not None:
-        _like(gamma, x, "gamma", torch, (width,))
-    if beta is not None:
-        _like(beta, x, "beta", torch, (width,))
-    return width, _flat(gamma), _flat(beta)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, activation=None, keep=False):
     """``activation((x - mean) rstd gamma + beta)`` over the last index, with the biased variance.
     ``keep=True`` returns (y, mean, rstd), the statistics float32 of shape x.shape[:-1]."""
-    lib, torch = _library()
+    lib, torch, stream = _bound or _library()
     act = _activation(activation)
     code = _type(x, "x", torch)
-    width, gamma, beta = _parameters(x, gamma, beta, torch)
-    device, shape = x.device, x.shape
-    with _On(torch, device):
-        y = torch.empty(shape, dtype=x.dtype, device=device)
-        mean = torch.empty(shape[:-1], dtype=torch.float32, device=device) if keep else None
-        rstd = torch.empty(shape[:-1], dtype=torch.float32, device=device) if keep else None
-        x, px, ldx = _rows(x) if x.dim() > 1 else _rows(x[None])
-        if lib.mace_layer_norm(code, _count(shape[:-1]), width, px, ldx, _address(gamma), _address(beta), eps, act,
-                               y.data_ptr(), width, _address(mean), _address(rstd), _stream(torch, device)):
-            raise RuntimeError(_error(lib))
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if torch.cuda.current_device() != device.index:
+        return _on(torch, device, layer_norm, x, gamma, beta, eps, activation, keep)
+    width = shape[-1]
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if gamma is not None:
+        gamma = _flat(_like(gamma, "gamma", torch, (width,), dtype, device))
+    if beta is not None:
+        beta = _flat(_like(beta, "beta", torch, (width,), dtype, device))
+    x, px, ldx = _rows(x)
+    y = x.new_empty(shape)
+    mean = rstd = None
+    if keep:
+        mean, rstd = x.new_empty((2, *shape[:-1]), dtype=torch.float32).unbind(0)
+    if lib.mace_layer_norm(code, rows, width, px, ldx, _address(gamma), _address(beta), eps, act, y.data_ptr(), width,
+                           _address(mean), _address(rstd), stream(device.index)):
+        raise RuntimeError(_error(lib))
     return (y, mean, rstd) if keep else y
 
 
@@ -245,26 +233,31 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, beta=None, activation=Non
     ``layer_norm(..., keep=True)`` gave and the gamma, beta and activation of that call (beta is
     read only with an activation).  ``need`` leaves gradients out: None comes back in their
     place."""
-    lib, torch = _library()
+    lib, torch, stream = _bound or _library()
     act = _activation(activation)
     code = _type(x, "x", torch)
-    width, gamma, beta = _parameters(x, gamma, beta, torch)
-    device, shape = x.device, x.shape
-    _like(dy, x, "dy", torch, shape)
-    _like(mean, x, "mean", torch, shape[:-1], torch.float32)
-    _like(rstd, x, "rstd", torch, shape[:-1], torch.float32)
-    with _On(torch, device):
-        dx = torch.empty(shape, dtype=x.dtype, device=device) if need[0] else None
-        dgamma = torch.empty(width, dtype=x.dtype, device=device) if need[1] else None
-        dbeta = torch.empty(width, dtype=x.dtype, device=device) if need[2] else None
-        rows = _count(shape[:-1])
-        x, px, ldx = _rows(x) if x.dim() > 1 else _rows(x[None])
-        dy, pd, ldd = _rows(dy) if dy.dim() > 1 else _rows(dy[None])
-        mean, rstd = _flat(mean), _flat(rstd)
-        size = lib.mace_layer_norm_backward_workspace(code, rows, width) if need[1] or need[2] else 0
-        ws = _workspace(torch, lib, size, device)
-        if lib.mace_layer_norm_backward(code, rows, width, pd, ldd, px, ldx, mean.data_ptr(), rstd.data_ptr(),
-                                        _address(gamma), _address(beta), act, _address(dx), width, _address(dgamma),
-                                        _address(dbeta), _address(ws), size, _stream(torch, device)):
-            raise RuntimeError(_error(lib))
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if torch.cuda.current_device() != device.index:
+        return _on(torch, device, layer_norm_backward, dy, x, mean, rstd, gamma, beta, activation, need)
+    width = shape[-1]
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if gamma is not None:
+        gamma = _flat(_like(gamma, "gamma", torch, (width,), dtype, device))
+    if beta is not None:
+        beta = _flat(_like(beta, "beta", torch, (width,), dtype, device))
+    dy, pd, ldd = _rows(_like(dy, "dy", torch, shape, dtype, device))
+    mean = _flat(_like(mean, "mean", torch, shape[:-1], torch.float32, device))
+    rstd = _flat(_like(rstd, "rstd", torch, shape[:-1], torch.float32, device))
+    x, px, ldx = _rows(x)
+    dx = x.new_empty(shape) if need[0] else None
+    dgamma = x.new_empty((width,)) if need[1] else None
+    dbeta = x.new_empty((width,)) if need[2] else None
+    size = 0
+    if need[1] or need[2]:
+        size = _size(lib, (2, code, rows, width, device.index), lib.mace_layer_norm_backward_workspace, code, rows, width)
+    ws = _workspace(torch, size, device)
+    if lib.mace_layer_norm_backward(code, rows, width, pd, ldd, px, ldx, mean.data_ptr(), rstd.data_ptr(),
+                                    _address(gamma), _address(beta), act, _address(dx), width, _address(dgamma),
+                                    _address(dbeta), _address(ws), size, stream(device.index)):
+        raise RuntimeError(_error(lib))
     return dx, dgamma, dbeta

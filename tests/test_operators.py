@@ -590,7 +590,7 @@ def test_in_place_and_untouched_memory(op, library):
     """Through the C entries: y over its residual, layer norm over its input, dx over dy; memory
     between the rows of a strided output, and behind the last row, stays as it was."""
     import torch
-    lib, _ = op._library()
+    lib = op._library()[0]
     s = torch.cuda.current_stream().cuda_stream
     for dt, code in ((torch.float32, 0), (torch.bfloat16, 1)):
         M, K, N, ld = 70, 48, 40, 56
@@ -698,13 +698,13 @@ REFUSED = [
 @pytest.mark.parametrize("call,wrong,message", REFUSED, ids=lambda v: v.__name__ if callable(v) else str(v)[:40])
 def test_refusals(op, call, wrong, message):
     """Wrong arguments are refused before anything is launched (the addresses are not real)."""
-    lib, _ = op._library()
+    lib = op._library()[0]
     code, error = call(lib, **wrong)
     assert code == -1 and message in error, error
 
 
 def test_no_rows_is_no_work(op):
-    lib, _ = op._library()
+    lib = op._library()[0]
     assert call_dense(lib, rows=0, x=None, y=None)[0] == 0
     assert call_norm(lib, rows=0, x=None, y=None)[0] == 0
     assert call_dense_backward(lib, rows=0, dy=None, dw=None, db=None, dx=None, size=0, ws=None)[0] == 0
