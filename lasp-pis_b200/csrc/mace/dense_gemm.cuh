@@ -189,31 +189,52 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
   send(m.y, plain ? part : 0);
 }
 
-// A warp's 32 x 32 block where rows allow no boxes: through 32 rows of 16 floats (their columns
-// permuted by row), so that neighbouring lanes write neighbouring columns.  partial != NULL: the
-// float values go to partial[row * J + col] instead.
+// A warp's 32 x 32 block where rows allow no boxes: through its box (columns permuted by row), so that
+// neighbouring lanes write neighbouring columns, 8 rows' residuals in flight at once.  partial !=
+// NULL: the float values go to partial[row * J + col] instead.
 template <class T>
 __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
-                                             long long row0, long long col0, float *v, float *stage) {
-  const int lane = threadIdx.x & 31;
-  const int rows = int(min(32ll, I - row0));
+                                             long long row0, long long col0, const float *v, unsigned char *box) {
+  constexpr bool Fast = sizeof(T) == 2;
+  const int lane = threadIdx.x & 31, rows = int(min(32ll, I - row0));
+  float *stage = reinterpret_cast<float *>(box);
+  __syncwarp();
 #pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    __syncwarp();
+  for (int k = 0; k < 32; ++k)
+    stage[lane * 32 + (k ^ lane)] = v[k];
+  __syncwarp();
+  const long long col = col0 + lane;
+  if (col < J) {
+    const float bias = e.bias && !partial ? to_float(static_cast<const T *>(e.bias)[col]) : 0.f;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      float x[8];
+      T res[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      stage[lane * 16 + (k ^ (lane & 15))] = v[h + k];
-    __syncwarp();
-    const long long col = col0 + h + (lane & 15);
-    if (col < J)
-#pragma unroll 4
-      for (int r = lane >> 4; r < rows; r += 2) {
-        const float x = stage[r * 16 + ((lane ^ r) & 15)];
-        if (partial)
-          partial[(row0 + r) * J + col] = x;
-        else
-          finish<T>(e, row0 + r, col, x);
+      for (int i = 0; i < 8; ++i)
+        if (!partial && e.residual && r0 + i < rows)
+          res[i] = static_cast<const T *>(e.residual)[(row0 + r0 + i) * e.ldr + col];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = stage[(r0 + i) * 32 + (lane ^ (r0 + i))] + bias;
+      if (partial) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r0 + i < rows)
+            partial[(row0 + r0 + i) * J + col] = x[i];
+        continue;
       }
+      if (e.z)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r0 + i < rows)
+            static_cast<T *>(e.z)[(row0 + r0 + i) * e.ldz + col] = from_float<T>(x[i]);
+      activate_all<Fast>(x, e.activation);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i < rows)
+          static_cast<T *>(e.out)[(row0 + r0 + i) * e.ldo + col] = from_float<T>(e.residual ? x[i] + to_float(res[i]) : x[i]);
+    }
   }
   __syncwarp();
 }

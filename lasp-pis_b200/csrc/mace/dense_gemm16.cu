@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int c = first; c < end && j * BN + c < g.J; c += 32) {
             float v[32];
             get(c, v);
-            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, reinterpret_cast<float *>(w.at));
+            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, w.at);
           }
         }
       }

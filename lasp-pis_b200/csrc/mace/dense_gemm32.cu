@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
                   v[c] = acc[c0 + c];
               });
         else
-          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, reinterpret_cast<float *>(boxes[0].at));
+          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, boxes[0].at);
       }
     }
     if (lane == 0)

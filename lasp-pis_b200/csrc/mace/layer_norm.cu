@@ -6,13 +6,14 @@
 //             dx = r (g - mean(g) - xhat mean(g xhat)),
 //             dgamma = sum over rows of dz xhat, dbeta = sum over rows of dz
 //
-// One pass over the data: a row stays in the registers of its group of threads (part of a warp,
-// or a block for wide rows) between its statistics and its result, and each row's loads are
-// issued before the arithmetic of the row before.  The variance is taken about a first mean and
-// corrected for that mean's own rounding, so a row far from zero loses nothing.  A group walks
-// the rows with a fixed set of columns per thread, so gamma, beta and the parameters' gradients
-// stay in registers too; each block writes one partial row of dgamma and dbeta, and a second
-// launch adds the partial rows in a fixed order.
+// One pass over the data: a row stays in the registers of its group of threads (part of a warp, a
+// warp, or a block for wide rows) between its statistics and its result.  HBM bounds it, so what
+// counts is bytes in flight: a warp holds rows of up to 8 KiB, and where a thread's share of a row is
+// small it takes several rows at once, and loads the next ones before the arithmetic of these.  The
+// variance is taken about a first mean and corrected for that mean's own rounding, so a row far from
+// zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
+// parameters' gradients stay in registers too; each block writes one partial row of dgamma and
+// dbeta, and a second launch adds the partial rows in a fixed order.
 #include "operators.cuh"
 #include <algorithm>
 #include <type_traits>
@@ -20,201 +21,259 @@
 namespace mace {
 namespace op {
 namespace {
-constexpr int kWarpBlock = 256; // threads of a block whose rows belong to parts of warps
+constexpr int kWarpBlock = 256; // threads of a block whose rows belong to warps or parts of them
+constexpr int kSharedChunks = 4; // forward: from as many units per lane on
 
-// Sum of two values over a row's group: G lanes (G <= 32, power of two), or the block.
-template <bool Warp> __device__ __forceinline__ float2 group_sum(float2 v, int G, float2 *shared) {
-  int top = Warp ? G >> 1 : 16;
-  for (int o = top; o; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  if (Warp)
-    return v;
-  int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  if (!lane)
-    shared[warp] = v;
-  __syncthreads();
-  v = lane < warps ? shared[lane] : make_float2(0.f, 0.f);
+// A unit of row `row` (column col) of an array, or zeros where it is not live.  The load itself is
+// unconditional, from a place inside the array: a load under a branch is waited for where the
+// branches join, which leaves one in flight instead of all of a row's.
+template <class T, int U>
+__device__ __forceinline__ Unit<T, U> load_unit(const T *p, long long ld, long long row, long long rows, int col, int width) {
+  Unit<T, U> v = *reinterpret_cast<const Unit<T, U> *>(p + min(row, rows - 1) * ld + min(col, width - U));
+  const bool live = row < rows && col < width;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
+  for (int u = 0; u < U; ++u)
+    v.v[u] = live ? v.v[u] : from_float<T>(0.f);
+  return v;
+}
+// A unit of gamma or beta (`none` where there is no array or no column).
+template <class T, int U>
+__device__ __forceinline__ Unit<T, U> parameter_unit(const void *p, int col, int width, float none) {
+  Unit<T, U> v;
+  if (p && col < width)
+    v = *reinterpret_cast<const Unit<T, U> *>(static_cast<const T *>(p) + col);
+  else
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v.v[u] = from_float<T>(none);
   return v;
 }
 
-// T elements in units of U, C units per thread (columns (c G + t) U ...), a row per group of G
-// threads: G lanes of a warp (Warp), or the block.
-template <class T, int U, int C, bool Warp>
-__global__ void __launch_bounds__(Warp ? kWarpBlock : 1024) layer_norm_kernel(const __grid_constant__ Norm a, int lanes) {
-  constexpr bool Fast = sizeof(T) == 2;
+// Sums of R pairs of values, each over a row's group: G lanes (G <= 32, power of two), or the block.
+template <bool Warp, int R>
+__device__ __forceinline__ void group_sum(float2 (&v)[R], int G, float2 (*shared)[32]) {
+  for (int o = Warp ? G >> 1 : 16; o; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      v[r].x += __shfl_xor_sync(0xffffffffu, v[r].x, o);
+      v[r].y += __shfl_xor_sync(0xffffffffu, v[r].y, o);
+    }
+  if (Warp)
+    return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (!lane)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      shared[r][warp] = v[r];
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    v[r] = lane < warps ? shared[r][lane] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      v[r].x += __shfl_xor_sync(0xffffffffu, v[r].x, o);
+      v[r].y += __shfl_xor_sync(0xffffffffu, v[r].y, o);
+    }
+}
+
+// T elements in units of U, C units per thread (columns (c G + t) U ...), a row per group of G threads
+// -- G lanes of a warp (Threads = kWarpBlock), or a block of at most Threads -- and R rows per group
+// at once.
+template <class T, int U, int C, int R, int Threads>
+__global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_constant__ Norm a, int lanes) {
+  // Lanes with many columns find gamma and beta in shared memory, others in registers.
+  constexpr bool Fast = sizeof(T) == 2, Ahead = C * R <= 4, Warp = Threads == kWarpBlock,
+                 Shared = Warp && C >= kSharedChunks;
   using Un = Unit<T, U>;
-  __shared__ float2 shared[2][32];
+  __shared__ float2 shared[2][R][32];
+  extern __shared__ __align__(16) unsigned char parameters[]; // [2][C][32] units (Shared)
+  Un *const common = reinterpret_cast<Un *>(parameters);
   const int G = Warp ? lanes : blockDim.x, t = Warp ? threadIdx.x & (G - 1) : threadIdx.x;
-  const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0;
+  const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0, width = int(a.width);
   const T *x = static_cast<const T *>(a.x);
   T *y = static_cast<T *>(a.y);
-  const float inv_n = 1.f / float(a.width);
-  Un gamma[C], beta[C];
-  long long col[C];
-  bool live[C];
+  const float inv_n = 1.f / float(width);
+  const long long step = (long long)gridDim.x * per_block * R;
+  long long base = (long long)blockIdx.x * per_block * R;
+  auto col = [&](int c) { return (c * G + t) * U; };
+  Un own[2][Shared ? 1 : C];
+  if (Shared) { // unit by unit
+    for (int i = threadIdx.x; i < C * G; i += Threads) {
+      common[i] = parameter_unit<T, U>(a.gamma, i * U, width, 1.f);
+      common[C * 32 + i] = parameter_unit<T, U>(a.beta, i * U, width, 0.f);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    col[c] = (long long)(c * G + t) * U;
-    live[c] = col[c] < a.width;
-    if (live[c] && a.gamma)
-      gamma[c] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.gamma) + col[c]);
-    if (live[c] && a.beta)
-      beta[c] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.beta) + col[c]);
+    for (int c = 0; c < C; ++c) {
+      own[0][c] = parameter_unit<T, U>(a.gamma, col(c), width, 1.f);
+      own[1][c] = parameter_unit<T, U>(a.beta, col(c), width, 0.f);
+    }
   }
-  const long long step = (long long)gridDim.x * per_block;
-  long long base = (long long)blockIdx.x * per_block;
-  Un next[C];
-  auto load = [&](long long row) {
+  Un next[R][C];
+  auto load = [&](long long from) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (live[c] && row < a.rows)
-        next[c] = *reinterpret_cast<const Un *>(x + row * a.ldx + col[c]);
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        next[r][c] = load_unit<T, U>(x, a.ldx, from + r * per_block + group, a.rows, col(c), width);
   };
-  load(base + group);
+  if (Ahead)
+    load(base);
   for (; base < a.rows; base += step) {
-    const long long row = base + group;
-    const bool mine = row < a.rows;
-    float v[C * U];
-    float2 s = make_float2(0.f, 0.f);
+    if (!Ahead)
+      load(base);
+    Un raw[R][C];
+    float2 s[R];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int r = 0; r < R; ++r) {
+      s[r] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        v[c * U + u] = live[c] && mine ? to_float(next[c].v[u]) : 0.f;
-        s.x += v[c * U + u];
+      for (int c = 0; c < C; ++c) {
+        raw[r][c] = next[r][c];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          s[r].x += to_float(raw[r][c].v[u]);
       }
-    load(row + step);
-    const float m1 = group_sum<Warp>(s, G, shared[0]).x * inv_n;
-    s = make_float2(0.f, 0.f);
+    }
+    if (Ahead)
+      load(base + step);
+    group_sum<Warp, R>(s, G, shared[0]);
+    float m1[R], fix[R], rs[R];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (live[c])
+    for (int r = 0; r < R; ++r) {
+      m1[r] = s[r].x * inv_n;
+      s[r] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          float d = v[c * U + u] -= m1;
-          s.x += d;
-          s.y = fmaf(d, d, s.y);
+          const float d = col(c) < width ? to_float(raw[r][c].v[u]) - m1[r] : 0.f;
+          s[r].x += d;
+          s[r].y = fmaf(d, d, s[r].y);
         }
-    s = group_sum<Warp>(s, G, shared[1]);
-    // The first mean's rounding error, and the variance about the corrected mean.
-    const float fix = s.x * inv_n;
-    const float var = fmaxf(fmaf(-fix, fix, s.y * inv_n), 0.f) + (s.y != s.y ? s.y : 0.f);
-    const float r = Fast ? rsqrtf(var + a.eps) : 1.f / sqrtf(var + a.eps);
-    if (!mine)
-      continue;
-    if (a.mean && !t) {
-      a.mean[row] = m1 + fix;
-      a.rstd[row] = Fast ? 1.f / sqrtf(var + a.eps) : r;
+    }
+    group_sum<Warp, R>(s, G, shared[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      // The first mean's rounding error, and the variance about the corrected mean (NaN stays).
+      fix[r] = s[r].x * inv_n;
+      const float v = fmaf(-fix[r], fix[r], s[r].y * inv_n), var = v < 0.f ? 0.f : v;
+      rs[r] = Fast ? rsqrtf(var + a.eps) : 1.f / sqrtf(var + a.eps);
+      const long long row = base + r * per_block + group;
+      if (a.mean && !t && row < a.rows) {
+        a.mean[row] = m1[r] + fix[r];
+        a.rstd[row] = Fast ? 1.f / sqrtf(var + a.eps) : rs[r];
+      }
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      if (!live[c])
-        continue;
-      Un o;
+      const Un gamma = Shared ? common[c * G + t] : own[0][Shared ? 0 : c],
+               beta = Shared ? common[(32 * C + c * G) + t] : own[1][Shared ? 0 : c];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float z = (v[c * U + u] - fix) * r;
-        if (a.gamma)
-          z *= to_float(gamma[c].v[u]);
-        if (a.beta)
-          z += to_float(beta[c].v[u]);
-        o.v[u] = from_float<T>(activate<Fast>(z, a.activation));
+      for (int r = 0; r < R; ++r) {
+        const long long row = base + r * per_block + group;
+        float z[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          z[u] = fmaf((to_float(raw[r][c].v[u]) - m1[r] - fix[r]) * rs[r], to_float(gamma.v[u]), to_float(beta.v[u]));
+        activate_all<Fast>(z, a.activation);
+        Un o;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          o.v[u] = from_float<T>(z[u]);
+        if (row < a.rows && col(c) < width)
+          *reinterpret_cast<Un *>(y + row * a.ldy + col(c)) = o;
       }
-      *reinterpret_cast<Un *>(y + row * a.ldy + col[c]) = o;
     }
   }
 }
 
 // partial: [gridDim.x][2][width] (dgamma, dbeta), or NULL.
-template <class T, int U, int C, bool Warp>
-__global__ void __launch_bounds__(Warp ? kWarpBlock : 1024)
+template <class T, int U, int C, int R, int Threads>
+__global__ void __launch_bounds__(Threads)
     layer_norm_backward_kernel(const __grid_constant__ NormBackward a, int lanes, float *partial) {
-  constexpr bool Fast = sizeof(T) == 2;
+  constexpr bool Fast = sizeof(T) == 2, Warp = Threads == kWarpBlock;
   using Un = Unit<T, U>;
-  __shared__ float2 shared[2][32];
+  __shared__ float2 shared[2][R][32];
   __shared__ float join[Warp ? kWarpBlock * C * U : 1];
   const int G = Warp ? lanes : blockDim.x, t = Warp ? threadIdx.x & (G - 1) : threadIdx.x;
-  const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0;
+  const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0, width = int(a.width);
   const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
   T *dx = static_cast<T *>(a.dx);
   const float inv_n = 1.f / float(a.width);
+  auto col = [&](int c) { return (c * G + t) * U; };
   Un gamma[C], beta[C];
-  long long col[C];
-  bool live[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    col[c] = (long long)(c * G + t) * U;
-    live[c] = col[c] < a.width;
-    if (live[c] && a.gamma)
-      gamma[c] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.gamma) + col[c]);
-    if (live[c] && a.beta && a.activation != None)
-      beta[c] = *reinterpret_cast<const Un *>(static_cast<const T *>(a.beta) + col[c]);
+    gamma[c] = parameter_unit<T, U>(a.gamma, col(c), width, 1.f);
+    beta[c] = parameter_unit<T, U>(a.activation != None ? a.beta : nullptr, col(c), width, 0.f);
   }
   float sum_gamma[C * U] = {}, sum_beta[C * U] = {};
-  const long long step = (long long)gridDim.x * per_block;
-  long long base = (long long)blockIdx.x * per_block;
-  Un next_x[C], next_dy[C];
-  float next_mean = 0.f, next_r = 0.f;
-  auto load = [&](long long row) {
-    if (row >= a.rows)
-      return;
+  const long long step = (long long)gridDim.x * per_block * R;
+  long long base = (long long)blockIdx.x * per_block * R;
+  Un next_x[R][C], next_dy[R][C];
+  float next_mean[R], next_r[R];
+  // Rows and columns outside read as zero: they add nothing to any sum.
+  auto load = [&](long long from) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (live[c]) {
-        next_x[c] = *reinterpret_cast<const Un *>(x + row * a.ldx + col[c]);
-        next_dy[c] = *reinterpret_cast<const Un *>(dy + row * a.lddy + col[c]);
+    for (int r = 0; r < R; ++r) {
+      const long long row = from + r * per_block + group;
+      next_mean[r] = a.mean[min(row, a.rows - 1)];
+      next_r[r] = a.rstd[min(row, a.rows - 1)];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        next_x[r][c] = load_unit<T, U>(x, a.ldx, row, a.rows, col(c), width);
+        next_dy[r][c] = load_unit<T, U>(dy, a.lddy, row, a.rows, col(c), width);
       }
-    next_mean = a.mean[row];
-    next_r = a.rstd[row];
+    }
   };
-  load(base + group);
+  load(base);
   for (int k = 0; base < a.rows; base += step, k ^= 1) {
-    const long long row = base + group;
-    const bool mine = row < a.rows;
-    const float mean = next_mean, r = next_r;
-    float xh[C * U], g[C * U];
-    float2 s = make_float2(0.f, 0.f);
+    float xh[R][C * U], g[R][C * U], rs[R];
+    float2 s[R];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int r = 0; r < R; ++r) {
+      const float mean = next_mean[r];
+      rs[r] = next_r[r];
+      s[r] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = c * U + u;
-        xh[i] = g[i] = 0.f;
-        if (live[c] && mine) {
-          xh[i] = (to_float(next_x[c].v[u]) - mean) * r;
-          float gm = a.gamma ? to_float(gamma[c].v[u]) : 1.f, dz = to_float(next_dy[c].v[u]);
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = c * U + u;
+          // Outside, dy is 0; xhat is made 0 as well, its row's statistics need not be finite.
+          xh[r][i] = col(c) < width && base + r * per_block + group < a.rows ? (to_float(next_x[r][c].v[u]) - mean) * rs[r] : 0.f;
+          const float gm = to_float(gamma[c].v[u]);
+          float dz = to_float(next_dy[r][c].v[u]);
           if (a.activation != None)
-            dz *= slope<Fast>(fmaf(xh[i], gm, a.beta ? to_float(beta[c].v[u]) : 0.f), a.activation);
-          sum_gamma[i] = fmaf(dz, xh[i], sum_gamma[i]);
+            dz *= slope<Fast>(fmaf(xh[r][i], gm, to_float(beta[c].v[u])), a.activation);
+          sum_gamma[i] = fmaf(dz, xh[r][i], sum_gamma[i]);
           sum_beta[i] += dz;
-          g[i] = dz * gm;
-          s.x += g[i];
-          s.y = fmaf(g[i], xh[i], s.y);
+          g[r][i] = dz * gm;
+          s[r].x += g[r][i];
+          s[r].y = fmaf(g[r][i], xh[r][i], s[r].y);
         }
-      }
-    load(row + step);
+    }
+    load(base + step);
     if (!dx)
       continue;
-    s = group_sum<Warp>(s, G, shared[k]); // two buffers: a row's sums are read while the next are written
-    if (!mine)
-      continue;
-    const float mg = s.x * inv_n, mgx = s.y * inv_n;
+    group_sum<Warp, R>(s, G, shared[k]); // two buffers: sums are read while the next are written
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if (!live[c])
-        continue;
-      Un o;
+    for (int r = 0; r < R; ++r) {
+      const long long row = base + r * per_block + group;
+      const float mg = s[r].x * inv_n, mgx = s[r].y * inv_n;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        o.v[u] = from_float<T>(r * (g[c * U + u] - fmaf(xh[c * U + u], mgx, mg)));
-      *reinterpret_cast<Un *>(dx + row * a.lddx + col[c]) = o;
+      for (int c = 0; c < C; ++c) {
+        Un o;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          o.v[u] = from_float<T>(rs[r] * (g[r][c * U + u] - fmaf(xh[r][c * U + u], mgx, mg)));
+        if (col(c) < width && row < a.rows)
+          *reinterpret_cast<Un *>(dx + row * a.lddx + col(c)) = o;
+      }
     }
   }
   if (!partial)
@@ -225,25 +284,24 @@ __global__ void __launch_bounds__(Warp ? kWarpBlock : 1024)
     if (Warp) { // the block's groups hold the same columns: add them in group order
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < C * U; ++i) // group-major: [group][c][u][t]
+      for (int i = 0; i < C * U; ++i)
         join[(group * C * U + i) * G + t] = k ? sum_beta[i] : sum_gamma[i];
       __syncthreads();
       for (int j = threadIdx.x; j < C * U * G; j += kWarpBlock) {
-        int i = j / G, tt = j % G;
-        long long cc = (long long)((i / U) * G + tt) * U + i % U;
+        const int i = j / G, cc = ((i / U) * G + j % G) * U + i % U;
         float v = 0.f;
         for (int q = 0; q < per_block; ++q)
           v += join[q * C * U * G + j];
-        if (cc < a.width)
+        if (cc < width)
           out[cc] = v;
       }
     } else {
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        if (live[c])
+        if (col(c) < width)
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            out[col[c] + u] = k ? sum_beta[c * U + u] : sum_gamma[c * U + u];
+            out[col(c) + u] = k ? sum_beta[c * U + u] : sum_gamma[c * U + u];
     }
   }
 }
@@ -252,24 +310,25 @@ __global__ void __launch_bounds__(Warp ? kWarpBlock : 1024)
 constexpr int kWideThreads = 1024;
 template <class T> __global__ void __launch_bounds__(kWideThreads) wide_norm_kernel(const __grid_constant__ Norm a) {
   constexpr bool Fast = sizeof(T) == 2;
-  __shared__ float2 shared[2][32];
+  __shared__ float2 shared[2][1][32];
   const float inv_n = 1.f / float(a.width);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(a.x) + row * a.ldx;
     T *y = static_cast<T *>(a.y) + row * a.ldy;
-    float2 s = make_float2(0.f, 0.f);
+    float2 s[1] = {};
     for (long long i = threadIdx.x; i < a.width; i += kWideThreads)
-      s.x += to_float(x[i]);
-    const float m1 = group_sum<false>(s, 0, shared[0]).x * inv_n;
-    s = make_float2(0.f, 0.f);
+      s[0].x += to_float(x[i]);
+    group_sum<false, 1>(s, 0, shared[0]);
+    const float m1 = s[0].x * inv_n;
+    s[0] = make_float2(0.f, 0.f);
     for (long long i = threadIdx.x; i < a.width; i += kWideThreads) {
       float d = to_float(x[i]) - m1;
-      s.x += d;
-      s.y = fmaf(d, d, s.y);
+      s[0].x += d;
+      s[0].y = fmaf(d, d, s[0].y);
     }
-    s = group_sum<false>(s, 0, shared[1]);
-    const float fix = s.x * inv_n;
-    const float var = fmaxf(fmaf(-fix, fix, s.y * inv_n), 0.f) + (s.y != s.y ? s.y : 0.f);
+    group_sum<false, 1>(s, 0, shared[1]);
+    const float fix = s[0].x * inv_n;
+    const float v = fmaf(-fix, fix, s[0].y * inv_n), var = v < 0.f ? 0.f : v;
     const float r = 1.f / sqrtf(var + a.eps);
     if (a.mean && !threadIdx.x) {
       a.mean[row] = m1 + fix;
@@ -298,19 +357,19 @@ template <class T> __device__ __forceinline__ float2 wide_element(const NormBack
 }
 template <class T>
 __global__ void __launch_bounds__(kWideThreads) wide_norm_backward_kernel(const __grid_constant__ NormBackward a) {
-  __shared__ float2 shared[2][32];
+  __shared__ float2 shared[2][1][32];
   const float inv_n = 1.f / float(a.width);
   int k = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, k ^= 1) {
-    float2 s = make_float2(0.f, 0.f);
+    float2 s[1] = {};
     for (long long i = threadIdx.x; i < a.width; i += kWideThreads) {
       float2 e = wide_element<T>(a, row, i);
       float g = e.y * (a.gamma ? to_float(static_cast<const T *>(a.gamma)[i]) : 1.f);
-      s.x += g;
-      s.y = fmaf(g, e.x, s.y);
+      s[0].x += g;
+      s[0].y = fmaf(g, e.x, s[0].y);
     }
-    s = group_sum<false>(s, 0, shared[k]);
-    const float mg = s.x * inv_n, mgx = s.y * inv_n, r = a.rstd[row];
+    group_sum<false, 1>(s, 0, shared[k]);
+    const float mg = s[0].x * inv_n, mgx = s[0].y * inv_n, r = a.rstd[row];
     // dx may be dy: an element is read and written by the same thread.
     for (long long i = threadIdx.x; i < a.width; i += kWideThreads) {
       float2 e = wide_element<T>(a, row, i);
@@ -336,64 +395,76 @@ __global__ void __launch_bounds__(256) wide_params_kernel(const __grid_constant_
   out[a.width + i] = sb;
 }
 
-// How a row is laid over threads.
+// How a row is laid over threads: units of `unit` elements, `chunks` of them per thread.  Part of a warp
+// or a warp holds it where that leaves a lane at most 8 units (32 single elements), or backward, where
+// every column has two sums in registers as well, 2 (8); else a block, as small as its chunks allow,
+// so that several share an SM and one computes while another waits at its barrier.
 struct Shape {
-  int unit, chunks, threads; // threads: lanes of a warp, or the block's threads
-  bool warp, wide;
+  int unit, chunks, threads, most; // threads: lanes of a warp, or the block's threads; most: its class
+  bool wide;
 };
-Shape shape_of(int type, long long width, bool vectors) {
-  int unit = vectors ? 16 / bytes_of(type) : 1;
-  long long units = (width + unit - 1) / unit;
-  int most = vectors ? 4 : 16;
-  Shape s{unit, 1, 0, false, false};
-  if (units <= 32 * most) { // part of a warp, or a warp
-    while (units > 32ll * s.chunks)
-      s.chunks *= vectors ? 2 : 4;
-    s.warp = true;
-    s.threads = 1;
-    while ((long long)s.threads * s.chunks < units)
-      s.threads *= 2;
-    return s;
-  }
-  s.chunks = vectors ? (units <= 1024 ? 1 : units <= 2048 ? 2 : 4) : (units <= 4096 ? 4 : 16);
-  long long threads = (units + s.chunks - 1) / s.chunks;
-  if (threads > 1024) {
-    s.wide = true;
-    return s;
-  }
-  s.threads = int((threads + 31) / 32 * 32);
+Shape shape_of(int type, long long width, bool vectors, bool backward) {
+  Shape s{vectors ? 16 / bytes_of(type) : 1, 0, 1, kWarpBlock, false};
+  const long long units = (width + s.unit - 1) / s.unit;
+  static constexpr int kLane[4][5] = {{1, 8, 32}, {1, 8}, {1, 2, 4, 8}, {1, 2}}; // [vectors][backward]
+  static constexpr int kBlock[4][3] = {{8}, {4, 8}, {4}, {1, 2}};
+  for (const int *c = kLane[2 * vectors + backward]; *c; ++c)
+    if (units <= 32 * *c) {
+      s.chunks = *c;
+      while ((long long)s.threads * *c < units)
+        s.threads *= 2;
+      return s;
+    }
+  for (int most : {512, 1024})
+    for (const int *c = kBlock[2 * vectors + backward]; *c; ++c)
+      if (units <= (long long)most * *c) {
+        s.chunks = *c;
+        s.threads = int((units + 32 * *c - 1) / (32 * *c) * 32);
+        s.most = most;
+        return s;
+      }
+  s.wide = true;
   return s;
 }
-template <class F> void with_shape(const Shape &s, F &&f) {
-  auto chunks = [&](auto warp) {
-    using std::integral_constant;
-    if (s.unit > 1) {
-      if (s.chunks == 1)
-        f(std::true_type{}, integral_constant<int, 1>{}, warp);
-      else if (s.chunks == 2)
-        f(std::true_type{}, integral_constant<int, 2>{}, warp);
-      else
-        f(std::true_type{}, integral_constant<int, 4>{}, warp);
-    } else {
-      if (s.chunks == 1)
-        f(std::false_type{}, integral_constant<int, 1>{}, warp);
-      else if (s.chunks == 4)
-        f(std::false_type{}, integral_constant<int, 4>{}, warp);
-      else
-        f(std::false_type{}, integral_constant<int, 16>{}, warp);
-    }
+// Rows at once: several where a thread's share of one is small.
+template <bool Backward> constexpr int rows_of(int share, int most) {
+  return most == 1024 ? 1 : Backward ? (share <= 4 ? 4 : share <= 8 ? 2 : 1) : (share <= 8 ? 4 : 1);
+}
+// launch(unit, chunks, most) with the shape's values as constants.
+template <bool Backward, int V, class F> void with_shape(const Shape &s, F &&launch) {
+  bool done = false;
+  auto is = [&](auto u, auto c, auto most) {
+    if (done || s.chunks != decltype(c)::value || s.most != decltype(most)::value || (s.unit > 1) != (decltype(u)::value > 1))
+      return;
+    launch(u, c, most);
+    done = true;
   };
-  if (s.warp)
-    chunks(std::true_type{});
-  else
-    chunks(std::false_type{});
+  using std::integral_constant;
+  integral_constant<int, V> v;
+  integral_constant<int, 1> one;
+  integral_constant<int, 2> two;
+  integral_constant<int, 4> four;
+  integral_constant<int, 8> eight;
+  integral_constant<int, kWarpBlock> warps;
+  integral_constant<int, 512> small;
+  integral_constant<int, 1024> large;
+  is(v, one, warps), is(v, two, warps), is(one, one, warps), is(one, eight, warps);
+  is(one, eight, small), is(one, eight, large);
+  if constexpr (Backward) {
+    is(v, one, small), is(v, two, small), is(v, two, large), is(one, four, small);
+  } else {
+    is(v, four, warps), is(v, eight, warps), is(v, four, small), is(v, four, large);
+    is(one, integral_constant<int, 32>{}, warps);
+  }
+  if (!done)
+    throw lapis::Error("Layer norm has no kernel for this row length");
 }
 // Blocks that fit on the device at once (asked once per kernel, block size and thread).
-template <auto Kernel> int resident_blocks(int threads) {
+template <auto Kernel> int resident_blocks(int threads, int shared = 0) {
   static thread_local int known[33] = {};
   int &b = known[threads / 32];
   if (!b) {
-    lapis::check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, Kernel, threads, 0));
+    lapis::check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, Kernel, threads, shared));
     b = std::max(b, 1);
   }
   return b * sm_count();
@@ -410,18 +481,20 @@ void layer_norm(const Norm &a, cudaStream_t stream) {
     constexpr int V = 16 / int(sizeof(T));
     bool vectors = a.width % V == 0 && aligned16(a.x) && aligned16(a.y) && aligned16(a.gamma) &&
                    aligned16(a.beta) && (a.rows == 1 || (a.ldx % V == 0 && a.ldy % V == 0));
-    Shape s = shape_of(a.type, a.width, vectors);
+    Shape s = shape_of(a.type, a.width, vectors, false);
     if (s.wide) {
       int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_kernel<T>>(kWideThreads)));
       lapis::launch(wide_norm_kernel<T>, grid, kWideThreads, 0, stream, a);
     } else {
-      with_shape(s, [&](auto vec, auto chunks, auto warp) {
-        constexpr auto kernel =
-            layer_norm_kernel<T, decltype(vec)::value ? V : 1, decltype(chunks)::value, decltype(warp)::value>;
-        int threads = s.warp ? kWarpBlock : s.threads;
-        long long blocks = s.warp ? (a.rows + kWarpBlock / s.threads - 1) / (kWarpBlock / s.threads) : a.rows;
-        int grid = int(std::min<long long>(blocks, resident_blocks<kernel>(threads)));
-        lapis::launch(kernel, grid, threads, 0, stream, a, s.threads);
+      with_shape<false, V>(s, [&](auto unit, auto chunks, auto most) {
+        constexpr int U = decltype(unit)::value, C = decltype(chunks)::value, M = decltype(most)::value;
+        constexpr int R = rows_of<false>(C * U, M);
+        constexpr auto kernel = layer_norm_kernel<T, U, C, R, M>;
+        const int threads = M == kWarpBlock ? kWarpBlock : s.threads;
+        const long long high = (long long)R * (M == kWarpBlock ? kWarpBlock / s.threads : 1);
+        constexpr int shared = M == kWarpBlock && C >= kSharedChunks ? 2 * C * 32 * U * int(sizeof(T)) : 0;
+        const int grid = int(std::min<long long>((a.rows + high - 1) / high, resident_blocks<kernel>(threads, shared)));
+        lapis::launch(kernel, grid, threads, shared, stream, a, s.threads);
       });
     }
     lapis::check(cudaGetLastError());
@@ -444,7 +517,7 @@ void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t st
       bool vectors = a.width % V == 0 && aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) &&
                      aligned16(a.gamma) && aligned16(a.beta) &&
                      (a.rows == 1 || (a.ldx % V == 0 && a.lddy % V == 0 && a.lddx % V == 0));
-      Shape s = shape_of(a.type, a.width, vectors);
+      Shape s = shape_of(a.type, a.width, vectors, true);
       if (s.wide) {
         if (a.dx) {
           int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_backward_kernel<T>>(kWideThreads)));
@@ -463,12 +536,14 @@ void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t st
                           kWideThreads, 0, stream, a);
         }
       } else {
-        with_shape(s, [&](auto vec, auto chunks, auto warp) {
-          constexpr auto kernel =
-              layer_norm_backward_kernel<T, decltype(vec)::value ? V : 1, decltype(chunks)::value, decltype(warp)::value>;
-          int threads = s.warp ? kWarpBlock : s.threads;
-          long long blocks = s.warp ? (a.rows + kWarpBlock / s.threads - 1) / (kWarpBlock / s.threads) : a.rows;
-          parts = int(std::min<long long>({blocks, (long long)resident_blocks<kernel>(threads), (long long)kMostParts}));
+        with_shape<true, V>(s, [&](auto unit, auto chunks, auto most) {
+          constexpr int U = decltype(unit)::value, C = decltype(chunks)::value, M = decltype(most)::value;
+          constexpr int R = rows_of<true>(C * U, M);
+          constexpr auto kernel = layer_norm_backward_kernel<T, U, C, R, M>;
+          const int threads = M == kWarpBlock ? kWarpBlock : s.threads;
+          const long long high = (long long)R * (M == kWarpBlock ? kWarpBlock / s.threads : 1);
+          parts = int(std::min<long long>(
+              {(a.rows + high - 1) / high, (long long)resident_blocks<kernel>(threads), (long long)kMostParts}));
           lapis::launch(kernel, parts, threads, 0, stream, a, s.threads, partial);
         });
       }

@@ -221,7 +221,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, activation=None, keep=False):
     y = x.new_empty(shape)
     mean = rstd = None
     if keep:
-        mean, rstd = x.new_empty((2, *shape[:-1]), dtype=torch.float32).unbind(0)
+        mean, rstd = (x.new_empty(shape[:-1], dtype=torch.float32) for _ in range(2))
     if lib.mace_layer_norm(code, rows, width, px, ldx, _address(gamma), _address(beta), eps, act, y.data_ptr(), width,
                            _address(mean), _address(rstd), stream(device.index)):
         raise RuntimeError(_error(lib))
