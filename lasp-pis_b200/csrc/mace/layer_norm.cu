@@ -24,16 +24,21 @@ namespace {
 constexpr int kWarpBlock = 256; // threads of a block whose rows belong to warps or parts of them
 constexpr int kSharedChunks = 4; // forward: from as many units per lane on
 
-// A unit of row `row` (column col) of an array, or zeros where it is not live.  The load itself is
-// unconditional, from a place inside the array: a load under a branch is waited for where the
+// A unit of an array, or zeros where it is not live.  The load itself is unconditional, from a place
+// inside the array: a load under a branch is waited for where the
 // branches join, which leaves one in flight instead of all of a row's.
 template <class T, int U>
-__device__ __forceinline__ Unit<T, U> load_unit(const T *p, long long ld, long long row, long long rows, int col, int width) {
-  Unit<T, U> v = *reinterpret_cast<const Unit<T, U> *>(p + min(row, rows - 1) * ld + min(col, width - U));
-  const bool live = row < rows && col < width;
+__device__ __forceinline__ Unit<T, U> load_unit(const T *row, bool live, int col) {
+  Unit<T, U> v = *reinterpret_cast<const Unit<T, U> *>(row + col);
+  if constexpr (sizeof(v) >= 4) {
+    uint32_t w[sizeof(v) / 4];
+    memcpy(w, &v, sizeof v);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    v.v[u] = live ? v.v[u] : from_float<T>(0.f);
+    for (int i = 0; i < int(sizeof(v) / 4); ++i)
+      w[i] = live ? w[i] : 0u;
+    memcpy(&v, w, sizeof v);
+  } else if (!live)
+    v.v[0] = from_float<T>(0.f);
   return v;
 }
 // A unit of gamma or beta (`none` where there is no array or no column).
@@ -78,9 +83,73 @@ __device__ __forceinline__ void group_sum(float2 (&v)[R], int G, float2 (*shared
     }
 }
 
+// Arithmetic on pairs of floats (one instruction for two), where a thread's elements come in pairs.
+template <int N> __device__ __forceinline__ float sum_of(const float *v) {
+  if constexpr (N % 4 == 0) {
+    float2 a = make_float2(v[0], v[1]), b = make_float2(v[2], v[3]);
+#pragma unroll
+    for (int i = 4; i < N; i += 4) {
+      a = __fadd2_rn(a, make_float2(v[i], v[i + 1]));
+      b = __fadd2_rn(b, make_float2(v[i + 2], v[i + 3]));
+    }
+    a = __fadd2_rn(a, b);
+    return a.x + a.y;
+  } else {
+    float s = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      s += v[i];
+    return s;
+  }
+}
+// v = v a + b, element by element.
+template <int N> __device__ __forceinline__ void scale_shift(float *v, float a, float b) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(a, a), make_float2(b, b));
+      v[i] = r.x, v[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = fmaf(v[i], a, b);
+  }
+}
+// c + sum a b
+template <int N> __device__ __forceinline__ float dot_of(const float *a, const float *b, float c) {
+  if constexpr (N % 2 == 0) {
+    float2 s = make_float2(c, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      s = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
+    return s.x + s.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      c = fmaf(a[i], b[i], c);
+    return c;
+  }
+}
+// z = z a + b with arrays.
+template <int N> __device__ __forceinline__ void fma_all(float *z, const float *a, const float *b) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = __ffma2_rn(make_float2(z[i], z[i + 1]), make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      z[i] = r.x, z[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      z[i] = fmaf(z[i], a[i], b[i]);
+  }
+}
+
 // T elements in units of U, C units per thread (columns (c G + t) U ...), a row per group of G threads
 // -- G lanes of a warp (Threads = kWarpBlock), or a block of at most Threads -- and R rows per group
-// at once.
+// at once.  Instructions come next after bytes: at 6.5 TB/s an SM has 22 issue slots for each 16-bit
+// element, so elements are converted by words and handled in pairs.
 template <class T, int U, int C, int R, int Threads>
 __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_constant__ Norm a, int lanes) {
   // Lanes with many columns find gamma and beta in shared memory, others in registers.
@@ -88,7 +157,7 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
                  Shared = Warp && C >= kSharedChunks;
   using Un = Unit<T, U>;
   __shared__ float2 shared[2][R][32];
-  extern __shared__ __align__(16) unsigned char parameters[]; // [2][C][32] units (Shared)
+  extern __shared__ __align__(16) unsigned char parameters[]; // [2][32 C] units (Shared)
   Un *const common = reinterpret_cast<Un *>(parameters);
   const int G = Warp ? lanes : blockDim.x, t = Warp ? threadIdx.x & (G - 1) : threadIdx.x;
   const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0, width = int(a.width);
@@ -115,77 +184,77 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
   Un next[R][C];
   auto load = [&](long long from) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      const long long row = from + r * per_block + group;
+      const T *p = x + min(row, a.rows - 1) * a.ldx;
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        next[r][c] = load_unit<T, U>(x, a.ldx, from + r * per_block + group, a.rows, col(c), width);
+        next[r][c] = load_unit<T, U>(p, col(c) < width, min(col(c), width - U));
+    }
   };
   if (Ahead)
     load(base);
   for (; base < a.rows; base += step) {
     if (!Ahead)
       load(base);
-    Un raw[R][C];
+    float v[R][C * U];
     float2 s[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[r] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        raw[r][c] = next[r][c];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          s[r].x += to_float(raw[r][c].v[u]);
-      }
+      for (int c = 0; c < C; ++c)
+        unpack<T, U>(next[r][c], v[r] + c * U);
+      s[r] = make_float2(sum_of<C * U>(v[r]), 0.f);
     }
     if (Ahead)
       load(base + step);
     group_sum<Warp, R>(s, G, shared[0]);
-    float m1[R], fix[R], rs[R];
+    float mean[R], rs[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      m1[r] = s[r].x * inv_n;
-      s[r] = make_float2(0.f, 0.f);
+      mean[r] = s[r].x * inv_n;
+      scale_shift<C * U>(v[r], 1.f, -mean[r]);
 #pragma unroll
       for (int c = 0; c < C; ++c)
+        if (col(c) >= width)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float d = col(c) < width ? to_float(raw[r][c].v[u]) - m1[r] : 0.f;
-          s[r].x += d;
-          s[r].y = fmaf(d, d, s[r].y);
-        }
+          for (int u = 0; u < U; ++u)
+            v[r][c * U + u] = 0.f;
+      // Floats may lie far from zero against their spread: the centred values' own mean is the first
+      // mean's rounding error.  16-bit values with such a mean are coarser than that error.
+      s[r] = make_float2(Fast ? 0.f : sum_of<C * U>(v[r]), dot_of<C * U>(v[r], v[r], 0.f));
     }
     group_sum<Warp, R>(s, G, shared[1]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      // The first mean's rounding error, and the variance about the corrected mean (NaN stays).
-      fix[r] = s[r].x * inv_n;
-      const float v = fmaf(-fix[r], fix[r], s[r].y * inv_n), var = v < 0.f ? 0.f : v;
+      const float fix = s[r].x * inv_n;
+      const float w = fmaf(-fix, fix, s[r].y * inv_n), var = w < 0.f ? 0.f : w; // (NaN stays)
       rs[r] = Fast ? rsqrtf(var + a.eps) : 1.f / sqrtf(var + a.eps);
       const long long row = base + r * per_block + group;
       if (a.mean && !t && row < a.rows) {
-        a.mean[row] = m1[r] + fix[r];
+        a.mean[row] = mean[r] + fix;
         a.rstd[row] = Fast ? 1.f / sqrtf(var + a.eps) : rs[r];
       }
+      if (!Fast)
+        scale_shift<C * U>(v[r], 1.f, -fix);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const Un gamma = Shared ? common[c * G + t] : own[0][Shared ? 0 : c],
-               beta = Shared ? common[(32 * C + c * G) + t] : own[1][Shared ? 0 : c];
+      float gamma[U], beta[U];
+      unpack<T, U>(Shared ? common[c * G + t] : own[0][Shared ? 0 : c], gamma);
+      unpack<T, U>(Shared ? common[(32 * C + c * G) + t] : own[1][Shared ? 0 : c], beta);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const long long row = base + r * per_block + group;
         float z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          z[u] = fmaf((to_float(raw[r][c].v[u]) - m1[r] - fix[r]) * rs[r], to_float(gamma.v[u]), to_float(beta.v[u]));
+          z[u] = v[r][c * U + u];
+        scale_shift<U>(z, rs[r], 0.f);
+        fma_all<U>(z, gamma, beta);
         activate_all<Fast>(z, a.activation);
-        Un o;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          o.v[u] = from_float<T>(z[u]);
         if (row < a.rows && col(c) < width)
-          *reinterpret_cast<Un *>(y + row * a.ldy + col(c)) = o;
+          *reinterpret_cast<Un *>(y + row * a.ldy + col(c)) = pack<T, U>(z);
       }
     }
   }
@@ -196,14 +265,15 @@ template <class T, int U, int C, int R, int Threads>
 __global__ void __launch_bounds__(Threads)
     layer_norm_backward_kernel(const __grid_constant__ NormBackward a, int lanes, float *partial) {
   constexpr bool Fast = sizeof(T) == 2, Warp = Threads == kWarpBlock;
+  constexpr int N = C * U;
   using Un = Unit<T, U>;
   __shared__ float2 shared[2][R][32];
-  __shared__ float join[Warp ? kWarpBlock * C * U : 1];
+  __shared__ float join[Warp ? kWarpBlock * N : 1];
   const int G = Warp ? lanes : blockDim.x, t = Warp ? threadIdx.x & (G - 1) : threadIdx.x;
   const int per_block = Warp ? kWarpBlock / G : 1, group = Warp ? threadIdx.x / G : 0, width = int(a.width);
   const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
   T *dx = static_cast<T *>(a.dx);
-  const float inv_n = 1.f / float(a.width);
+  const float inv_n = 1.f / float(width);
   auto col = [&](int c) { return (c * G + t) * U; };
   Un gamma[C], beta[C];
 #pragma unroll
@@ -211,51 +281,85 @@ __global__ void __launch_bounds__(Threads)
     gamma[c] = parameter_unit<T, U>(a.gamma, col(c), width, 1.f);
     beta[c] = parameter_unit<T, U>(a.activation != None ? a.beta : nullptr, col(c), width, 0.f);
   }
-  float sum_gamma[C * U] = {}, sum_beta[C * U] = {};
+  float sum_gamma[N] = {}, sum_beta[N] = {};
   const long long step = (long long)gridDim.x * per_block * R;
   long long base = (long long)blockIdx.x * per_block * R;
   Un next_x[R][C], next_dy[R][C];
   float next_mean[R], next_r[R];
-  // Rows and columns outside read as zero: they add nothing to any sum.
+  // Rows and columns outside: dy reads as zero, so they add nothing to any sum.
   auto load = [&](long long from) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = from + r * per_block + group;
-      next_mean[r] = a.mean[min(row, a.rows - 1)];
-      next_r[r] = a.rstd[min(row, a.rows - 1)];
+      const long long row = from + r * per_block + group, in = min(row, a.rows - 1);
+      next_mean[r] = a.mean[in];
+      next_r[r] = a.rstd[in];
+      const T *px = x + in * a.ldx, *pd = dy + in * a.lddy;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        next_x[r][c] = load_unit<T, U>(x, a.ldx, row, a.rows, col(c), width);
-        next_dy[r][c] = load_unit<T, U>(dy, a.lddy, row, a.rows, col(c), width);
+        const int at = min(col(c), width - U);
+        next_x[r][c] = load_unit<T, U>(px, col(c) < width && row < a.rows, at);
+        next_dy[r][c] = load_unit<T, U>(pd, col(c) < width && row < a.rows, at);
       }
     }
   };
   load(base);
   for (int k = 0; base < a.rows; base += step, k ^= 1) {
-    float xh[R][C * U], g[R][C * U], rs[R];
+    float xh[R][N], g[R][N], rs[R];
     float2 s[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      const bool mine = base + r * per_block + group < a.rows;
       const float mean = next_mean[r];
       rs[r] = next_r[r];
-      s[r] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        unpack<T, U>(next_x[r][c], xh[r] + c * U);
+        unpack<T, U>(next_dy[r][c], g[r] + c * U);
+      }
+      scale_shift<N>(xh[r], 1.f, -mean);
+      scale_shift<N>(xh[r], rs[r], 0.f);
+#pragma unroll
+      for (int c = 0; c < C; ++c) // outside xhat is 0 too: its row's statistics need not be finite
+        if (col(c) >= width || !mine)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            xh[r][c * U + u] = 0.f;
+      float gm[N];
 #pragma unroll
       for (int c = 0; c < C; ++c)
+        unpack<T, U>(gamma[c], gm + c * U);
+      if (a.activation != None) {
+        float z[N];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = c * U + u;
-          // Outside, dy is 0; xhat is made 0 as well, its row's statistics need not be finite.
-          xh[r][i] = col(c) < width && base + r * per_block + group < a.rows ? (to_float(next_x[r][c].v[u]) - mean) * rs[r] : 0.f;
-          const float gm = to_float(gamma[c].v[u]);
-          float dz = to_float(next_dy[r][c].v[u]);
-          if (a.activation != None)
-            dz *= slope<Fast>(fmaf(xh[r][i], gm, to_float(beta[c].v[u])), a.activation);
-          sum_gamma[i] = fmaf(dz, xh[r][i], sum_gamma[i]);
-          sum_beta[i] += dz;
-          g[r][i] = dz * gm;
-          s[r].x += g[r][i];
-          s[r].y = fmaf(g[r][i], xh[r][i], s[r].y);
+        for (int c = 0; c < C; ++c)
+          unpack<T, U>(beta[c], z + c * U);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          z[i] = fmaf(xh[r][i], gm[i], z[i]);
+        slope_all<Fast>(z, a.activation);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          g[r][i] *= z[i];
+      }
+      const float none[N] = {};
+      if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const float2 d = make_float2(g[r][i], g[r][i + 1]);
+          const float2 p = __ffma2_rn(d, make_float2(xh[r][i], xh[r][i + 1]), make_float2(sum_gamma[i], sum_gamma[i + 1]));
+          const float2 q = __fadd2_rn(d, make_float2(sum_beta[i], sum_beta[i + 1]));
+          sum_gamma[i] = p.x, sum_gamma[i + 1] = p.y;
+          sum_beta[i] = q.x, sum_beta[i + 1] = q.y;
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sum_gamma[i] = fmaf(g[r][i], xh[r][i], sum_gamma[i]);
+          sum_beta[i] += g[r][i];
+        }
+      }
+      fma_all<N>(g[r], gm, none);
+      s[r] = make_float2(sum_of<N>(g[r]), dot_of<N>(g[r], xh[r], 0.f));
     }
     load(base + step);
     if (!dx)
@@ -265,15 +369,24 @@ __global__ void __launch_bounds__(Threads)
     for (int r = 0; r < R; ++r) {
       const long long row = base + r * per_block + group;
       const float mg = s[r].x * inv_n, mgx = s[r].y * inv_n;
+      scale_shift<N>(xh[r], -mgx, -mg);
+      float o[N];
+      if constexpr (N % 2 == 0) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        Un o;
+        for (int i = 0; i < N; i += 2) {
+          const float2 f = __fmul2_rn(__fadd2_rn(make_float2(g[r][i], g[r][i + 1]), make_float2(xh[r][i], xh[r][i + 1])),
+                                      make_float2(rs[r], rs[r]));
+          o[i] = f.x, o[i + 1] = f.y;
+        }
+      } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          o.v[u] = from_float<T>(rs[r] * (g[r][c * U + u] - fmaf(xh[r][c * U + u], mgx, mg)));
-        if (col(c) < width && row < a.rows)
-          *reinterpret_cast<Un *>(dx + row * a.lddx + col(c)) = o;
+        for (int i = 0; i < N; ++i)
+          o[i] = rs[r] * (g[r][i] + xh[r][i]);
       }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (col(c) < width && row < a.rows)
+          *reinterpret_cast<Un *>(dx + row * a.lddx + col(c)) = pack<T, U>(o + c * U);
     }
   }
   if (!partial)
@@ -284,14 +397,14 @@ __global__ void __launch_bounds__(Threads)
     if (Warp) { // the block's groups hold the same columns: add them in group order
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < C * U; ++i)
-        join[(group * C * U + i) * G + t] = k ? sum_beta[i] : sum_gamma[i];
+      for (int i = 0; i < N; ++i)
+        join[(group * N + i) * G + t] = k ? sum_beta[i] : sum_gamma[i];
       __syncthreads();
-      for (int j = threadIdx.x; j < C * U * G; j += kWarpBlock) {
+      for (int j = threadIdx.x; j < N * G; j += kWarpBlock) {
         const int i = j / G, cc = ((i / U) * G + j % G) * U + i % U;
         float v = 0.f;
         for (int q = 0; q < per_block; ++q)
-          v += join[q * C * U * G + j];
+          v += join[q * N * G + j];
         if (cc < width)
           out[cc] = v;
       }

@@ -5,6 +5,7 @@
 #include "../lapis/launch.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cstring>
 
 namespace mace {
 namespace op {
@@ -20,6 +21,52 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <class T, int U> struct alignas(sizeof(T) * U) Unit {
   T v[U];
 };
+// Two 16-bit elements of one word.
+__device__ __forceinline__ float2 to_floats(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 to_floats(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t to_word(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t to_word(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// A unit to floats and back, whole words at a time.
+template <class T, int U> __device__ __forceinline__ void unpack(const Unit<T, U> &u, float *v) {
+  if constexpr (sizeof(T) == 2 && U > 1) {
+    uint32_t w[U / 2];
+    memcpy(w, &u, sizeof u);
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) {
+      const float2 f = to_floats(T{}, w[i]);
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      v[i] = to_float(u.v[i]);
+  }
+}
+template <class T, int U> __device__ __forceinline__ Unit<T, U> pack(const float *v) {
+  Unit<T, U> u;
+  if constexpr (sizeof(T) == 2 && U > 1) {
+    uint32_t w[U / 2];
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i)
+      w[i] = to_word(T{}, v[2 * i], v[2 * i + 1]);
+    memcpy(&u, w, sizeof u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      u.v[i] = from_float<T>(v[i]);
+  }
+  return u;
+}
 
 // 1 + exp(-z).  16-bit results take the fast exponential (2^-21 of the value and a little more for
 // large |z|, far below their own rounding).  The quotients below take the fast division (2 ulp): the
@@ -65,6 +112,22 @@ template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
   if (act == Relu)
     return z <= 0.f ? 0.f : 1.f; // NaN passes the gradient, as a comparison that fails
   return 1.f;
+}
+// The slopes of N values in their place.
+template <bool Fast, int N> __device__ __forceinline__ void slope_all(float (&v)[N], int act) {
+  if (act == Silu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = slope<Fast>(v[i], Silu);
+  } else if (act == Gelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = slope<Fast>(v[i], Gelu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = slope<Fast>(v[i], act);
+  }
 }
 
 // Second stage of a sum over rows: out_k[c] = sum over p < parts of partial[p][k][c], k < 2
