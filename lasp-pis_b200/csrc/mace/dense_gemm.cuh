@@ -30,6 +30,7 @@ struct Epilogue {
 struct Boxes {
   CUtensorMap y, z, residual; // y: the parts, when K is cut
   int on;
+  int sectors; // rows of all of them begin and end with whole 32-byte sectors
 };
 struct Product {
   int type;
@@ -187,6 +188,87 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
     }
   }
   send(m.y, plain ? part : 0);
+}
+
+// 32 bytes at once (aligned to 32).
+__device__ __forceinline__ void store32(void *p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32(const void *p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+// The residual of 32 columns of a lane's row, for finish_row.
+template <class T> struct Sectors {
+  static constexpr int S = 32 / int(sizeof(T)); // elements of a sector
+  uint32_t w[32 / S][8];
+  __device__ __forceinline__ void load(const Epilogue &e, long long I, long long J, long long row, long long col0) {
+#pragma unroll
+    for (int k = 0; k < 32; k += S)
+      if (row < I && col0 + k < J)
+        load32(static_cast<const T *>(e.residual) + row * e.ldr + col0 + k, w[k / S]);
+  }
+};
+// 32 columns of a lane's row from col0, for rows of whole sectors (Boxes::sectors): each lane writes its
+// row 32 bytes at a time, a sector each, with nothing staged and nothing waited for (bf16 84613 x 64
+// -> 1280: 50 us, 62 through boxes; float rows, twice as long, take longer this way: 227 us, 195).  bias: in shared memory.  part: the float values as they are,
+// to that array.
+template <class T>
+__device__ __forceinline__ void finish_row(const Epilogue &e, float *part, long long I, long long J, long long row,
+                                           long long col0, float (&v)[32], const T *bias, const Sectors<T> &residual) {
+  constexpr bool Fast = sizeof(T) == 2;
+  if (part) {
+    if (row < I)
+#pragma unroll
+      for (int k = 0; k < 32; k += 8)
+        if (col0 + k < J) {
+          uint32_t w[8];
+          memcpy(w, v + k, 32);
+          store32(part + row * J + col0 + k, w);
+        }
+    return;
+  }
+  constexpr int S = Sectors<T>::S;
+  if (e.bias) {
+    constexpr int U = 16 / int(sizeof(T));
+#pragma unroll
+    for (int i = 0; i < 32; i += U) {
+      float b[U];
+      unpack<T, U>(*reinterpret_cast<const Unit<T, U> *>(bias + i), b);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[i + u] += b[u];
+    }
+  }
+  auto write = [&](void *out, long long ld) {
+#pragma unroll
+    for (int k = 0; k < 32; k += S)
+      if (row < I && col0 + k < J) {
+        const Unit<T, S> o = pack<T, S>(v + k);
+        uint32_t w[8];
+        memcpy(w, &o, 32);
+        store32(static_cast<T *>(out) + row * ld + col0 + k, w);
+      }
+  };
+  if (e.z)
+    write(e.z, e.ldz);
+  activate_all<Fast>(v, e.activation);
+  if (e.residual)
+#pragma unroll
+    for (int k = 0; k < 32; k += S) {
+      Unit<T, S> o;
+      memcpy(&o, residual.w[k / S], 32);
+      float f[S];
+      unpack<T, S>(o, f);
+#pragma unroll
+      for (int u = 0; u < S; ++u)
+        v[k + u] += f[u];
+    }
+  write(e.out, e.ldo);
 }
 
 // A warp's 32 x 32 block where rows allow no boxes: through its box (columns permuted by row), so that

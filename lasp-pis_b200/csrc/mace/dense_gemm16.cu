@@ -179,10 +179,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
       tiles.at(u - s * tiles.count, i, j);
       if (!g.partial)
         fetch_bias<T>(g.e, g.J, j * BN + (BN >= 128 ? half * (BN / 2) : 0), BN >= 128 ? BN / 2 : 64, bias);
+      const long long row0 = i * kBM + 32 * quarter;
+      Sectors<T> residual; // of the next 32 columns, on its way before they are
+      if (g.boxes.sectors && BN >= 128 && g.e.residual && !g.partial)
+        residual.load(g.e, g.I, g.J, row0 + lane, j * BN + half * (BN / 2));
       ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(tile / 2) & 1, &abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const long long row0 = i * kBM + 32 * quarter;
       const uint32_t d = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN);
       auto get = [&](int c, float (&v)[32]) { // the tile's columns c ..
         uint32_t r[32];
@@ -195,7 +198,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
       };
       const int first = half * (BN / 2), end = first + BN / 2;
       if (row0 < g.I) {
-        if (g.boxes.on && g.partial) {
+        if (g.boxes.sectors && BN >= 128) {
+          float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
+#pragma unroll 1
+          for (int c = first; c < end && j * BN + c < g.J; c += 32) {
+            const Sectors<T> now = residual;
+            if (g.e.residual && c + 32 < end)
+              residual.load(g.e, g.I, g.J, row0 + lane, j * BN + c + 32);
+            float v[32];
+            get(c, v);
+            finish_row<T>(g.e, partial, g.I, g.J, row0 + lane, j * BN + c, v, bias + c - first, now);
+          }
+        } else if (g.boxes.on && g.partial) {
 #pragma unroll 1
           for (int c = first; c < end && j * BN + c < g.J; c += 32)
             finish_box<float>(g.e, g.boxes, row0, j * BN + c, int(s), w, phase, false,
@@ -265,8 +279,8 @@ __global__ void __launch_bounds__(256) finish_parts_kernel(const __grid_constant
   }
 }
 
-// A tile twice as wide costs less than twice the time (P is read once);
-// few tiles are cut along K until they fill the device, parts of at least four slabs.
+// A narrower tile saves little: at K = 4096 a 128 x 256 tile takes 28 us, a 128 x 128 one 24 us (P's
+// shared-memory reads bound both); few tiles are cut along K until they fill the device, parts of at least four slabs.
 } // namespace
 Plan plan16(long long I, long long J, long long K) {
   const int sms = sm_count();
@@ -277,7 +291,7 @@ Plan plan16(long long I, long long J, long long K) {
     long long tiles = (I + kBM - 1) / kBM * ((J + bn - 1) / bn);
     int parts = int(std::min<long long>({std::max(1ll, sms / tiles), std::max(1ll, slabs / 4), 64}));
     long long waves = (tiles * parts + sms - 1) / sms;
-    double c = double(waves) * double((slabs + parts - 1) / parts) * (bn == 256 ? 1. : bn == 128 ? .56 : .36);
+    double c = double(waves) * double((slabs + parts - 1) / parts) * (bn == 256 ? 1. : bn == 128 ? .85 : .75);
     if (!best.bn || c < cost)
       best = {bn, parts}, cost = c;
   }
@@ -340,6 +354,12 @@ CUtensorMap tile_map(int type, const void *base, long long rows, long long cols,
 Boxes boxes_of(const Product &p, float *partial, int parts) {
   Boxes b{};
   const Epilogue &e = p.e;
+  auto sectors = [&](const void *a, long long ld) {
+    return !a || (reinterpret_cast<uintptr_t>(a) % 32 == 0 && (p.I <= 1 || ld * bytes_of(p.type) % 32 == 0));
+  };
+  b.sectors = partial ? p.J % 8 == 0 && reinterpret_cast<uintptr_t>(partial) % 32 == 0
+                      : p.J * bytes_of(p.type) % 32 == 0 && sectors(e.out, e.ldo) && sectors(e.z, e.ldz) &&
+                            sectors(e.residual, e.ldr);
   if (partial) {
     b.on = p.J % 4 == 0;
     if (b.on)

@@ -74,9 +74,30 @@ template <class T, int U> __device__ __forceinline__ Unit<T, U> pack(const float
 template <bool Fast> __device__ __forceinline__ float exp_plus_one(float z) {
   return 1.f + (Fast ? __expf(-z) : expf(-z));
 }
+// Phi(-m) for m >= 0, as exp(-m^2 / 2) g(m): g, a scaled complementary error function, is a polynomial
+// in t = 1 / (1 + 0.32 m), fitted here for the least relative error (4.4e-7).  e: the exponential.
+// For 16-bit results (15 instructions, no branch; erff takes twice that).
+__device__ __forceinline__ float normal_tail(float m, float &e) {
+  const float t = __fdividef(1.f, fmaf(0.32f, m, 1.f));
+  e = __expf(-0.5f * m * m);
+  float q = 0.03452073782682419f;
+  q = fmaf(q, t, -0.12243109941482544f);
+  q = fmaf(q, t, 0.10611509531736374f);
+  q = fmaf(q, t, 0.015589500777423382f);
+  q = fmaf(q, t, 0.09737381339073181f);
+  q = fmaf(q, t, 0.11343884468078613f);
+  q = fmaf(q, t, 0.12773342430591583f);
+  q = fmaf(q, t, 0.1276599019765854f);
+  return q * t * e;
+}
 template <bool Fast> __device__ __forceinline__ float activate(float z, int act) {
   if (act == Silu)
     return __fdividef(z, exp_plus_one<Fast>(z));
+  if (act == Gelu && Fast) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the tail is 0 from 40 on, NaN stays
+    const float m = fminf(fabsf(z), 40.f);
+    float e;
+    return fmaf(-m, normal_tail(m, e), z < 0.f ? 0.f : z);
+  }
   if (act == Gelu)
     return 0.5f * z * (1.f + erff(z * 0.70710678f));
   if (act == Relu)
@@ -105,8 +126,14 @@ template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
     float s = __fdividef(1.f, exp_plus_one<Fast>(z));
     return s * (1.f + z * (1.f - s));
   }
+  if (act == Gelu && Fast) {
+    const float m = fminf(fabsf(z), 40.f);
+    float e;
+    const float h = normal_tail(m, e), s = fmaf(copysignf(m, z), e * 0.39894228f, z < 0.f ? h : 1.f - h);
+    return z != z ? z : s;
+  }
   if (act == Gelu) {
-    float e = Fast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+    float e = expf(-0.5f * z * z);
     return 0.5f * (1.f + erff(z * 0.70710678f)) + z * e * 0.39894228f;
   }
   if (act == Relu)

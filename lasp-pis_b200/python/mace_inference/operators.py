@@ -128,8 +128,14 @@ def _size(lib, key, call, *args):
     return size
 
 
-def _workspace(torch, size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _workspace(x, code, size):
+    """`size` bytes (a multiple of 16) beside x."""
+    return x.new_empty(size >> (1 if code else 2)) if size else None
+
+
+def _new_like(t, torch):
+    """A new contiguous tensor like t (empty_like costs half of new_empty, but keeps other layouts)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def dense(x, weight, bias=None, activation=None, residual=None, keep=False):
@@ -156,10 +162,10 @@ def dense(x, weight, bias=None, activation=None, residual=None, keep=False):
     x, px, ldx = _rows(x)
     weight, pw, ldw = _rows(weight)
     y = x.new_empty(shape)
-    z = x.new_empty(shape) if keep else None
+    z = torch.empty_like(y) if keep else None
     size = _size(lib, (0, code, rows, inputs, outputs, px & 15, ldx, pw & 15, ldw, device.index),
                  lib.mace_dense_workspace, code, rows, inputs, outputs, px, ldx, pw, ldw)
-    ws = _workspace(torch, size, device)
+    ws = _workspace(x, code, size)
     if lib.mace_dense(code, rows, inputs, outputs, px, ldx, pw, ldw, _address(bias), act, pr, ldr, y.data_ptr(), outputs,
                       _address(z), outputs, _address(ws), size, stream(device.index)):
         raise RuntimeError(_error(lib))
@@ -191,11 +197,11 @@ def dense_backward(dy, x, weight, activation=None, z=None, need=(True, True, Tru
     x, px, ldx = _rows(x)
     weight, pw, ldw = _rows(weight)
     dx = x.new_empty(shape) if need[0] else None
-    dweight = x.new_empty((outputs, inputs)) if need[1] else None
-    dbias = x.new_empty((outputs,)) if need[2] else None
+    dweight = _new_like(weight, torch) if need[1] else None
+    dbias = x.new_empty(outputs) if need[2] else None
     size = _size(lib, (1, code, rows, inputs, outputs, pd & 15, ldd, px & 15, ldx, pw & 15, ldw, act, device.index),
                  lib.mace_dense_backward_workspace, code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act)
-    ws = _workspace(torch, size, device)
+    ws = _workspace(x, code, size)
     if lib.mace_dense_backward(code, rows, inputs, outputs, pd, ldd, px, ldx, pw, ldw, act, pz, ldz, _address(dx), inputs,
                                _address(dweight), inputs, _address(dbias), _address(ws), size, stream(device.index)):
         raise RuntimeError(_error(lib))
@@ -218,10 +224,11 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, activation=None, keep=False):
     if beta is not None:
         beta = _flat(_like(beta, "beta", torch, (width,), dtype, device))
     x, px, ldx = _rows(x)
-    y = x.new_empty(shape)
+    y = _new_like(x, torch) if x.dim() == len(shape) else x.new_empty(shape)
     mean = rstd = None
     if keep:
-        mean, rstd = (x.new_empty(shape[:-1], dtype=torch.float32) for _ in range(2))
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if lib.mace_layer_norm(code, rows, width, px, ldx, _address(gamma), _address(beta), eps, act, y.data_ptr(), width,
                            _address(mean), _address(rstd), stream(device.index)):
         raise RuntimeError(_error(lib))
@@ -249,13 +256,15 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, beta=None, activation=Non
     mean = _flat(_like(mean, "mean", torch, shape[:-1], torch.float32, device))
     rstd = _flat(_like(rstd, "rstd", torch, shape[:-1], torch.float32, device))
     x, px, ldx = _rows(x)
-    dx = x.new_empty(shape) if need[0] else None
-    dgamma = x.new_empty((width,)) if need[1] else None
-    dbeta = x.new_empty((width,)) if need[2] else None
+    dx = None
+    if need[0]:
+        dx = _new_like(x, torch) if x.dim() == len(shape) else x.new_empty(shape)
+    dgamma = x.new_empty(width) if need[1] else None
+    dbeta = x.new_empty(width) if need[2] else None
     size = 0
     if need[1] or need[2]:
         size = _size(lib, (2, code, rows, width, device.index), lib.mace_layer_norm_backward_workspace, code, rows, width)
-    ws = _workspace(torch, size, device)
+    ws = _workspace(x, code, size)
     if lib.mace_layer_norm_backward(code, rows, width, pd, ldd, px, ldx, mean.data_ptr(), rstd.data_ptr(),
                                     _address(gamma), _address(beta), act, _address(dx), width, _address(dgamma),
                                     _address(dbeta), _address(ws), size, stream(device.index)):
