@@ -15,6 +15,7 @@
 // parameters' gradients stay in registers too; each block writes one partial row of dgamma and
 // dbeta, and a second launch adds the partial rows in a fixed order.
 #include "operators.cuh"
+#include "tcgen05.cuh"
 #include <algorithm>
 #include <type_traits>
 
@@ -508,6 +509,208 @@ __global__ void __launch_bounds__(256) wide_params_kernel(const __grid_constant_
   out[a.width + i] = sb;
 }
 
+// ---------------- rows that start anywhere, in one contiguous array ----------------
+// Odd widths leave a row no wide loads, but 8 rows together start and end on 16-byte boundaries: a block
+// copies a span of 8 k whole rows into shared memory (one bulk copy per array, the last few bytes of
+// the array one by one), works on it element by element there and sends the result back the same
+// way.  Several blocks share an SM, so one computes while another's copies are under way.
+// f16 8191 x 2053, backward: single-element loads take 105 us.
+constexpr int kSpanThreads = 256;
+struct Span {
+  int rows, bytes; // of a span; bytes rounded up to 16
+};
+// Starts the copies of `elements` elements of `arrays` spans, and waits for them.
+template <class T>
+__device__ __forceinline__ bool bring_spans(const T *const (&from)[2], T *const (&to)[2], int arrays, int elements,
+                                            unsigned bar, unsigned phase) {
+  const unsigned whole = unsigned(elements) * unsigned(sizeof(T)) & ~15u;
+  if (whole && threadIdx.x == 0) {
+    tc::mbar_expect_tx(bar, whole * unsigned(arrays));
+    for (int k = 0; k < arrays; ++k)
+      tc::bulk_load(tc::smem_u32(to[k]), from[k], whole, bar);
+  }
+  for (int k = 0; k < arrays; ++k)
+    for (int i = int(whole / sizeof(T)) + int(threadIdx.x); i < elements; i += kSpanThreads)
+      to[k][i] = from[k][i];
+  bool there = true;
+  if (whole) {
+    const long long start = clock64();
+    while (!(there = tc::mbar_try(bar, phase)) && clock64() - start < tc::kWaitCycles) {
+    }
+  }
+  return __syncthreads_and(there);
+}
+template <class T> __device__ __forceinline__ void send_span(T *to, const T *from, int elements) {
+  const unsigned whole = unsigned(elements) * unsigned(sizeof(T)) & ~15u;
+  tc::fence_proxy_async_smem();
+  __syncthreads();
+  if (whole && threadIdx.x == 0) {
+    tc::bulk_store(to, tc::smem_u32(from), whole);
+    tc::bulk_commit();
+    tc::bulk_wait_read();
+  }
+  for (int i = int(whole / sizeof(T)) + int(threadIdx.x); i < elements; i += kSpanThreads)
+    to[i] = from[i];
+  __syncthreads();
+}
+// gamma and beta (1 and 0 where there is none) into shared memory.
+template <class T> __device__ __forceinline__ void bring_parameters(const void *gamma, const void *beta, int width, T *to) {
+  for (int i = threadIdx.x; i < width; i += kSpanThreads) {
+    to[i] = gamma ? static_cast<const T *>(gamma)[i] : from_float<T>(1.f);
+    to[width + i] = beta ? static_cast<const T *>(beta)[i] : from_float<T>(0.f);
+  }
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A warp per row.
+template <class T>
+__global__ void __launch_bounds__(kSpanThreads) span_norm_kernel(const __grid_constant__ Norm a, Span span) {
+  constexpr bool Fast = sizeof(T) == 2;
+  extern __shared__ __align__(16) unsigned char parameters[];
+  __shared__ uint64_t bar;
+  T *x = reinterpret_cast<T *>(parameters), *gamma = reinterpret_cast<T *>(parameters + span.bytes), *beta = gamma + a.width;
+  const int width = int(a.width), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float inv_n = 1.f / float(width);
+  if (threadIdx.x == 0) {
+    tc::mbar_init(tc::smem_u32(&bar), 1);
+    tc::fence_proxy_async_smem();
+  }
+  bring_parameters(a.gamma, a.beta, width, gamma);
+  __syncthreads();
+  unsigned phase = 0;
+  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows, phase ^= 1) {
+    const int rows = int(min((long long)span.rows, a.rows - first)), elements = rows * width;
+    const T *from[2] = {static_cast<const T *>(a.x) + first * width, nullptr};
+    T *const to[2] = {x, nullptr};
+    const bool there = bring_spans<T>(from, to, 1, elements, tc::smem_u32(&bar), phase);
+    for (int r = warp; r < rows; r += kSpanThreads / 32) {
+      T *row = x + r * width;
+      float s = 0.f, q = 0.f;
+#pragma unroll 8
+      for (int c = lane; c < width; c += 32)
+        s += to_float(row[c]);
+      const float m1 = warp_sum(s) * inv_n;
+      s = 0.f;
+#pragma unroll 8
+      for (int c = lane; c < width; c += 32) {
+        const float d = to_float(row[c]) - m1;
+        s += d;
+        q = fmaf(d, d, q);
+      }
+      const float fix = warp_sum(s) * inv_n, v = fmaf(-fix, fix, warp_sum(q) * inv_n), var = v < 0.f ? 0.f : v;
+      // A wait that ran out shows as NaN.
+      const float rs = there ? 1.f / sqrtf(var + a.eps) : __uint_as_float(0x7fc00000u);
+      if (a.mean && !lane) {
+        a.mean[first + r] = m1 + fix;
+        a.rstd[first + r] = rs;
+      }
+      for (int c0 = 0; c0 < width; c0 += 32 * 8) { // (the same trips in every lane: they synchronise)
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = min(c0 + 32 * i + lane, width - 1);
+          z[i] = fmaf((to_float(row[c]) - m1 - fix) * rs, to_float(gamma[c]), to_float(beta[c]));
+        }
+        activate_all<Fast>(z, a.activation);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c0 + 32 * i + lane < width)
+            row[c0 + 32 * i + lane] = from_float<T>(z[i]);
+      }
+    }
+    send_span<T>(static_cast<T *>(a.y) + first * width, x, elements);
+  }
+}
+
+// Row sums by a warp per row, then dx and the parameters' gradients by columns: thread t has columns
+// t, t + 256, ... (at most C of them).
+template <class T, int C>
+__global__ void __launch_bounds__(kSpanThreads)
+    span_norm_backward_kernel(const __grid_constant__ NormBackward a, Span span, float *partial) {
+  constexpr bool Fast = sizeof(T) == 2;
+  extern __shared__ __align__(16) unsigned char parameters[];
+  __shared__ uint64_t bar;
+  __shared__ float4 stats[256]; // mean, r, mean(g), mean(g xhat) of each row
+  T *x = reinterpret_cast<T *>(parameters), *dy = reinterpret_cast<T *>(parameters + span.bytes),
+    *gamma = reinterpret_cast<T *>(parameters + 2 * span.bytes), *beta = gamma + a.width;
+  const int width = int(a.width), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float inv_n = 1.f / float(width);
+  if (threadIdx.x == 0) {
+    tc::mbar_init(tc::smem_u32(&bar), 1);
+    tc::fence_proxy_async_smem();
+  }
+  bring_parameters(a.gamma, a.activation != None ? a.beta : nullptr, width, gamma);
+  __syncthreads();
+  auto element = [&](int at, int c, float mean, float r, float &xh) { // dz
+    xh = (to_float(x[at]) - mean) * r;
+    float dz = to_float(dy[at]);
+    if (a.activation != None)
+      dz *= slope<Fast>(fmaf(xh, to_float(gamma[c]), to_float(beta[c])), a.activation);
+    return dz;
+  };
+  float sum_gamma[C] = {}, sum_beta[C] = {};
+  unsigned phase = 0;
+  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows, phase ^= 1) {
+    const int rows = int(min((long long)span.rows, a.rows - first)), elements = rows * width;
+    const T *from[2] = {static_cast<const T *>(a.x) + first * width, static_cast<const T *>(a.dy) + first * width};
+    T *const to[2] = {x, dy};
+    const bool there = bring_spans<T>(from, to, 2, elements, tc::smem_u32(&bar), phase);
+    for (int r = warp; r < rows; r += kSpanThreads / 32) {
+      const float mean = a.mean[first + r], rs = there ? a.rstd[first + r] : __uint_as_float(0x7fc00000u);
+      float s = 0.f, q = 0.f;
+#pragma unroll 8
+      for (int c = lane; c < width; c += 32) {
+        float xh;
+        const float g = element(r * width + c, c, mean, rs, xh) * to_float(gamma[c]);
+        s += g;
+        q = fmaf(g, xh, q);
+      }
+      s = warp_sum(s) * inv_n;
+      q = warp_sum(q) * inv_n;
+      if (!lane)
+        stats[r] = make_float4(mean, rs, s, q);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      const int c = k * kSpanThreads + threadIdx.x;
+      if (c < width) {
+        const float gm = to_float(gamma[c]);
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+          const float4 st = stats[r];
+          float xh;
+          const float dz = element(r * width + c, c, st.x, st.y, xh);
+          sum_gamma[k] = fmaf(dz, xh, sum_gamma[k]);
+          sum_beta[k] += dz;
+          x[r * width + c] = from_float<T>(st.y * (dz * gm - fmaf(xh, st.w, st.z)));
+        }
+      }
+    }
+    if (a.dx)
+      send_span<T>(static_cast<T *>(a.dx) + first * width, x, elements);
+    else
+      __syncthreads();
+  }
+  if (!partial)
+    return;
+  float *out = partial + (long long)blockIdx.x * 2 * width;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = k * kSpanThreads + threadIdx.x;
+    if (c < width) {
+      out[c] = sum_gamma[k];
+      out[width + c] = sum_beta[k];
+    }
+  }
+}
+
 // How a row is laid over threads: units of `unit` elements, `chunks` of them per thread.  Part of a warp
 // or a warp holds it where that leaves a lane at most 8 units (32 single elements), or backward, where
 // every column has two sums in registers as well, 2 (8); else a block, as small as its chunks allow,
@@ -586,6 +789,31 @@ template <auto Kernel> int resident_blocks(int threads, int shared = 0) {
 // threads each; other devices may hold more blocks, the grid is cut at this number.
 constexpr int kMostParts = 1184;
 int wide_parts(long long rows) { return int(std::min<long long>(rows, 32)); }
+// Whether spans are used: rows of 128 elements and more that lie one behind another without gaps, in
+// arrays that start on 16-byte boundaries but whose rows do not; two blocks' shared memory must fit
+// an SM.  `per_row`: bytes in shared memory for each of a span's rows.
+bool span_of(int type, long long width, bool contiguous, int arrays, Span &s, int &shared) {
+  const int b = bytes_of(type);
+  const long long row = width * b;
+  if (!contiguous || width < 128 || row * 8 * arrays + 2 * row > 110000)
+    return false;
+  const long long spans = std::max(1ll, std::min(32ll, 65536 / (row * 8 * arrays)));
+  s.rows = int(8 * spans);
+  s.bytes = int((s.rows * row + 15) / 16 * 16);
+  shared = s.bytes * arrays + int(2 * row);
+  return true;
+}
+template <auto Kernel> int span_blocks(int shared) {
+  static thread_local int device = -1;
+  int now = 0;
+  lapis::check(cudaGetDevice(&now));
+  if (device != now) {
+    lapis::check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+    device = now;
+  }
+  // Per SM: shared memory (228 KiB, one of them each block's own) and 6 blocks for the registers.
+  return std::max(1, std::min(6, 233472 / (shared + 6144))) * sm_count();
+}
 } // namespace
 
 void layer_norm(const Norm &a, cudaStream_t stream) {
@@ -595,7 +823,13 @@ void layer_norm(const Norm &a, cudaStream_t stream) {
     bool vectors = a.width % V == 0 && aligned16(a.x) && aligned16(a.y) && aligned16(a.gamma) &&
                    aligned16(a.beta) && (a.rows == 1 || (a.ldx % V == 0 && a.ldy % V == 0));
     Shape s = shape_of(a.type, a.width, vectors, false);
-    if (s.wide) {
+    Span span;
+    int shared = 0;
+    if (!vectors && span_of(a.type, a.width, a.ldx == a.width && a.ldy == a.width && aligned16(a.x) && aligned16(a.y), 1,
+                            span, shared)) {
+      const int grid = int(std::min<long long>((a.rows + span.rows - 1) / span.rows, span_blocks<span_norm_kernel<T>>(shared)));
+      lapis::launch(span_norm_kernel<T>, grid, kSpanThreads, shared, stream, a, span);
+    } else if (s.wide) {
       int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_kernel<T>>(kWideThreads)));
       lapis::launch(wide_norm_kernel<T>, grid, kWideThreads, 0, stream, a);
     } else {
@@ -631,7 +865,22 @@ void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t st
                      aligned16(a.gamma) && aligned16(a.beta) &&
                      (a.rows == 1 || (a.ldx % V == 0 && a.lddy % V == 0 && a.lddx % V == 0));
       Shape s = shape_of(a.type, a.width, vectors, true);
-      if (s.wide) {
+      Span span;
+      int shared = 0;
+      const bool contiguous = a.ldx == a.width && a.lddy == a.width && (!a.dx || a.lddx == a.width) && aligned16(a.x) &&
+                              aligned16(a.dy) && aligned16(a.dx);
+      if (!vectors && span_of(a.type, a.width, contiguous, 2, span, shared)) {
+        auto go = [&](auto columns) {
+          constexpr auto kernel = span_norm_backward_kernel<T, decltype(columns)::value>;
+          parts = int(std::min<long long>({(a.rows + span.rows - 1) / span.rows, (long long)span_blocks<kernel>(shared),
+                                           (long long)kMostParts}));
+          lapis::launch(kernel, parts, kSpanThreads, shared, stream, a, span, partial);
+        };
+        if (a.width <= 4 * kSpanThreads)
+          go(std::integral_constant<int, 4>{});
+        else
+          go(std::integral_constant<int, 12>{});
+      } else if (s.wide) {
         if (a.dx) {
           int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_backward_kernel<T>>(kWideThreads)));
           if (params && a.dx == a.dy)
