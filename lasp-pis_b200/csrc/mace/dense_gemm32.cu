@@ -54,6 +54,7 @@ struct Gemm32 {
   int slabs, parts;
   uint32_t idesc;
   float *partial;
+  float *sums; // of P's rows over each part's k, [parts][I] (turned P; NULL: not wanted)
   Epilogue e;
   Boxes boxes;
 };
@@ -117,8 +118,9 @@ struct Shared {
 // ROWS rows by 32 k; a thread's row is its own.  Turned: boxes of 64 k by 32 rows; the rows of a box
 // are read by a warp's lanes together, and all of the operand's threads have read before any
 // writes (named barrier `id` of ROWS threads).  Returns the power of two that scales back, biased.
+// sum (turned, not NULL): grows by the row's values.
 template <int ROWS, bool Turned>
-__device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id) {
+__device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id, float *sum) {
   float v[64];
   if (Turned) {
     const unsigned char *box = base + (r >> 5) * 8192 + (r & 3) * 4;
@@ -148,8 +150,17 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
       m[j] = fmaxf(m[j], m[j + w]);
   const int e = split_power(__float_as_uint(m[0]));
   const float2 scale = make_float2(pow2(e), pow2(e));
-  if (Turned)
+  if (Turned) {
+    if (sum) {
+      float2 s[4] = {};
+#pragma unroll
+      for (int k = 0; k < 64; k += 2)
+        s[k / 2 & 3] = __fadd2_rn(s[k / 2 & 3], make_float2(v[k], v[k + 1]));
+      s[0] = __fadd2_rn(__fadd2_rn(s[0], s[1]), __fadd2_rn(s[2], s[3]));
+      *sum += s[0].x + s[0].y;
+    }
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(ROWS) : "memory");
+  }
   unsigned char *hi = base + r * 128, *lo = hi + ROWS * 128;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
@@ -283,33 +294,43 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     const int r = threadIdx.x & 127;
     bool ok = true; // the same in the whole warp
     int n = 0;
-    if (warp < kSplitWarps)
-    for (Walk w(g); w.live(g); w.next(g), ++n) {
+    float sum = 0.f;
+    for (Walk w(g); warp < kSplitWarps && w.live(g); ++n) {
       ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
       if (!ok) { // the other warps of the operand may wait at this slab's barrier
         if (of_q ? QT : PT)
           asm volatile("bar.sync %0, %1;" ::"r"(of_q ? 2 : 1), "r"(of_q ? BN : kBM) : "memory");
-        continue;
-      }
-      unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
-      if (of_q)
-        reinterpret_cast<unsigned short *>(scale)[r] =
-            static_cast<unsigned short>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2) << 7);
-      else
-        scale[2 * BN + r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1));
-      // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
-      // last to arrive sees all of them.
-      fence_proxy_async_smem();
-      __threadfence_block();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
-        if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
-          sh.arrived[n % kSlots] = 0;
-          __threadfence_block();
-          fence_proxy_async_smem();
-          multiply(n);
+        sum = __uint_as_float(0x7fc00000u);
+      } else {
+        unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
+        if (of_q)
+          reinterpret_cast<unsigned short *>(scale)[r] =
+              static_cast<unsigned short>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2, nullptr) << 7);
+        else
+          scale[2 * BN + r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1, PT && g.sums ? &sum : nullptr));
+        // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
+        // last to arrive sees all of them.
+        fence_proxy_async_smem();
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
+          if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
+            sh.arrived[n % kSlots] = 0;
+            __threadfence_block();
+            fence_proxy_async_smem();
+            multiply(n);
+          }
         }
+      }
+      const unsigned tile = w.tile;
+      const int part = w.part;
+      if (w.next(g) && PT && g.sums && !of_q) { // the unit is done: the tiles of the first column have the sums
+        long long i, j;
+        g.tiles.at(tile, i, j);
+        if (j == 0 && i * kBM + r < g.I)
+          g.sums[part * g.I + i * kBM + r] = sum;
+        sum = 0.f;
       }
     }
   } else {
@@ -481,7 +502,7 @@ Plan plan32(long long I, long long J, long long K) {
   return p;
 }
 
-void product32(const Product &p, void *workspace, cudaStream_t stream) {
+void product32(const Product &p, void *workspace, cudaStream_t stream, float *sums) {
   const Plan plan = plan32(p.I, p.J, p.K);
   Gemm32 g{};
   g.I = p.I, g.J = p.J, g.K = p.K;
@@ -496,6 +517,7 @@ void product32(const Product &p, void *workspace, cudaStream_t stream) {
   g.units = g.tiles.count * unsigned(plan.parts);
   g.idesc = idesc_f16(kBM, plan.bn);
   g.partial = plan.parts > 1 ? static_cast<float *>(workspace) : nullptr;
+  g.sums = sums;
   g.e = p.e;
   g.boxes = boxes_of(p, g.partial, plan.parts);
   auto width = [&](auto bn) {
