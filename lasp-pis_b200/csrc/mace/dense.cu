@@ -257,7 +257,7 @@ struct BackwardLayout {
   explicit BackwardLayout(const DenseBackward &d) {
     long long used = 0;
     partial = used;
-    used += std::max(partial_bytes(d), d.type == F32 ? round_up(plan32(d.outputs, d.inputs, d.rows).parts * d.outputs * 4, 16) : 0);
+    used += std::max(partial_bytes(d), d.type == F32 ? round_up(plan32(d.outputs, d.inputs, d.rows).parts * d.outputs * 8, 16) : 0);
     write_dz = d.activation != None || !tma_ready(d.type, d.dy, d.rows, d.lddy);
     dz.ld = d.lddy;
     if (write_dz) {
@@ -335,7 +335,7 @@ void dense_backward(const DenseBackward &d, void *workspace, cudaStream_t stream
              Epilogue{nullptr, None, nullptr, 0, d.dweight, d.lddw}},
             ws + l.product, stream, fused ? sums : nullptr);
   if (fused) {
-    const int parts = plan32(d.outputs, d.inputs, d.rows).parts;
+    const int parts = 2 * plan32(d.outputs, d.inputs, d.rows).parts;
     lapis::launch(column_sum_kernel<float>, dim3(unsigned((d.outputs + 31) / 32), 1), 1024, 0, stream, sums, parts, 1,
                   d.outputs, static_cast<float *>(d.dbias), static_cast<float *>(nullptr));
     lapis::check(cudaGetLastError());

@@ -349,7 +349,7 @@ inline long long parts_workspace(const Plan &p, long long I, long long J) {
 Plan plan16(long long I, long long J, long long K);
 void product16(const Product &, void *workspace, cudaStream_t);
 Plan plan32(long long I, long long J, long long K);
-// sums (p turned; NULL: not wanted): the sums over k of P's rows, [parts][I].
+// sums (p turned; NULL: not wanted): partial sums over k of P's rows, [2 parts][I].
 void product32(const Product &, void *workspace, cudaStream_t, float *sums = nullptr);
 // Sum of `parts` float products [parts][I][J], through the epilogue.
 void finish_parts(int type, const Epilogue &, const float *partial, int parts, long long I, long long J, cudaStream_t);

@@ -11,11 +11,16 @@
 // must not add up over long k.  A slab's result comes out 8.7e-8 too small in the mean (tc_gemm.cu),
 // so three slabs of four are scaled by 1 + 2^-23: 8.9e-8.
 //
-// TMA brings the slab's floats into the place of the split (128 rows of 64 floats are as large as two
-// fp16 planes), whichever index is contiguous; the split reads a row per thread and leaves it k-major,
-// hi over the first half and lo over the second.  16 warps, 128 registers each:
-//   0..7    split, a row per thread: four warps P, four Q (two in 64-wide tiles).  The warp that
-//           finishes a slab last issues its MMAs.
+// TMA brings the slab's floats into shared memory, whichever index is contiguous; the split reads a row
+// per thread.  P's rows go to TMEM, the first operand's other place; Q's over their floats, k-major
+// (64 floats are as long as two rows of fp16), hi over the first half and lo over the second.
+// Shared memory's bandwidth bounds this kernel: with P split in place a 64-wide slab took 2.7k
+// cycles for 216 KB, TMEM spares 80 KB of them.  16 warps, 128 registers each:
+//   0..7    split, a row per thread.  64-wide tiles: two groups take the slabs in turn, a row of P and
+//           (half of them) one of Q per thread; the latencies of a split, not its instructions, take
+//           its time, and so two are under way (gradients of 84613 x 64 -> 1280: 351 -> 291 us).  128-
+//           wide ones have only two stages, which one group uses better: four warps P, four Q.  The
+//           warp that finishes a slab last issues its MMAs.
 //   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
 //           epilogue.  A slab that has reached TMEM has left its stage: warp 8 then starts the
 //           loads of the slab two ahead.
@@ -31,13 +36,15 @@ namespace {
 using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 512, kDrainThreads = 256;
-constexpr int kBuffers = 4; // TMEM accumulators
 template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2; }
-// 64-wide tiles: three stages, and a box of results per drain warp; 128-wide ones: two and two.
+// 64-wide tiles: three stages, and a box of results per drain warp; 128-wide ones: two and two.  TMEM
+// holds P's split slabs, 64 columns for each stage, and as many accumulators as then fit.
 template <int BN> constexpr int stages() { return BN == 64 ? 3 : 2; }
+template <int BN> constexpr int buffers() { return BN == 64 ? 4 : 3; }
+static_assert(buffers<64>() * 64 + stages<64>() * 64 <= 512 && buffers<128>() * 128 + stages<128>() * 64 <= 512, "TMEM");
 // The split of slab g runs after the MMAs of g - stages, which waited for the drain of the slab
-// kBuffers before that.
-template <int BN> constexpr int slots() { return kBuffers + stages<BN>(); }
+// `buffers` before that.
+template <int BN> constexpr int slots() { return buffers<BN>() + stages<BN>(); }
 template <int BN> constexpr int slot_bytes() { return 2 * BN + kBM; }
 template <int BN> constexpr int smem_bytes() {
   return stages<BN>() * stage_bytes<BN>() + 8 * (BN / 64) * kBoxBytes + 8 * (BN / 2) * 4 + slots<BN>() * slot_bytes<BN>() + 512;
@@ -54,7 +61,7 @@ struct Gemm32 {
   int slabs, parts;
   uint32_t idesc;
   float *partial;
-  float *sums; // of P's rows over each part's k, [parts][I] (turned P; NULL: not wanted)
+  float *sums; // of P's rows over each part's k, [parts][2][I] (turned P; NULL: not wanted)
   Epilogue e;
   Boxes boxes;
 };
@@ -114,14 +121,9 @@ struct Shared {
   int arrived[8]; // per slot: split warps that are through with a slab
 };
 
-// Splits row r of an operand's slab (ROWS rows, floats at `base`) in place.  k-major: two boxes of
-// ROWS rows by 32 k; a thread's row is its own.  Turned: boxes of 64 k by 32 rows; the rows of a box
-// are read by a warp's lanes together, and all of the operand's threads have read before any
-// writes (named barrier `id` of ROWS threads).  Returns the power of two that scales back, biased.
-// sum (turned, not NULL): grows by the row's values.
-template <int ROWS, bool Turned>
-__device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id, float *sum) {
-  float v[64];
+// Row r of an operand's slab (ROWS rows, floats at `base`).  k-major: two boxes of ROWS rows by 32 k; a
+// thread's row is its own.  Turned: boxes of 64 k by 32 rows, which a warp's lanes read together.
+template <int ROWS, bool Turned> __device__ __forceinline__ void read_row(const unsigned char *base, int r, float (&v)[64]) {
   if (Turned) {
     const unsigned char *box = base + (r >> 5) * 8192 + (r & 3) * 4;
     const int chunk = r >> 2 & 7;
@@ -135,7 +137,10 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
       v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
     }
   }
-  // The largest magnitude; NaN does not count, and stays NaN in the split.
+}
+// The exponent that scales a row, from its largest magnitude; NaN does not count, and stays NaN in the
+// split.
+__device__ __forceinline__ int row_power(const float (&v)[64]) {
   float m[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
@@ -148,19 +153,55 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
 #pragma unroll
     for (int j = 0; j < w; ++j)
       m[j] = fmaxf(m[j], m[j + w]);
-  const int e = split_power(__float_as_uint(m[0]));
-  const float2 scale = make_float2(pow2(e), pow2(e));
-  if (Turned) {
-    if (sum) {
-      float2 s[4] = {};
+  return split_power(__float_as_uint(m[0]));
+}
+__device__ __forceinline__ float row_sum(const float (&v)[64]) {
+  float2 s[4] = {};
 #pragma unroll
-      for (int k = 0; k < 64; k += 2)
-        s[k / 2 & 3] = __fadd2_rn(s[k / 2 & 3], make_float2(v[k], v[k + 1]));
-      s[0] = __fadd2_rn(__fadd2_rn(s[0], s[1]), __fadd2_rn(s[2], s[3]));
-      *sum += s[0].x + s[0].y;
-    }
+  for (int k = 0; k < 64; k += 2)
+    s[k / 2 & 3] = __fadd2_rn(s[k / 2 & 3], make_float2(v[k], v[k + 1]));
+  s[0] = __fadd2_rn(__fadd2_rn(s[0], s[1]), __fadd2_rn(s[2], s[3]));
+  return s[0].x + s[0].y;
+}
+// 32 columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+               "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+               "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
+}
+// P's row r to TMEM, lane = row: hi in 32 columns from `taddr` (two k each), lo in the next 32.  Returns
+// the power of two that scales back, biased.  sum (not NULL) grows by the row's values.
+template <bool Turned>
+__device__ __forceinline__ unsigned split_p(const unsigned char *base, int r, uint32_t taddr, float *sum) {
+  float v[64];
+  read_row<kBM, Turned>(base, r, v);
+  if (Turned && sum)
+    *sum += row_sum(v);
+  const int e = row_power(v);
+  const float2 scale = make_float2(pow2(e), pow2(e));
+  uint32_t h[32], l[32];
+#pragma unroll
+  for (int p = 0; p < 32; ++p)
+    split2(make_float2(v[2 * p], v[2 * p + 1]), scale, h[p], l[p]);
+  tmem_st32(taddr, h);
+  tmem_st32(taddr + 32, l);
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  tc_fence_before();
+  return unsigned(127 - e);
+}
+// Q's row r in place.  Turned: all of its threads have read before any writes (named barrier `id` of
+// ROWS threads).
+template <int ROWS, bool Turned> __device__ __forceinline__ unsigned split_q(unsigned char *base, int r, int id) {
+  float v[64];
+  read_row<ROWS, Turned>(base, r, v);
+  const int e = row_power(v);
+  const float2 scale = make_float2(pow2(e), pow2(e));
+  if (Turned)
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(ROWS) : "memory");
-  }
   unsigned char *hi = base + r * 128, *lo = hi + ROWS * 128;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
@@ -173,6 +214,13 @@ __device__ __forceinline__ unsigned split_row(unsigned char *base, int r, int id
     *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
   return unsigned(127 - e);
+}
+// D (TMEM) (+)= A (TMEM) B (shared memory).
+template <bool Add> __device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+               "r"(a), "l"(b), "r"(idesc), "n"(int(Add)));
 }
 
 // sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time; ends early at NaN.
@@ -195,8 +243,8 @@ __device__ __forceinline__ float plain_sum(const float *p, long long pk, const f
 template <int BN, bool PT, bool QT>
 __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_constant__ Gemm32 g) {
   constexpr int kPBytes = kBM * kBK * 2, kQBytes = BN * kBK * 2, kStageBytes = stage_bytes<BN>();
-  constexpr int kStages = stages<BN>(), kSlots = slots<BN>(), kSlotBytes = slot_bytes<BN>(), kBoxes = BN / 64;
-  constexpr int kTmemCols = kBuffers * BN;
+  constexpr int kStages = stages<BN>(), kSlots = slots<BN>(), kSlotBytes = slot_bytes<BN>(), kBoxes = BN / 64,
+                kBuffers = buffers<BN>(), kTmemCols = 512;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *staging = smem + kStages * kStageBytes; // the drain warps' boxes, then their bias
   float *biases = reinterpret_cast<float *>(staging + 8 * kBoxes * kBoxBytes);
@@ -211,7 +259,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned full0 = smem_u32(bars), tfull0 = full0 + 8 * kStages, tfree0 = tfull0 + 8 * kBuffers, scaled0 = tfree0 + 8 * kBuffers,
                  residual0 = scaled0 + 8 * kSlots;
-  constexpr int kSplitWarps = 4 + BN / 32;
+  constexpr bool kInTurn = BN == 64;             // two groups of split warps take the slabs in turn
+  constexpr int kSplitWarps = kInTurn ? 4 : 8; // of each slab
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kStages; ++s)
@@ -239,22 +288,28 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
 
+  // P's split slab n: 64 columns behind the accumulators, a place for each stage.
+  auto p_columns = [&](int n) { return tmem + uint32_t(kBuffers * BN + n % kStages * 64); };
   // The MMAs of slab n (one thread).
   auto multiply = [&](int n) {
     const int b = n % kBuffers;
     if (n >= kBuffers && !mbar_wait(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, &sh.abort_flag))
       return;
     tc_fence_after();
-    const unsigned ph = smem_u32(smem + n % kStages * kStageBytes), pl = ph + kPBytes, qh = pl + kPBytes, ql = qh + kQBytes;
-    const uint32_t d = tmem + uint32_t(b * BN);
+    // Few instructions per MMA: while one thread issues, its warp's share of the next slab waits.  A
+    // 16-wide step is 32 bytes (2 descriptor units) of Q, 8 columns of P.
+    const uint64_t qh = smem_desc(smem_u32(smem + n % kStages * kStageBytes) + 2 * kPBytes), ql = qh + (kQBytes >> 4);
+    const uint32_t d = tmem + uint32_t(b * BN), ph = p_columns(n), pl = ph + 32, idesc = g.idesc;
+    umma_f16_tmem<false>(d, pl, qh, idesc); // the small terms first
+    umma_f16_tmem<true>(d, ph, ql, idesc);
 #pragma unroll
-    for (int m = 0; m < kBK / 16; ++m) { // the small terms first
-      umma_f16_desc(d, smem_desc(pl + 32 * m), smem_desc(qh + 32 * m), g.idesc, m ? 1u : 0u);
-      umma_f16_desc(d, smem_desc(ph + 32 * m), smem_desc(ql + 32 * m), g.idesc, 1u);
+    for (int m = 1; m < kBK / 16; ++m) {
+      umma_f16_tmem<true>(d, pl + 8 * m, qh + 2 * m, idesc);
+      umma_f16_tmem<true>(d, ph + 8 * m, ql + 2 * m, idesc);
     }
 #pragma unroll
     for (int m = 0; m < kBK / 16; ++m)
-      umma_f16_desc(d, smem_desc(ph + 32 * m), smem_desc(qh + 32 * m), g.idesc, 1u);
+      umma_f16_tmem<true>(d, ph + 8 * m, qh + 2 * m, idesc);
     umma_commit(tfull0 + 8 * b);
   };
   // The loads of slab n at sh.ahead, which moves on (one thread; the MMAs of slab n - 2 are done).
@@ -290,46 +345,52 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   // Registers: 128 each at launch; 256 threads give 32 to the other 256 (96 + 160 = 2 x 128).
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    const bool of_q = warp >= 4;
-    const int r = threadIdx.x & 127;
+    const int group = warp >> 2, r = threadIdx.x & 127;
+    const bool has_p = kInTurn || group == 0, has_q = kInTurn ? r < BN : group == 1;
     bool ok = true; // the same in the whole warp
-    int n = 0;
     float sum = 0.f;
-    for (Walk w(g); warp < kSplitWarps && w.live(g); ++n) {
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
-      if (!ok) { // the other warps of the operand may wait at this slab's barrier
-        if (of_q ? QT : PT)
-          asm volatile("bar.sync %0, %1;" ::"r"(of_q ? 2 : 1), "r"(of_q ? BN : kBM) : "memory");
-        sum = __uint_as_float(0x7fc00000u);
-      } else {
-        unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
-        if (of_q)
-          reinterpret_cast<unsigned short *>(scale)[r] =
-              static_cast<unsigned short>(split_row<BN, QT>(stage + 2 * kPBytes, r, 2, nullptr) << 7);
-        else
-          scale[2 * BN + r] = static_cast<unsigned char>(split_row<kBM, PT>(stage, r, 1, PT && g.sums ? &sum : nullptr));
-        // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
-        // last to arrive sees all of them.
-        fence_proxy_async_smem();
-        __threadfence_block();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
-          if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
-            sh.arrived[n % kSlots] = 0;
-            __threadfence_block();
-            fence_proxy_async_smem();
-            multiply(n);
+    int n = 0;
+    for (Walk w(g); w.live(g); ++n) {
+      if (!kInTurn || (n & 1) == group) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
+        if (!ok) { // Q's other warps may wait at this slab's barrier
+          if (QT && has_q)
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(BN) : "memory");
+          sum = __uint_as_float(0x7fc00000u);
+        } else {
+          unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
+          if (has_p)
+            scale[2 * BN + r] = static_cast<unsigned char>(
+                split_p<PT>(stage, r, p_columns(n) + (uint32_t(32 * (warp & 3)) << 16), PT && g.sums ? &sum : nullptr));
+          if (has_q)
+            reinterpret_cast<unsigned short *>(scale)[r] =
+                static_cast<unsigned short>(split_q<BN, QT>(stage + 2 * kPBytes, r, 1 + group) << 7);
+          // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
+          // last to arrive sees all of them.
+          fence_proxy_async_smem();
+          __threadfence_block();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
+            if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
+              sh.arrived[n % kSlots] = 0;
+              __threadfence_block();
+              fence_proxy_async_smem();
+              multiply(n);
+            }
           }
         }
       }
       const unsigned tile = w.tile;
       const int part = w.part;
-      if (w.next(g) && PT && g.sums && !of_q) { // the unit is done: the tiles of the first column have the sums
+      if (w.next(g) && PT && g.sums && has_p) { // the unit is done: the tiles of the first column have the sums
         long long i, j;
         g.tiles.at(tile, i, j);
-        if (j == 0 && i * kBM + r < g.I)
-          g.sums[part * g.I + i * kBM + r] = sum;
+        if (j == 0 && i * kBM + r < g.I) {
+          g.sums[(2ll * part + group) * g.I + i * kBM + r] = sum;
+          if (!kInTurn)
+            g.sums[(2ll * part + 1) * g.I + i * kBM + r] = 0.f;
+        }
         sum = 0.f;
       }
     }
