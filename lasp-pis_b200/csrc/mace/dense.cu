@@ -100,6 +100,157 @@ void narrow(const Dense &d, cudaStream_t stream) {
   });
 }
 
+// ---------------- few rows ----------------
+// y for up to kFew rows (a token, or a few): W is read once and HBM bounds the call, so the warps only
+// stream it.  A warp has four rows of W under way, eight 16-byte loads per lane in flight, finds x in
+// L1, and `ks` warps of a block share them along k where there are few outputs.  Float
+// sums: lanes, then the warps in order.  M: d.rows or a little more (rows past the last read it).
+constexpr int kFew = 8, kFewOutputs = 4;
+// A unit that is read once, in the order written (all of a step's loads before the first use).
+template <class T, int U> __device__ __forceinline__ Unit<T, U> stream_unit(const T *p) {
+  Unit<T, U> u;
+  if constexpr (sizeof(u) == 16) {
+    uint4 w;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                 : "l"(p));
+    memcpy(&u, &w, 16);
+  } else {
+    u = *reinterpret_cast<const Unit<T, U> *>(p);
+  }
+  return u;
+}
+template <class T, int U, int M>
+__global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ Dense d, int ks) {
+  constexpr int R = kFewOutputs;
+  using Un = Unit<T, U>;
+  __shared__ float parts[8][R * M];
+  const T *const x = static_cast<const T *>(d.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = warp % ks, slot = warp / ks, slots = 8 / ks;
+  // Groups of four outputs go round the blocks first, so that every SM reads as much.
+  const long long groups = (d.outputs + R - 1) / R;
+  for (long long first = 0; first < groups; first += (long long)gridDim.x * slots) {
+    const long long group = first + (long long)slot * gridDim.x + blockIdx.x;
+    const long long n0 = group * R; // rows past the end: the last row, not written
+    const long long units = group < groups ? d.inputs / U : 0;
+    const T *w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      w[r] = static_cast<const T *>(d.weight) + min(n0 + r, d.outputs - 1) * d.ldw;
+    float acc[R][M] = {};
+    auto add = [&](const Un (&u)[R], const Un (&v)[M]) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        float xv[U];
+        unpack<T, U>(v[m], xv);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float wv[U];
+          unpack<T, U>(u[r], wv);
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            acc[r][m] = fmaf(wv[i], xv[i], acc[r][m]);
+        }
+      }
+    };
+    const int step = 32 * ks;
+    long long at = sub * 32 + lane;
+    for (; at + step < units; at += 2 * step) {
+      Un a[R], b[R], v[M], u[M];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        a[r] = stream_unit<T, U>(w[r] + at * U);
+        b[r] = stream_unit<T, U>(w[r] + (at + step) * U);
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + at * U);
+        u[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + (at + step) * U);
+      }
+      add(a, v);
+      add(b, u);
+    }
+    if (at < units) {
+      Un a[R], v[M];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        a[r] = stream_unit<T, U>(w[r] + at * U);
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + at * U);
+      add(a, v);
+    }
+    __syncwarp();
+    float mine = 0.f; // lane i has output i / M of the group, row i % M
+#pragma unroll
+    for (int i = 0; i < R * M; ++i) {
+      float v = acc[i / M][i % M];
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == i)
+        mine = v;
+    }
+    if (ks > 1) {
+      if (lane < R * M)
+        parts[warp][lane] = mine;
+      __syncthreads();
+      if (!sub && lane < R * M)
+        for (int s = 1; s < ks; ++s)
+          mine += parts[warp + s][lane];
+      __syncthreads();
+    }
+    const long long col = n0 + lane / M;
+    if (!sub && lane < R * M && col < d.outputs && lane % M < d.rows) {
+      const Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz};
+      finish<T>(e, lane % M, col, mine);
+    }
+  }
+}
+bool few_vectors(const Dense &d) {
+  const int V = 16 / bytes_of(d.type);
+  return d.inputs % V == 0 && aligned16(d.weight) && (d.outputs <= 1 || d.ldw % V == 0) && aligned16(d.x) &&
+         (d.rows <= 1 || d.ldx % V == 0);
+}
+// bf16 1 x 4096 -> 16384 takes 24.5 us here (5.5 TB/s) and 28.5 on the tensor cores, 4 x 1024 -> 1024 3.5
+// and 7.5, f32 4 x 4096 -> 16384 56 and 124; but 16-bit weights of that size from two rows on 33 to
+// 36 and 28.9: the conversions and products of each weight then take longer than its bytes.
+bool is_few(const Dense &d) {
+  return d.rows <= kFew && (d.rows == 1 || d.type == F32 || !few_vectors(d) || d.inputs <= (1ll << 24) / d.outputs);
+}
+template <class T, int U, int M> void launch_few(const Dense &d, cudaStream_t stream) {
+  const long long groups = (d.outputs + kFewOutputs - 1) / kFewOutputs;
+  // Warps share a group while there are fewer groups than warps and each keeps two steps of k.
+  int ks = 1;
+  while (ks < 8 && groups * ks < 16ll * sm_count() && d.inputs / U >= 128ll * ks)
+    ks *= 2;
+  const long long blocks = (groups + 8 / ks - 1) / (8 / ks);
+  // As many blocks as fit, so that groups spread evenly over the SMs; fewer where they are not filled.
+  lapis::launch(few_rows_kernel<T, U, M>, dim3(unsigned(std::min<long long>(blocks, 4ll * sm_count()))), 256, 0, stream, d, ks);
+  lapis::check(cudaGetLastError());
+}
+void few_rows(const Dense &d, cudaStream_t stream) {
+  with_type(d.type, [&](auto tag) {
+    using T = decltype(tag);
+    auto rows = [&](auto unit) {
+      constexpr int U = decltype(unit)::value;
+      if (d.rows == 1)
+        launch_few<T, U, 1>(d, stream);
+      else if (d.rows == 2)
+        launch_few<T, U, 2>(d, stream);
+      else if (d.rows <= 4)
+        launch_few<T, U, 4>(d, stream);
+      else
+        launch_few<T, U, 8>(d, stream);
+    };
+    if (few_vectors(d))
+      rows(std::integral_constant<int, 16 / int(sizeof(T))>{});
+    else
+      rows(std::integral_constant<int, 1>{});
+  });
+}
+
 // ---------------- one pass over dy ----------------
 // A block is `lanes` columns units wide (a power of two up to 32) and 256 / lanes rows high; it walks
 // rows by gridDim.y blocks' heights, writes dz = dy act'(z) (dz NULL: not wanted) and adds its columns:
@@ -274,10 +425,14 @@ struct BackwardLayout {
 };
 } // namespace
 
-long long dense_workspace(const Dense &d) { return is_narrow(d) ? 0 : ForwardLayout(d).total; }
+long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) ? 0 : ForwardLayout(d).total; }
 void dense(const Dense &d, void *workspace, cudaStream_t stream) {
   if (is_narrow(d)) {
     narrow(d, stream);
+    return;
+  }
+  if (is_few(d)) {
+    few_rows(d, stream);
     return;
   }
   const ForwardLayout l(d);
