@@ -105,6 +105,7 @@ void narrow(const Dense &d, cudaStream_t stream) {
 // stream it.  A warp has four rows of W under way, eight 16-byte loads per lane in flight, finds x in
 // L1, and `ks` warps of a block share them along k where there are few outputs.  Float
 // sums: lanes, then the warps in order.  M: d.rows or a little more (rows past the last read it).
+// Turned: the same for a few outputs, with x in W's place and W in x's.
 constexpr int kFew = 8, kFewOutputs = 4;
 // A unit that is read once, in the order written (all of a step's loads before the first use).
 template <class T, int U> __device__ __forceinline__ Unit<T, U> stream_unit(const T *p) {
@@ -120,16 +121,18 @@ template <class T, int U> __device__ __forceinline__ Unit<T, U> stream_unit(cons
   }
   return u;
 }
-template <class T, int U, int M>
+template <class T, int U, int M, bool Turned>
 __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ Dense d, int ks) {
   constexpr int R = kFewOutputs;
+  const long long many = Turned ? d.rows : d.outputs, few = Turned ? d.outputs : d.rows, ldm = Turned ? d.ldx : d.ldw,
+                  ldf = Turned ? d.ldw : d.ldx;
   using Un = Unit<T, U>;
   __shared__ float parts[8][R * M];
-  const T *const x = static_cast<const T *>(d.x);
+  const T *const x = static_cast<const T *>(Turned ? d.weight : d.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = warp % ks, slot = warp / ks, slots = 8 / ks;
   // Groups of four outputs go round the blocks first, so that every SM reads as much.
-  const long long groups = (d.outputs + R - 1) / R;
+  const long long groups = (many + R - 1) / R;
   for (long long first = 0; first < groups; first += (long long)gridDim.x * slots) {
     const long long group = first + (long long)slot * gridDim.x + blockIdx.x;
     const long long n0 = group * R; // rows past the end: the last row, not written
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
     const T *w[R];
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      w[r] = static_cast<const T *>(d.weight) + min(n0 + r, d.outputs - 1) * d.ldw;
+      w[r] = static_cast<const T *>(Turned ? d.x : d.weight) + min(n0 + r, many - 1) * ldm;
     float acc[R][M] = {};
     auto add = [&](const Un (&u)[R], const Un (&v)[M]) {
 #pragma unroll
@@ -165,8 +168,8 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
       }
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + at * U);
-        u[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + (at + step) * U);
+        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + at * U);
+        u[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + (at + step) * U);
       }
       add(a, v);
       add(b, u);
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
         a[r] = stream_unit<T, U>(w[r] + at * U);
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, d.rows - 1) * d.ldx + at * U);
+        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + at * U);
       add(a, v);
     }
     __syncwarp();
@@ -201,10 +204,10 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
           mine += parts[warp + s][lane];
       __syncthreads();
     }
-    const long long col = n0 + lane / M;
-    if (!sub && lane < R * M && col < d.outputs && lane % M < d.rows) {
+    const long long at_many = n0 + lane / M, at_few = lane % M;
+    if (!sub && lane < R * M && at_many < many && at_few < few) {
       const Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz};
-      finish<T>(e, lane % M, col, mine);
+      finish<T>(e, Turned ? at_many : at_few, Turned ? at_few : at_many, mine);
     }
   }
 }
@@ -219,35 +222,46 @@ bool few_vectors(const Dense &d) {
 bool is_few(const Dense &d) {
   return d.rows <= kFew && (d.rows == 1 || d.type == F32 || !few_vectors(d) || d.inputs <= (1ll << 24) / d.outputs);
 }
-template <class T, int U, int M> void launch_few(const Dense &d, cudaStream_t stream) {
-  const long long groups = (d.outputs + kFewOutputs - 1) / kFewOutputs;
+// Few outputs: the tensor cores' tiles would be mostly empty, and x is what streams.
+bool is_few_outputs(const Dense &d) { return d.outputs <= kFew; }
+template <class T, int U, int M, bool Turned> void launch_few(const Dense &d, cudaStream_t stream) {
+  const long long groups = ((Turned ? d.rows : d.outputs) + kFewOutputs - 1) / kFewOutputs;
   // Warps share a group while there are fewer groups than warps and each keeps two steps of k.
   int ks = 1;
   while (ks < 8 && groups * ks < 16ll * sm_count() && d.inputs / U >= 128ll * ks)
     ks *= 2;
   const long long blocks = (groups + 8 / ks - 1) / (8 / ks);
   // As many blocks as fit, so that groups spread evenly over the SMs; fewer where they are not filled.
-  lapis::launch(few_rows_kernel<T, U, M>, dim3(unsigned(std::min<long long>(blocks, 4ll * sm_count()))), 256, 0, stream, d, ks);
+  lapis::launch(few_rows_kernel<T, U, M, Turned>, dim3(unsigned(std::min<long long>(blocks, 4ll * sm_count()))), 256, 0,
+                stream, d, ks);
   lapis::check(cudaGetLastError());
 }
-void few_rows(const Dense &d, cudaStream_t stream) {
+void few_rows(const Dense &d, bool turned, cudaStream_t stream) {
   with_type(d.type, [&](auto tag) {
     using T = decltype(tag);
-    auto rows = [&](auto unit) {
+    const long long few = turned ? d.outputs : d.rows;
+    auto rows = [&](auto unit, auto way) {
       constexpr int U = decltype(unit)::value;
-      if (d.rows == 1)
-        launch_few<T, U, 1>(d, stream);
-      else if (d.rows == 2)
-        launch_few<T, U, 2>(d, stream);
-      else if (d.rows <= 4)
-        launch_few<T, U, 4>(d, stream);
+      constexpr bool Turned = decltype(way)::value;
+      if (few == 1)
+        launch_few<T, U, 1, Turned>(d, stream);
+      else if (few == 2)
+        launch_few<T, U, 2, Turned>(d, stream);
+      else if (few <= 4)
+        launch_few<T, U, 4, Turned>(d, stream);
       else
-        launch_few<T, U, 8>(d, stream);
+        launch_few<T, U, 8, Turned>(d, stream);
     };
-    if (few_vectors(d))
-      rows(std::integral_constant<int, 16 / int(sizeof(T))>{});
+    auto units = [&](auto way) {
+      if (few_vectors(d))
+        rows(std::integral_constant<int, 16 / int(sizeof(T))>{}, way);
+      else
+        rows(std::integral_constant<int, 1>{}, way);
+    };
+    if (turned)
+      units(std::true_type{});
     else
-      rows(std::integral_constant<int, 1>{});
+      units(std::false_type{});
   });
 }
 
@@ -314,13 +328,26 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Copy of a [rows][cols] array with any row distance and alignment into rows of ldo elements.
+// Copy of a [rows][cols] array with any row distance and alignment into rows of ldo elements (a multiple
+// of 16 bytes): a lane gathers 16 bytes of a row by single elements, all in flight, and stores them at
+// once; what lies behind cols in a row's last 16 bytes is zero.  A warp takes 32 neighbouring units.
 template <class T>
 __global__ void __launch_bounds__(256) pack_kernel(const T *in, long long ldi, T *out, long long ldo, long long rows,
                                                    long long cols) {
-  for (long long r = blockIdx.y; r < rows; r += gridDim.y)
-    for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < cols; c += 256ll * gridDim.x)
-      out[r * ldo + c] = in[r * ldi + c];
+  constexpr int U = 16 / int(sizeof(T));
+  const long long units = ldo / U, total = rows * units;
+  for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < total; x += 256ll * gridDim.x) {
+    const long long r = x / units, c = (x - r * units) * U;
+    const T *p = in + r * ldi;
+    Unit<T, U> u;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      u.v[i] = p[min(c + i, cols - 1)];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      u.v[i] = c + i < cols ? u.v[i] : T(0);
+    *reinterpret_cast<Unit<T, U> *>(out + r * ldo + c) = u;
+  }
 }
 
 // The pass's grid: about 8 blocks per SM.
@@ -367,7 +394,8 @@ Operand bring(int type, const Place &w, const void *p, long long rows, long long
   if (w.at < 0)
     return {p, ld, turned};
   void *to = static_cast<char *>(workspace) + w.at;
-  dim3 grid(unsigned(std::min<long long>((cols + 255) / 256, 1024)), unsigned(std::min<long long>(rows, 8192)));
+  const long long units = rows * (w.ld * bytes_of(type) / 16);
+  const dim3 grid(unsigned(std::min<long long>((units + 255) / 256, 16ll * sm_count())));
   auto copy = [&](auto tag) {
     using U = decltype(tag);
     lapis::launch(pack_kernel<U>, grid, 256, 0, stream, static_cast<const U *>(p), ld, static_cast<U *>(to), w.ld, rows, cols);
@@ -425,14 +453,14 @@ struct BackwardLayout {
 };
 } // namespace
 
-long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) ? 0 : ForwardLayout(d).total; }
+long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) || is_few_outputs(d) ? 0 : ForwardLayout(d).total; }
 void dense(const Dense &d, void *workspace, cudaStream_t stream) {
   if (is_narrow(d)) {
     narrow(d, stream);
     return;
   }
-  if (is_few(d)) {
-    few_rows(d, stream);
+  if (is_few(d) || is_few_outputs(d)) {
+    few_rows(d, !is_few(d), stream);
     return;
   }
   const ForwardLayout l(d);

@@ -509,72 +509,109 @@ __global__ void __launch_bounds__(256) wide_params_kernel(const __grid_constant_
   out[a.width + i] = sb;
 }
 
-// ---------------- rows that start anywhere, in one contiguous array ----------------
-// Odd widths leave a row no wide loads, but 8 rows together start and end on 16-byte boundaries: a block
-// copies a span of 8 k whole rows into shared memory (one bulk copy per array, the last few bytes of
-// the array one by one), works on it element by element there and sends the result back the same
-// way.  Several blocks share an SM, so one computes while another's copies are under way.
-// f16 8191 x 2053, backward: single-element loads take 105 us.
-constexpr int kSpanThreads = 256;
+// ---------------- rows that start anywhere ----------------
+// Rows that allow no wide loads (odd widths) are copied into shared memory as spans: several rows that
+// lie one behind another without gaps, or one row.  One bulk copy brings what of a span lies between
+// 16-byte boundaries, single loads its two ends, to a place with the same offset from a boundary; the
+// result goes back the same way.  Element by element there, with several blocks to an SM, so that one
+// computes while another's copies are under way.  f16 8191 x 2053, backward: single-element loads take
+// 105 us, spans 56.
 struct Span {
-  int rows, bytes; // of a span; bytes rounded up to 16
+  int rows, bytes; // of a span; bytes: of its place in shared memory
 };
-// Starts the copies of `elements` elements of `arrays` spans, and waits for them.
-template <class T>
-__device__ __forceinline__ bool bring_spans(const T *const (&from)[2], T *const (&to)[2], int arrays, int elements,
-                                            unsigned bar, unsigned phase) {
-  const unsigned whole = unsigned(elements) * unsigned(sizeof(T)) & ~15u;
-  if (whole && threadIdx.x == 0) {
-    tc::mbar_expect_tx(bar, whole * unsigned(arrays));
-    for (int k = 0; k < arrays; ++k)
-      tc::bulk_load(tc::smem_u32(to[k]), from[k], whole, bar);
+struct Ends {
+  int head, whole; // elements before the first boundary, and from there to the last one
+};
+template <class T> __device__ __forceinline__ Ends ends_of(const T *p, int elements) {
+  const int off = int(reinterpret_cast<uintptr_t>(p) & 15), head = min(off ? (16 - off) / int(sizeof(T)) : 0, elements);
+  return {head, (elements - head) * int(sizeof(T)) / 16 * (16 / int(sizeof(T)))};
+}
+// A span's first element in its place.
+template <class T> __device__ __forceinline__ T *placed(unsigned char *place, const T *p) {
+  return reinterpret_cast<T *>(place + (reinterpret_cast<uintptr_t>(p) & 15));
+}
+// Copies `elements` elements of each of K spans; whether they came.
+template <class T, int K>
+__device__ __forceinline__ bool bring_spans(const T *const (&from)[K], T *const (&to)[K], int elements, unsigned bar,
+                                            unsigned &phase) {
+  Ends e[K];
+  unsigned bytes = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    e[k] = ends_of(from[k], elements);
+    bytes += unsigned(e[k].whole) * unsigned(sizeof(T));
   }
-  for (int k = 0; k < arrays; ++k)
-    for (int i = int(whole / sizeof(T)) + int(threadIdx.x); i < elements; i += kSpanThreads)
+  if (bytes && threadIdx.x == 0) {
+    tc::mbar_expect_tx(bar, bytes);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (e[k].whole)
+        tc::bulk_load(tc::smem_u32(to[k] + e[k].head), from[k] + e[k].head, unsigned(e[k].whole) * unsigned(sizeof(T)), bar);
+  }
+  // (16 / size ends at most on each side)
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = threadIdx.x;
+    if (i < e[k].head)
       to[k][i] = from[k][i];
+    const int tail = e[k].head + e[k].whole + i;
+    if (i < 32 && tail < elements)
+      to[k][tail] = from[k][tail];
+  }
   bool there = true;
-  if (whole) {
+  if (bytes) {
     const long long start = clock64();
     while (!(there = tc::mbar_try(bar, phase)) && clock64() - start < tc::kWaitCycles) {
     }
+    phase ^= 1;
   }
   return __syncthreads_and(there);
 }
 template <class T> __device__ __forceinline__ void send_span(T *to, const T *from, int elements) {
-  const unsigned whole = unsigned(elements) * unsigned(sizeof(T)) & ~15u;
   tc::fence_proxy_async_smem();
   __syncthreads();
-  if (whole && threadIdx.x == 0) {
-    tc::bulk_store(to, tc::smem_u32(from), whole);
+  // Bulk where both sides agree about the boundaries (they do, but for rows of different distances).
+  Ends e = ends_of(to, elements);
+  if ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(from)) & 15)
+    e = {0, 0};
+  if (e.whole && threadIdx.x == 0) {
+    tc::bulk_store(to + e.head, tc::smem_u32(from + e.head), unsigned(e.whole) * unsigned(sizeof(T)));
     tc::bulk_commit();
     tc::bulk_wait_read();
   }
-  for (int i = int(whole / sizeof(T)) + int(threadIdx.x); i < elements; i += kSpanThreads)
+  for (int i = threadIdx.x; i < e.head; i += blockDim.x)
+    to[i] = from[i];
+  for (int i = e.head + e.whole + int(threadIdx.x); i < elements; i += blockDim.x)
     to[i] = from[i];
   __syncthreads();
 }
 // gamma and beta (1 and 0 where there is none) into shared memory.
 template <class T> __device__ __forceinline__ void bring_parameters(const void *gamma, const void *beta, int width, T *to) {
-  for (int i = threadIdx.x; i < width; i += kSpanThreads) {
+  for (int i = threadIdx.x; i < width; i += blockDim.x) {
     to[i] = gamma ? static_cast<const T *>(gamma)[i] : from_float<T>(1.f);
     to[width + i] = beta ? static_cast<const T *>(beta)[i] : from_float<T>(0.f);
   }
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1)
-    v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// A row of a span belongs to a warp, or to the whole block where a span is a single row (Block):
+// its first thread and stride, and sums over it.
+template <bool Block> struct Team {
+  static __device__ __forceinline__ int first() { return Block ? threadIdx.x : threadIdx.x & 31; }
+  static __device__ __forceinline__ int stride() { return Block ? blockDim.x : 32; }
+  static __device__ __forceinline__ float2 sum(float2 v, float2 (*shared)[32]) {
+    float2 s[1] = {v};
+    group_sum<!Block, 1>(s, 32, shared);
+    return s[0];
+  }
+};
 
-// A warp per row.
-template <class T>
-__global__ void __launch_bounds__(kSpanThreads) span_norm_kernel(const __grid_constant__ Norm a, Span span) {
+template <class T, bool Block>
+__global__ void __launch_bounds__(Block ? 1024 : 256) span_norm_kernel(const __grid_constant__ Norm a, Span span) {
   constexpr bool Fast = sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char parameters[];
   __shared__ uint64_t bar;
-  T *x = reinterpret_cast<T *>(parameters), *gamma = reinterpret_cast<T *>(parameters + span.bytes), *beta = gamma + a.width;
-  const int width = int(a.width), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float2 shared[2][1][32];
+  T *gamma = reinterpret_cast<T *>(parameters + span.bytes), *beta = gamma + a.width;
+  const int width = int(a.width), warp = threadIdx.x >> 5, t = Team<Block>::first(), stride = Team<Block>::stride();
   const float inv_n = 1.f / float(width);
   if (threadIdx.x == 0) {
     tc::mbar_init(tc::smem_u32(&bar), 1);
@@ -583,63 +620,64 @@ __global__ void __launch_bounds__(kSpanThreads) span_norm_kernel(const __grid_co
   bring_parameters(a.gamma, a.beta, width, gamma);
   __syncthreads();
   unsigned phase = 0;
-  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows, phase ^= 1) {
+  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows) {
     const int rows = int(min((long long)span.rows, a.rows - first)), elements = rows * width;
-    const T *from[2] = {static_cast<const T *>(a.x) + first * width, nullptr};
-    T *const to[2] = {x, nullptr};
-    const bool there = bring_spans<T>(from, to, 1, elements, tc::smem_u32(&bar), phase);
-    for (int r = warp; r < rows; r += kSpanThreads / 32) {
+    const T *const from[1] = {static_cast<const T *>(a.x) + first * a.ldx};
+    T *const x = placed(parameters, from[0]), *const to[1] = {x};
+    const bool there = bring_spans<T, 1>(from, to, elements, tc::smem_u32(&bar), phase);
+    for (int r = Block ? 0 : warp; r < rows; r += Block ? 1 : 8) {
       T *row = x + r * width;
-      float s = 0.f, q = 0.f;
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll 8
-      for (int c = lane; c < width; c += 32)
-        s += to_float(row[c]);
-      const float m1 = warp_sum(s) * inv_n;
-      s = 0.f;
+      for (int c = t; c < width; c += stride)
+        s.x += to_float(row[c]);
+      const float m1 = Team<Block>::sum(s, shared[0]).x * inv_n;
+      s = make_float2(0.f, 0.f);
 #pragma unroll 8
-      for (int c = lane; c < width; c += 32) {
+      for (int c = t; c < width; c += stride) {
         const float d = to_float(row[c]) - m1;
-        s += d;
-        q = fmaf(d, d, q);
+        s.x += d;
+        s.y = fmaf(d, d, s.y);
       }
-      const float fix = warp_sum(s) * inv_n, v = fmaf(-fix, fix, warp_sum(q) * inv_n), var = v < 0.f ? 0.f : v;
+      s = Team<Block>::sum(s, shared[1]);
+      const float fix = s.x * inv_n, v = fmaf(-fix, fix, s.y * inv_n), var = v < 0.f ? 0.f : v;
       // A wait that ran out shows as NaN.
       const float rs = there ? 1.f / sqrtf(var + a.eps) : __uint_as_float(0x7fc00000u);
-      if (a.mean && !lane) {
+      if (a.mean && !t) {
         a.mean[first + r] = m1 + fix;
         a.rstd[first + r] = rs;
       }
-      for (int c0 = 0; c0 < width; c0 += 32 * 8) { // (the same trips in every lane: they synchronise)
+      // Each thread rewrites the elements that it reads.
+      for (int c0 = t; c0 < width; c0 += 8 * stride) {
         float z[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int c = min(c0 + 32 * i + lane, width - 1);
-          z[i] = fmaf((to_float(row[c]) - m1 - fix) * rs, to_float(gamma[c]), to_float(beta[c]));
+          const int c = min(c0 + i * stride, width - 1);
+          z[i] = c0 + i * stride < width ? fmaf((to_float(row[c]) - m1 - fix) * rs, to_float(gamma[c]), to_float(beta[c])) : 0.f;
         }
         activate_all<Fast>(z, a.activation);
-        __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c0 + 32 * i + lane < width)
-            row[c0 + 32 * i + lane] = from_float<T>(z[i]);
+          if (c0 + i * stride < width)
+            row[c0 + i * stride] = from_float<T>(z[i]);
       }
     }
-    send_span<T>(static_cast<T *>(a.y) + first * width, x, elements);
+    send_span<T>(static_cast<T *>(a.y) + first * a.ldy, x, elements);
   }
 }
 
-// Row sums by a warp per row, then dx and the parameters' gradients by columns: thread t has columns
-// t, t + 256, ... (at most C of them).
-template <class T, int C>
-__global__ void __launch_bounds__(kSpanThreads)
+// Row sums, then dx and the parameters' gradients by columns: thread t has columns t, t + blockDim.x, ...
+// (at most C of them).
+template <class T, int C, bool Block>
+__global__ void __launch_bounds__(Block ? 1024 : 256)
     span_norm_backward_kernel(const __grid_constant__ NormBackward a, Span span, float *partial) {
   constexpr bool Fast = sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char parameters[];
   __shared__ uint64_t bar;
-  __shared__ float4 stats[256]; // mean, r, mean(g), mean(g xhat) of each row
-  T *x = reinterpret_cast<T *>(parameters), *dy = reinterpret_cast<T *>(parameters + span.bytes),
-    *gamma = reinterpret_cast<T *>(parameters + 2 * span.bytes), *beta = gamma + a.width;
-  const int width = int(a.width), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float2 shared[2][1][32];
+  __shared__ float4 stats[Block ? 1 : 256]; // mean, r, mean(g), mean(g xhat) of each row
+  T *gamma = reinterpret_cast<T *>(parameters + 2 * span.bytes), *beta = gamma + a.width;
+  const int width = int(a.width), warp = threadIdx.x >> 5, t = Team<Block>::first(), stride = Team<Block>::stride();
   const float inv_n = 1.f / float(width);
   if (threadIdx.x == 0) {
     tc::mbar_init(tc::smem_u32(&bar), 1);
@@ -647,39 +685,41 @@ __global__ void __launch_bounds__(kSpanThreads)
   }
   bring_parameters(a.gamma, a.activation != None ? a.beta : nullptr, width, gamma);
   __syncthreads();
-  auto element = [&](int at, int c, float mean, float r, float &xh) { // dz
-    xh = (to_float(x[at]) - mean) * r;
-    float dz = to_float(dy[at]);
-    if (a.activation != None)
-      dz *= slope<Fast>(fmaf(xh, to_float(gamma[c]), to_float(beta[c])), a.activation);
-    return dz;
-  };
   float sum_gamma[C] = {}, sum_beta[C] = {};
   unsigned phase = 0;
-  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows, phase ^= 1) {
+  int k2 = 0;
+  for (long long first = (long long)blockIdx.x * span.rows; first < a.rows; first += (long long)gridDim.x * span.rows) {
     const int rows = int(min((long long)span.rows, a.rows - first)), elements = rows * width;
-    const T *from[2] = {static_cast<const T *>(a.x) + first * width, static_cast<const T *>(a.dy) + first * width};
-    T *const to[2] = {x, dy};
-    const bool there = bring_spans<T>(from, to, 2, elements, tc::smem_u32(&bar), phase);
-    for (int r = warp; r < rows; r += kSpanThreads / 32) {
+    const T *const from[2] = {static_cast<const T *>(a.x) + first * a.ldx, static_cast<const T *>(a.dy) + first * a.lddy};
+    T *const x = placed(parameters, from[0]), *const dy = placed(parameters + span.bytes, from[1]), *const to[2] = {x, dy};
+    const bool there = bring_spans<T, 2>(from, to, elements, tc::smem_u32(&bar), phase);
+    auto element = [&](int at, int c, float mean, float r, float &xh) { // dz
+      xh = (to_float(x[at]) - mean) * r;
+      float dz = to_float(dy[at]);
+      if (a.activation != None)
+        dz *= slope<Fast>(fmaf(xh, to_float(gamma[c]), to_float(beta[c])), a.activation);
+      return dz;
+    };
+    for (int r = Block ? 0 : warp; r < rows; r += Block ? 1 : 8) {
       const float mean = a.mean[first + r], rs = there ? a.rstd[first + r] : __uint_as_float(0x7fc00000u);
-      float s = 0.f, q = 0.f;
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll 8
-      for (int c = lane; c < width; c += 32) {
+      for (int c = t; c < width; c += stride) {
         float xh;
         const float g = element(r * width + c, c, mean, rs, xh) * to_float(gamma[c]);
-        s += g;
-        q = fmaf(g, xh, q);
+        s.x += g;
+        s.y = fmaf(g, xh, s.y);
       }
-      s = warp_sum(s) * inv_n;
-      q = warp_sum(q) * inv_n;
-      if (!lane)
-        stats[r] = make_float4(mean, rs, s, q);
+      s = Team<Block>::sum(s, shared[k2 ^= 1]);
+      if (!t)
+        stats[r] = make_float4(mean, rs, s.x * inv_n, s.y * inv_n);
     }
     __syncthreads();
+    // dx over dy's place where it lies like dy, else over x's: both are read by their thread only.
+    T *const out = a.dx && ((reinterpret_cast<uintptr_t>(static_cast<T *>(a.dx) + first * a.lddx) ^ reinterpret_cast<uintptr_t>(dy)) & 15) == 0 ? dy : x;
 #pragma unroll
     for (int k = 0; k < C; ++k) {
-      const int c = k * kSpanThreads + threadIdx.x;
+      const int c = k * int(blockDim.x) + int(threadIdx.x);
       if (c < width) {
         const float gm = to_float(gamma[c]);
 #pragma unroll 4
@@ -689,24 +729,24 @@ __global__ void __launch_bounds__(kSpanThreads)
           const float dz = element(r * width + c, c, st.x, st.y, xh);
           sum_gamma[k] = fmaf(dz, xh, sum_gamma[k]);
           sum_beta[k] += dz;
-          x[r * width + c] = from_float<T>(st.y * (dz * gm - fmaf(xh, st.w, st.z)));
+          out[r * width + c] = from_float<T>(st.y * (dz * gm - fmaf(xh, st.w, st.z)));
         }
       }
     }
     if (a.dx)
-      send_span<T>(static_cast<T *>(a.dx) + first * width, x, elements);
+      send_span<T>(static_cast<T *>(a.dx) + first * a.lddx, out, elements);
     else
       __syncthreads();
   }
   if (!partial)
     return;
-  float *out = partial + (long long)blockIdx.x * 2 * width;
+  float *sums = partial + (long long)blockIdx.x * 2 * width;
 #pragma unroll
   for (int k = 0; k < C; ++k) {
-    const int c = k * kSpanThreads + threadIdx.x;
+    const int c = k * int(blockDim.x) + int(threadIdx.x);
     if (c < width) {
-      out[c] = sum_gamma[k];
-      out[width + c] = sum_beta[k];
+      sums[c] = sum_gamma[k];
+      sums[width + c] = sum_beta[k];
     }
   }
 }
@@ -789,30 +829,33 @@ template <auto Kernel> int resident_blocks(int threads, int shared = 0) {
 // threads each; other devices may hold more blocks, the grid is cut at this number.
 constexpr int kMostParts = 1184;
 int wide_parts(long long rows) { return int(std::min<long long>(rows, 32)); }
-// Whether spans are used: rows of 128 elements and more that lie one behind another without gaps, in
-// arrays that start on 16-byte boundaries but whose rows do not; two blocks' shared memory must fit
-// an SM.  `per_row`: bytes in shared memory for each of a span's rows.
-bool span_of(int type, long long width, bool contiguous, int arrays, Span &s, int &shared) {
+// Whether spans are used, for rows that allow no wide loads: from 128 elements on, as far as their
+// place (and gamma and beta) fits in shared memory.  Rows that lie without gaps form spans of up to 64
+// KiB a block, a multiple of 8 rows with a warp each, while two blocks fit an SM; other rows, and longer
+// ones, are a span each for a block of 512 or 1024 threads.
+bool span_of(int type, long long rows, long long width, bool contiguous, int arrays, Span &s, int &shared, bool &block) {
   const int b = bytes_of(type);
   const long long row = width * b;
-  if (!contiguous || width < 128 || row * 8 * arrays + 2 * row > 110000)
+  if (width < 128)
     return false;
-  const long long spans = std::max(1ll, std::min(32ll, 65536 / (row * 8 * arrays)));
-  s.rows = int(8 * spans);
-  s.bytes = int((s.rows * row + 15) / 16 * 16);
-  shared = s.bytes * arrays + int(2 * row);
-  return true;
+  block = !contiguous || 8 * row * arrays + 2 * row > 110000;
+  // (As few rows to a span as give every SM four.)
+  s.rows = block ? 1 : int(8 * std::max(1ll, std::min({32ll, 65536 / (row * 8 * arrays), rows / (32ll * sm_count())})));
+  const long long place = (s.rows * row + 31) / 16 * 16, all = place * arrays + 2 * row;
+  s.bytes = int(std::min(place, 1ll << 30));
+  shared = int(std::min(all, 1ll << 30));
+  return all <= 216 * 1024 && (arrays == 1 || width <= 12 * (block ? 1024 : 256));
 }
-template <auto Kernel> int span_blocks(int shared) {
+template <auto Kernel> int span_blocks(int shared, int threads) {
   static thread_local int device = -1;
   int now = 0;
   lapis::check(cudaGetDevice(&now));
   if (device != now) {
-    lapis::check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+    lapis::check(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
     device = now;
   }
-  // Per SM: shared memory (228 KiB, one of them each block's own) and 6 blocks for the registers.
-  return std::max(1, std::min(6, 233472 / (shared + 6144))) * sm_count();
+  // Per SM: shared memory (228 KiB, some of them each block's own) and registers.
+  return std::max(1, std::min(1536 / threads, 233472 / (shared + 6144))) * sm_count();
 }
 } // namespace
 
@@ -825,10 +868,16 @@ void layer_norm(const Norm &a, cudaStream_t stream) {
     Shape s = shape_of(a.type, a.width, vectors, false);
     Span span;
     int shared = 0;
-    if (!vectors && span_of(a.type, a.width, a.ldx == a.width && a.ldy == a.width && aligned16(a.x) && aligned16(a.y), 1,
-                            span, shared)) {
-      const int grid = int(std::min<long long>((a.rows + span.rows - 1) / span.rows, span_blocks<span_norm_kernel<T>>(shared)));
-      lapis::launch(span_norm_kernel<T>, grid, kSpanThreads, shared, stream, a, span);
+    bool block = false;
+    if (!vectors && span_of(a.type, a.rows, a.width, a.ldx == a.width && a.ldy == a.width, 1, span, shared, block)) {
+      auto go = [&](auto whole) {
+        constexpr bool Block = decltype(whole)::value;
+        constexpr auto kernel = span_norm_kernel<T, Block>;
+        const int threads = !Block ? 256 : a.width <= 8192 ? 512 : 1024;
+        const int grid = int(std::min<long long>((a.rows + span.rows - 1) / span.rows, span_blocks<kernel>(shared, threads)));
+        lapis::launch(kernel, grid, threads, shared, stream, a, span);
+      };
+      block ? go(std::true_type{}) : go(std::false_type{});
     } else if (s.wide) {
       int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_kernel<T>>(kWideThreads)));
       lapis::launch(wide_norm_kernel<T>, grid, kWideThreads, 0, stream, a);
@@ -867,19 +916,23 @@ void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t st
       Shape s = shape_of(a.type, a.width, vectors, true);
       Span span;
       int shared = 0;
-      const bool contiguous = a.ldx == a.width && a.lddy == a.width && (!a.dx || a.lddx == a.width) && aligned16(a.x) &&
-                              aligned16(a.dy) && aligned16(a.dx);
-      if (!vectors && span_of(a.type, a.width, contiguous, 2, span, shared)) {
-        auto go = [&](auto columns) {
-          constexpr auto kernel = span_norm_backward_kernel<T, decltype(columns)::value>;
-          parts = int(std::min<long long>({(a.rows + span.rows - 1) / span.rows, (long long)span_blocks<kernel>(shared),
-                                           (long long)kMostParts}));
-          lapis::launch(kernel, parts, kSpanThreads, shared, stream, a, span, partial);
+      bool block = false;
+      const bool contiguous = a.ldx == a.width && a.lddy == a.width && (!a.dx || a.lddx == a.width);
+      if (!vectors && span_of(a.type, a.rows, a.width, contiguous, 2, span, shared, block)) {
+        auto go = [&](auto columns, auto whole) {
+          constexpr bool Block = decltype(whole)::value;
+          constexpr auto kernel = span_norm_backward_kernel<T, decltype(columns)::value, Block>;
+          const int threads = !Block ? 256 : a.width <= 6144 ? 512 : 1024;
+          parts = int(std::min<long long>({(a.rows + span.rows - 1) / span.rows,
+                                           (long long)span_blocks<kernel>(shared, threads), (long long)kMostParts}));
+          lapis::launch(kernel, parts, threads, shared, stream, a, span, partial);
         };
-        if (a.width <= 4 * kSpanThreads)
-          go(std::integral_constant<int, 4>{});
+        using std::integral_constant;
+        const bool narrow = a.width <= 4 * (block ? 512 : 256);
+        if (block)
+          narrow ? go(integral_constant<int, 4>{}, std::true_type{}) : go(integral_constant<int, 12>{}, std::true_type{});
         else
-          go(std::integral_constant<int, 12>{});
+          narrow ? go(integral_constant<int, 4>{}, std::false_type{}) : go(integral_constant<int, 12>{}, std::false_type{});
       } else if (s.wide) {
         if (a.dx) {
           int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_backward_kernel<T>>(kWideThreads)));
