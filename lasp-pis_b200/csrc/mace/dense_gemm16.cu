@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
 #pragma unroll 1
           for (int c = first; c < end && j * BN + c < g.J; c += 32) {
             const Sectors<T> now = residual;
-            if (g.e.residual && c + 32 < end)
+            if (g.e.residual && !partial && c + 32 < end)
               residual.load(g.e, g.I, g.J, row0 + lane, j * BN + c + 32);
             float v[32];
             get(c, v);

@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         const unsigned char *scale = scales + n % kSlots * kSlotBytes;
         const unsigned char *fq = scale + 2 * (half * kCols);
         // 2^-e of P's row, one ulp more in three slabs of four.
-        const float fp = __uint_as_float((uint32_t(scale[2 * BN + 32 * quarter + lane]) << 23) + ((n & 3) != 3));
+        const float fp = __uint_as_float((uint32_t(scale[2 * BN + 32 * quarter + lane]) << 23) + ((w.k & 3) != 3));
         const float2 fp2 = make_float2(fp, fp);
         uint32_t r[kCols / 32][32];
 #pragma unroll

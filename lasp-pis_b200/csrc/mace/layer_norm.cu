@@ -752,27 +752,29 @@ __global__ void __launch_bounds__(Block ? 1024 : 256)
 }
 
 // How a row is laid over threads: units of `unit` elements, `chunks` of them per thread.  Part of a warp
-// or a warp holds it where that leaves a lane at most 8 units (32 single elements), or backward, where
-// every column has two sums in registers as well, 2 (8); else a block, as small as its chunks allow,
-// so that several share an SM and one computes while another waits at its barrier.
+// or a warp holds it where that leaves a lane at most 8 units, or backward, where every column has two
+// sums in registers as well, 2; else a block, as small as its chunks allow, so that several share an SM
+// and one computes while another waits at its barrier.  Rows that allow no wide loads: below 128
+// elements, 1 or 8 per lane (longer ones are spans, see span_of).
 struct Shape {
   int unit, chunks, threads, most; // threads: lanes of a warp, or the block's threads; most: its class
   bool wide;
 };
+constexpr int kShort = 128; // single elements
 Shape shape_of(int type, long long width, bool vectors, bool backward) {
   Shape s{vectors ? 16 / bytes_of(type) : 1, 0, 1, kWarpBlock, false};
   const long long units = (width + s.unit - 1) / s.unit;
-  static constexpr int kLane[4][5] = {{1, 8, 32}, {1, 8}, {1, 2, 4, 8}, {1, 2}}; // [vectors][backward]
-  static constexpr int kBlock[4][3] = {{8}, {4, 8}, {4}, {1, 2}};
+  static constexpr int kLane[4][5] = {{1, 8}, {1, 8}, {1, 2, 4, 8}, {1, 2}}; // [vectors][backward]
+  static constexpr int kBlock[2][3] = {{4}, {1, 2}};                          // [backward]
   for (const int *c = kLane[2 * vectors + backward]; *c; ++c)
-    if (units <= 32 * *c) {
+    if (units <= 32 * *c && (vectors || width < kShort)) {
       s.chunks = *c;
       while ((long long)s.threads * *c < units)
         s.threads *= 2;
       return s;
     }
   for (int most : {512, 1024})
-    for (const int *c = kBlock[2 * vectors + backward]; *c; ++c)
+    for (const int *c = kBlock[backward]; vectors && *c; ++c)
       if (units <= (long long)most * *c) {
         s.chunks = *c;
         s.threads = int((units + 32 * *c - 1) / (32 * *c) * 32);
@@ -805,13 +807,10 @@ template <bool Backward, int V, class F> void with_shape(const Shape &s, F &&lau
   integral_constant<int, 512> small;
   integral_constant<int, 1024> large;
   is(v, one, warps), is(v, two, warps), is(one, one, warps), is(one, eight, warps);
-  is(one, eight, small), is(one, eight, large);
-  if constexpr (Backward) {
-    is(v, one, small), is(v, two, small), is(v, two, large), is(one, four, small);
-  } else {
+  if constexpr (Backward)
+    is(v, one, small), is(v, two, small), is(v, two, large);
+  else
     is(v, four, warps), is(v, eight, warps), is(v, four, small), is(v, four, large);
-    is(one, integral_constant<int, 32>{}, warps);
-  }
   if (!done)
     throw lapis::Error("Layer norm has no kernel for this row length");
 }
@@ -836,7 +835,7 @@ int wide_parts(long long rows) { return int(std::min<long long>(rows, 32)); }
 bool span_of(int type, long long rows, long long width, bool contiguous, int arrays, Span &s, int &shared, bool &block) {
   const int b = bytes_of(type);
   const long long row = width * b;
-  if (width < 128)
+  if (width < kShort)
     return false;
   block = !contiguous || 8 * row * arrays + 2 * row > 110000;
   // (As few rows to a span as give every SM four.)

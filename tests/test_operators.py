@@ -13,6 +13,7 @@ Tolerances are bounds, derived from how a result is computed, not fitted:
   * Gradients of 16-bit layers round dz to the type before the products: u |dz| more.
 """
 import math
+import random
 
 import pytest
 
@@ -172,6 +173,76 @@ def test_dense_backward_many_rows(op, dtype):
         check_dense_backward(op, dy, x, w, act, z)
     for need in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
         check_dense_backward(op, dy, x, w, "silu", z, need)
+
+
+def spread(rng, low, high):
+    return min(high, max(low, round(math.exp(rng.uniform(math.log(low), math.log(high))))))
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(30))
+def test_dense_anywhere(op, seed):
+    """Shapes drawn over the whole range, types, activations and options at random: few rows, few
+    outputs, few inputs, several tiles per SM, sums cut into parts, rows that start anywhere."""
+    rng = random.Random(seed)
+    dt = dtype_of(rng.choice(TYPES))
+    while True:
+        M, K, N = spread(rng, 1, 6000), spread(rng, 1, 3000), spread(rng, 1, 3000)
+        if rng.random() < 0.5:
+            K, N = (K + 15) // 16 * 16, (N + 15) // 16 * 16
+        if M * K * N < 4e9:
+            break
+    act = rng.choice(ACTS)
+    x, w = normal(1, M, K, dtype=dt), normal(2, N, K, dtype=dt, scale=K ** -0.5)
+    b = normal(3, N, dtype=dt) if rng.random() < 0.7 else None
+    r = normal(4, M, N, dtype=dt) if rng.random() < 0.5 else None
+    check_dense(op, x, w, b, act, r, rng.random() < 0.5)
+    check_dense_backward(op, normal(5, M, N, dtype=dt), x, w, act, normal(6, M, N, dtype=dt))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9])
+def test_dense_few_rows_and_few_outputs(op, rows, dtype):
+    dt = dtype_of(dtype)
+    for K, N in ((33, 3), (256, 70), (1000, 1), (1001, 517), (5000, 64)):
+        x, w, b = normal(1, rows, K, dtype=dt), normal(2, N, K, dtype=dt, scale=K ** -0.5), normal(3, N, dtype=dt)
+        check_dense(op, x, w, b, "gelu", normal(4, rows, N, dtype=dt), True)
+        x, w, b = normal(1, N, K, dtype=dt), normal(2, rows, K, dtype=dt, scale=K ** -0.5), normal(3, rows, dtype=dt)
+        check_dense(op, x, w, b, "silu", normal(4, N, rows, dtype=dt), True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dense_larger(op, dtype):
+    """Several tiles per SM with every part of the epilogue; a wide layer of few rows; a long sum."""
+    dt = dtype_of(dtype)
+    for M, K, N in ((5000, 200, 1200), (4097, 64, 2056), (40, 1024, 4104), (16, 20000, 24)):
+        x, w = normal(1, M, K, dtype=dt), normal(2, N, K, dtype=dt, scale=K ** -0.5)
+        b, r = normal(3, N, dtype=dt), normal(4, M, N, dtype=dt)
+        for act, bias, residual, keep in ((None, None, None, False), ("gelu", b, None, True), ("silu", b, r, False),
+                                          ("relu", None, r, True)):
+            check_dense(op, x, w, bias, act, residual, keep)
+        check_dense_backward(op, r, x, w, "gelu", normal(5, M, N, dtype=dt))
+        check_dense_backward(op, r, x, w, None, None)
+
+
+@gpu
+def test_dense_offsets_beyond_32_bits(op):
+    """Arrays whose elements lie more than 2^31 apart (rows of a wide buffer)."""
+    import torch
+    buf = torch.empty(5, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    x, r = buf[:, -136:-8], buf[:, 1 << 29:(1 << 29) + 64]
+    x.copy_(normal(1, 5, 128, dtype=torch.bfloat16))
+    r.copy_(normal(2, 5, 64, dtype=torch.bfloat16))
+    w = normal(3, 64, 128, dtype=torch.bfloat16, scale=0.1)
+    check_dense(op, x, w, None, "silu", r, False)
+    mean, rstd = check_norm(op, x, None, None, 1e-5, None)
+    check_norm_backward(op, normal(4, 5, 128, dtype=torch.bfloat16), x, mean, rstd, None, None, None)
+    wide = torch.as_strided(buf.view(-1), (20, 128), (1 << 27, 1), 64)
+    wide.copy_(normal(5, 20, 128, dtype=torch.bfloat16))
+    check_dense(op, wide, w, None, None, None, True)
+    check_dense_backward(op, normal(6, 20, 64, dtype=torch.bfloat16), wide, w, None, None)
 
 
 @gpu
@@ -349,6 +420,27 @@ def test_layer_norm(op, shape, dtype):
     check_norm(op, x, gamma, None, 1e-3, "silu")
     check_norm_backward(op, dy, x, mean, rstd, gamma, None, "silu")
     check_norm_backward(op, dy, x, mean, rstd, None, beta, "gelu")
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(30))
+def test_layer_norm_anywhere(op, seed):
+    """Shapes drawn over the whole range, with types, activations and parameters at random; half of the
+    arrays are column blocks of wider ones."""
+    rng = random.Random(seed)
+    dt = dtype_of(rng.choice(TYPES))
+    M, n = spread(rng, 1, 5000), spread(rng, 8, 14000)
+    M = min(M, 4000000 // n)
+    if rng.random() < 0.4:
+        n = (n + 7) // 8 * 8
+    wide = n + rng.choice([0, 0, 8, 3])
+    x = normal(1, M, wide, dtype=dt, scale=1.7, shift=0.4)[:, :n]
+    dy = normal(4, M, wide, dtype=dt)[:, wide - n:]
+    gamma = normal(2, n, dtype=dt, scale=0.3, shift=1.0) if rng.random() < 0.8 else None
+    beta = normal(3, n, dtype=dt, scale=0.3) if rng.random() < 0.8 else None
+    act = rng.choice(ACTS)
+    mean, rstd = check_norm(op, x, gamma, beta, 1e-5, act)
+    check_norm_backward(op, dy, x, mean, rstd, gamma, beta, act)
 
 
 @gpu
