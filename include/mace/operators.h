@@ -18,7 +18,7 @@
  * NULL where that is 0, its contents do not matter, and it is free again when the call's work
  * on the stream is done.  Calls that may run at the same time need workspaces of their own.
  * Outputs do not overlap inputs, the workspace or each other, with the exceptions named below.
- * rows may be 0. */
+ * rows may be 0.  Waits inside the kernels are bounded; one that ran out would show as NaN. */
 #pragma once
 #include <mace/export.h>
 #ifdef __cplusplus
@@ -33,9 +33,11 @@ enum { MACE_ACT_NONE = 0, MACE_ACT_SILU = 1, MACE_ACT_GELU = 2, MACE_ACT_RELU = 
  * [outputs][inputs], bias [outputs] (or NULL), residual, y and z [rows][outputs] (residual or
  * z NULL: left out).  z, kept for mace_dense_backward, is written before the activation.
  * residual may be y itself (same address and ld).
- * float products run on the tensor cores as split fp16 pairs: per row and 64 consecutive
- * inputs the largest magnitude sets the scale, values down to 2^-18 of it keep 22 bits, and
- * smaller ones are held to 2^-40 of it. */
+ * float products run on the tensor cores as split fp16 pairs (but for up to 8 rows or outputs, or
+ * few inputs: plain float arithmetic): per row and 64 consecutive inputs the largest magnitude sets
+ * the scale, values down to 2^-18 of it keep 22 bits, and smaller ones are held to 2^-40 of it.
+ * Infinities and NaN give what the sum gives (such results are summed again, which is slow where
+ * there are many). */
 MACE_EXPORT int mace_dense(int type, long long rows, long long inputs, long long outputs, const void *x,
                            long long ldx, const void *weight, long long ldw, const void *bias, int activation,
                            const void *residual, long long ldr, void *y, long long ldy, void *z, long long ldz,

@@ -215,8 +215,8 @@ template <class T> struct Sectors {
 };
 // 32 columns of a lane's row from col0, for rows of whole sectors (Boxes::sectors): each lane writes its
 // row 32 bytes at a time, a sector each, with nothing staged and nothing waited for (bf16 84613 x 64
-// -> 1280: 50 us, 62 through boxes; float rows, twice as long, take longer this way: 227 us, 195).  bias: in shared memory.  part: the float values as they are,
-// to that array.
+// -> 1280: 50 us, 62 through boxes; float rows, twice as long, take longer this way: 227 us, 195).
+// bias: in shared memory.  part: the float values as they are, to that array.
 template <class T>
 __device__ __forceinline__ void finish_row(const Epilogue &e, float *part, long long I, long long J, long long row,
                                            long long col0, float (&v)[32], const T *bias, const Sectors<T> &residual) {

@@ -10,6 +10,10 @@
 // thread), and eight that move a finished tile out of TMEM, through the epilogue and to global
 // memory while the next tile accumulates in TMEM's other half.  With too few tiles for the
 // device, K is cut into parts whose float products a second launch adds in order.
+//
+// bf16, back to back: 8192 x 4096 -> 16384 in 813 us (1.35 PFLOP/s, 0.98 of the measured sustained rate;
+// with bias, GELU and z kept 931), 4096 x 2048 -> 8192 in 123 us (1.1 PFLOP/s).  84613 x 64 -> 1280 in 50 us
+// (4.5 TB/s written and read): one slab per tile, so the epilogue bounds it.
 #include "dense_gemm.cuh"
 
 namespace mace {
@@ -279,26 +283,33 @@ __global__ void __launch_bounds__(256) finish_parts_kernel(const __grid_constant
   }
 }
 
-// A narrower tile saves little: at K = 4096 a 128 x 256 tile takes 28 us, a 128 x 128 one 24 us (P's
-// shared-memory reads bound both); few tiles are cut along K until they fill the device, parts of at least four slabs.
 } // namespace
+
+// The cheapest of the tile widths, in units of a 128 x 256 tile's slab (0.43 us at K = 4096).  A narrower
+// tile saves little: a 128 x 128 one takes 0.85 of that (P's shared-memory reads bound both); but with
+// one row of tiles Q comes from HBM, and a slab costs what its bytes do (1.7 for 256 columns).  Few tiles
+// are cut along K until they fill the device, parts of at least four slabs; a second launch then
+// reads the parts.
 Plan plan16(long long I, long long J, long long K) {
   const int sms = sm_count();
   const long long slabs = (K + kBK - 1) / kBK;
   Plan best{0, 1};
   double cost = 0;
   for (int bn : {256, 128, 64}) {
-    long long tiles = (I + kBM - 1) / kBM * ((J + bn - 1) / bn);
-    int parts = int(std::min<long long>({std::max(1ll, sms / tiles), std::max(1ll, slabs / 4), 64}));
-    long long waves = (tiles * parts + sms - 1) / sms;
-    double c = double(waves) * double((slabs + parts - 1) / parts) * (bn == 256 ? 1. : bn == 128 ? .85 : .75);
-    if (!best.bn || c < cost)
-      best = {bn, parts}, cost = c;
+    const long long tiles = (I + kBM - 1) / kBM * ((J + bn - 1) / bn);
+    const double slab = std::max(bn == 256 ? 1. : bn == 128 ? .85 : .75, I <= kBM ? 1.7 * bn / 256 : 0.);
+    for (int cut : {0, 1}) {
+      const int parts = cut ? int(std::min<long long>({std::max(1ll, sms / tiles), std::max(1ll, slabs / 4), 64})) : 1;
+      const long long waves = (tiles * parts + sms - 1) / sms;
+      const double c = double(waves) * double((slabs + parts - 1) / parts) * slab +
+                       (parts > 1 ? 8. + double(parts) * double(I) * double(J) * 3e-6 : 0.);
+      if (!best.bn || c < cost)
+        best = {bn, parts}, cost = c;
+    }
   }
   return best;
 }
 namespace {
-
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

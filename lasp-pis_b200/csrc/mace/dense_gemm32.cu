@@ -3,29 +3,33 @@
 //
 //   out(i, j) = sum_k P(i, k) Q(j, k)
 //
-// Both operands are split on the way into shared memory: per row and 64-wide slab of k, with 2^e the
+// Both operands are split on the way to the tensor cores: per row and 64-wide slab of k, with 2^e the
 // power of two that brings the largest magnitude into [2^14, 2^15), v 2^e = hi + lo, both fp16
 // rounded to nearest (22 significant bits for values down to 2^-18 of the largest).  A slab's
 // products lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22) accumulate fresh in TMEM, are scaled back
 // by the two exact powers of two and added to float registers: the tensor pipe truncates, which
 // must not add up over long k.  A slab's result comes out 8.7e-8 too small in the mean (tc_gemm.cu),
-// so three slabs of four are scaled by 1 + 2^-23: 8.9e-8.
+// so three slabs of four are scaled by 1 + 2^-23: 8.9e-8.  2-norm errors against 64 bits: 0.8e-7 to
+// 2.2e-7, where float sums in order have 1.4e-7 to 1.4e-6.
 //
 // TMA brings the slab's floats into shared memory, whichever index is contiguous; the split reads a row
 // per thread.  P's rows go to TMEM, the first operand's other place; Q's over their floats, k-major
-// (64 floats are as long as two rows of fp16), hi over the first half and lo over the second.
-// Shared memory's bandwidth bounds this kernel: with P split in place a 64-wide slab took 2.7k
-// cycles for 216 KB, TMEM spares 80 KB of them.  16 warps, 128 registers each:
-//   0..7    split, a row per thread.  64-wide tiles: two groups take the slabs in turn, a row of P and
-//           (half of them) one of Q per thread; the latencies of a split, not its instructions, take
-//           its time, and so two are under way (gradients of 84613 x 64 -> 1280: 351 -> 291 us).  128-
-//           wide ones have only two stages, which one group uses better: four warps P, four Q.  The
-//           warp that finishes a slab last issues its MMAs.
+// (64 floats are as long as two rows of fp16), hi over the first half and lo over the second.  16 warps,
+// 128 registers each at launch:
+//   0..7    split.  64-wide tiles: two groups take the slabs in turn, a row of P and (half of them) one
+//           of Q per thread; the latencies of a split, not its instructions, take its time, and so
+//           two are under way (gradients of 84613 x 64 -> 1280: 351 -> 291 us).  128-wide ones have
+//           only two stages, which one group uses better (61 us against 67 for 10000 x 512 -> 512):
+//           four warps P, four Q.  The warp that finishes a slab last issues its MMAs.
 //   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
 //           epilogue.  A slab that has reached TMEM has left its stage: warp 8 then starts the
-//           loads of the slab two ahead.
-// (Loading by plain loads straight into the registers of the split was 5 times slower: the loads of
-// 64 KB per slab stalled the split warps.)
+//           loads of the slab that takes its place.
+// What bounds it: no unit (gradients of 84613 x 64 -> 1280: issue slots 34% busy, DRAM 33%, tensor pipe
+// 12%), but the chain load, split, multiply, drain of a slab at one CTA per SM; with one slab per
+// tile (84613 x 64 -> 1280: 200 us, 2.3 TB/s) the drain's epilogue.  Measured and not kept: plain loads
+// straight into the split's registers (10000 x 512 -> 512: 174 us, then 104 with TMA), P split in place
+// (358 us where TMEM gave 351), L2 prefetches of P (no change), three stages and one box of results for
+// 128-wide tiles (84613 x 64 -> 1280: 245 us), results written from registers by sectors (227 us).
 // Infinities and NaN make every result of their row (of P or Q) NaN in this scheme; results that
 // are not finite are summed again, one product at a time.
 #include "dense_gemm.cuh"

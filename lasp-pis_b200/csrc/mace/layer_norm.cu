@@ -10,10 +10,13 @@
 // warp, or a block for wide rows) between its statistics and its result.  HBM bounds it, so what
 // counts is bytes in flight: a warp holds rows of up to 8 KiB, and where a thread's share of a row is
 // small it takes several rows at once, and loads the next ones before the arithmetic of these.  The
-// variance is taken about a first mean and corrected for that mean's own rounding, so a row far from
-// zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
+// variance is taken about a first mean and, for floats, corrected for that mean's own rounding, so a
+// row far from zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
 // parameters' gradients stay in registers too; each block writes one partial row of dgamma and
 // dbeta, and a second launch adds the partial rows in a fixed order.
+//
+// bf16 16384 x 4096 forward: 57 us, 4.7 TB/s (0.72 of the measured copy rate); f16 8191 x 2048: 18 us
+// forward, 29 backward (3.5 TB/s); f32 84613 x 64 with SiLU: 11.5 and 17.8.
 #include "operators.cuh"
 #include "tcgen05.cuh"
 #include <algorithm>
@@ -26,8 +29,8 @@ constexpr int kWarpBlock = 256; // threads of a block whose rows belong to warps
 constexpr int kSharedChunks = 4; // forward: from as many units per lane on
 
 // A unit of an array, or zeros where it is not live.  The load itself is unconditional, from a place
-// inside the array: a load under a branch is waited for where the
-// branches join, which leaves one in flight instead of all of a row's.
+// inside the array: a load under a branch is waited for where the branches join, which leaves one in
+// flight instead of all of a row's (bf16 16384 x 4096: 192 us, 93 without).
 template <class T, int U>
 __device__ __forceinline__ Unit<T, U> load_unit(const T *row, bool live, int col) {
   Unit<T, U> v = *reinterpret_cast<const Unit<T, U> *>(row + col);

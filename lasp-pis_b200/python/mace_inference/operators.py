@@ -259,8 +259,11 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, beta=None, activation=Non
     dx = None
     if need[0]:
         dx = _new_like(x, torch) if x.dim() == len(shape) else x.new_empty(shape)
-    dgamma = x.new_empty(width) if need[1] else None
-    dbeta = x.new_empty(width) if need[2] else None
+    dgamma = dbeta = None
+    if need[1]:
+        dgamma = x.new_empty(width) if gamma is None else torch.empty_like(gamma)
+    if need[2]:
+        dbeta = x.new_empty(width) if dgamma is None else torch.empty_like(dgamma)
     size = 0
     if need[1] or need[2]:
         size = _size(lib, (2, code, rows, width, device.index), lib.mace_layer_norm_backward_workspace, code, rows, width)
