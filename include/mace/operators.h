@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 enum { MACE_F32 = 0, MACE_BF16 = 1, MACE_F16 = 2 };
-/* silu z / (1 + exp(-z)); gelu z Phi(z) (the error function's, not a fit); relu max(z, 0) with
+/* silu z / (1 + exp(-z)); gelu z Phi(z) (by the error function, not by tanh); relu max(z, 0) with
  * slope 0 at 0. */
 enum { MACE_ACT_NONE = 0, MACE_ACT_SILU = 1, MACE_ACT_GELU = 2, MACE_ACT_RELU = 3 };
 

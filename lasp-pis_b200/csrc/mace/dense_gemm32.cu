@@ -122,8 +122,31 @@ struct Shared {
   int i0, j0; // its tile
   uint32_t tmem_base;
   volatile int abort_flag;
+  volatile int progress; // of sums that a drain warp adds again
   int arrived[8]; // per slot: split warps that are through with a slab
 };
+
+// Bounded wait, as mbar_wait; but results that are summed again may take a drain warp longer than that (a
+// finite number of them, each ends), and while their count grows the others wait on.
+__device__ __forceinline__ bool wait_for(unsigned bar, unsigned parity, Shared &sh) {
+  long long start = clock64();
+  int seen = sh.progress;
+  for (unsigned it = 1;; ++it) {
+    if (mbar_try(bar, parity))
+      return true;
+    if (sh.abort_flag)
+      return false;
+    if (it & 255)
+      continue;
+    if (sh.progress != seen) {
+      seen = sh.progress;
+      start = clock64();
+    } else if (clock64() - start > kWaitCycles) {
+      sh.abort_flag = 1;
+      return false;
+    }
+  }
+}
 
 // Row r of an operand's slab (ROWS rows, floats at `base`).  k-major: two boxes of ROWS rows by 32 k; a
 // thread's row is its own.  Turned: boxes of 64 k by 32 rows, which a warp's lanes read together.
@@ -227,14 +250,24 @@ template <bool Add> __device__ __forceinline__ void umma_f16_tmem(uint32_t d, ui
                "r"(a), "l"(b), "r"(idesc), "n"(int(Add)));
 }
 
-// sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time; ends early at NaN.
+// sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time, 8 per lane under way;
+// ends early at NaN.
 __device__ __forceinline__ float plain_sum(const float *p, long long pk, const float *q, long long qk, long long k0,
-                                        long long k1) {
+                                           long long k1) {
   float s = 0.f;
 #pragma unroll 1
-  for (long long k = k0 + (threadIdx.x & 31); k - (threadIdx.x & 31) < k1; k += 32) {
-    if (k < k1)
-      s = fmaf(p[k * pk], q[k * qk], s);
+  for (; k0 < k1; k0 += 256) {
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long long k = k0 + 32 * i + (threadIdx.x & 31), in = min(k, k1 - 1);
+      a[i] = p[in * pk];
+      b[i] = k < k1 ? q[in * qk] : 0.f;
+      a[i] = k < k1 ? a[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      s = fmaf(a[i], b[i], s);
     if (__any_sync(0xffffffffu, s != s))
       break;
   }
@@ -267,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   constexpr int kSplitWarps = kInTurn ? 4 : 8; // of each slab
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    sh.progress = 0;
     for (int s = 0; s < kStages; ++s)
       mbar_init(full0 + 8 * s, 1);
     for (int b = 0; b < kBuffers; ++b) {
@@ -297,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   // The MMAs of slab n (one thread).
   auto multiply = [&](int n) {
     const int b = n % kBuffers;
-    if (n >= kBuffers && !mbar_wait(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, &sh.abort_flag))
+    if (n >= kBuffers && !wait_for(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, sh))
       return;
     tc_fence_after();
     // Few instructions per MMA: while one thread issues, its warp's share of the next slab waits.  A
@@ -356,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
     int n = 0;
     for (Walk w(g); w.live(g); ++n) {
       if (!kInTurn || (n & 1) == group) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, &sh.abort_flag));
+        ok = __all_sync(0xffffffffu, ok && wait_for(full0 + 8 * (n % kStages), unsigned(n / kStages) & 1, sh));
         if (!ok) { // Q's other warps may wait at this slab's barrier
           if (QT && has_q)
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(BN) : "memory");
@@ -440,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         acc[c] = 0.f;
       for (bool same = true; same; same = !w.next(g), ++n) {
         const int b = n % kBuffers;
-        ok = ok && mbar_wait(tfull0 + 8 * b, unsigned(n / kBuffers) & 1, &sh.abort_flag) &&
-             mbar_wait(scaled0 + 8 * (n % kSlots), unsigned(n / kSlots) & 1, &sh.abort_flag);
+        ok = ok && wait_for(tfull0 + 8 * b, unsigned(n / kBuffers) & 1, sh) &&
+             wait_for(scaled0 + 8 * (n % kSlots), unsigned(n / kSlots) & 1, sh);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
           continue;
@@ -507,6 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
                                     g.q + (col0 + c) * (QT ? 1 : g.ldq), QT ? g.ldq : 1,
                                     (long long)s * g.slabs / g.parts * kBK,
                                     min(g.K, (s + 1ll) * g.slabs / g.parts * kBK));
+          if (lane == 0)
+            sh.progress = sh.progress + 1;
           if (lane == at) {
             odd &= odd - 1;
 #pragma unroll

@@ -94,7 +94,7 @@ template <bool Fast> __device__ __forceinline__ float activate(float z, int act)
   if (act == Silu)
     return __fdividef(z, exp_plus_one<Fast>(z));
   if (act == Gelu && Fast) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the tail is 0 from 40 on, NaN stays
-    const float m = fminf(fabsf(z), 40.f);
+    const float m = fmaxf(-z, fminf(z, 40.f)); // |z|; the formula's NaN for -infinity, but not for infinity
     float e;
     return fmaf(-m, normal_tail(m, e), z < 0.f ? 0.f : z);
   }
@@ -130,7 +130,7 @@ template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
     const float m = fminf(fabsf(z), 40.f);
     float e;
     const float h = normal_tail(m, e), s = fmaf(copysignf(m, z), e * 0.39894228f, z < 0.f ? h : 1.f - h);
-    return z != z ? z : s;
+    return fmaf(z, 0.f, s); // NaN where z is not finite, as the formula
   }
   if (act == Gelu) {
     float e = expf(-0.5f * z * z);

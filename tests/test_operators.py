@@ -317,6 +317,51 @@ def test_dense_not_finite_values_stay_in_their_rows(op, dtype):
 
 
 @gpu
+def test_dense_f32_all_results_infinite(op):
+    """Every result is an infinity, over long sums: each is summed again, which takes far longer
+    than the products, and the waits inside the kernel outlast it."""
+    import torch
+    M, K, N = 9600, 32768, 128
+    x = torch.ones(M, K, device="cuda")
+    x[:, K - 1] = math.inf
+    w = torch.ones(N, K, device="cuda")
+    w[::2, K - 1] = -1.0
+    want = torch.where(torch.arange(N, device="cuda") % 2 == 0, -math.inf, math.inf)
+    assert torch.equal(op.dense(x, w), want.expand(M, N))
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_activations_of_special_values(op, dtype, act):
+    """Infinities, NaN and the type's largest values give what the formulas give, in every type."""
+    import torch
+    dt = dtype_of(dtype)
+    big = torch.finfo(dt).max
+    v = torch.tensor([math.inf, -math.inf, math.nan, big, -big, 0.0, 100.0, -100.0], dtype=dt, device="cuda")
+    want, slope = act64(v.double(), act), slope64(v.double(), act)
+    for k in (1, 64):  # both kinds of product; the first input carries the value
+        x = torch.zeros(8, k, dtype=dt, device="cuda").repeat(20, 1)
+        x[:, 0] = v.repeat(20)
+        w = torch.zeros(16, k, dtype=dt, device="cuda")
+        w[:, 0] = 1
+        y, z = op.dense(x, w, None, act, keep=True)
+        expected = want.to(dt).repeat(20)[:, None].expand(160, 16)
+        assert torch.equal(y.isnan(), expected.isnan()) and torch.equal(z.isnan(), x[:, :1].isnan().expand(160, 16))
+        # (1e-30: the floats' exponential overflows where the formula's value is far below that.)
+        finite, bound = expected.isfinite(), (accumulation(dt, k) + 2 * half_step(dt)) * want.abs().repeat(20)[:, None] + 1e-30
+        assert torch.equal(y[expected.isinf()], expected[expected.isinf()])
+        close(y[finite], expected[finite].double(), bound.expand(160, 16)[finite], act)
+        one = torch.ones(1, 16, dtype=dt, device="cuda")
+        for i in range(8):
+            _, _, db = op.dense_backward(one, x[i:i + 1], w, act, z[i:i + 1], need=(False, False, True))
+            if slope[i].isnan():
+                assert db.isnan().all()
+            else:
+                assert (db.double() - slope[i]).abs().max() <= 2 * half_step(dt)
+
+
+@gpu
 def test_dense_f32_rows_of_any_magnitude(op):
     """Rows from 1e-25 to 1e25, and weights whose rows differ as much: the error stays relative to
     each row's own products."""
