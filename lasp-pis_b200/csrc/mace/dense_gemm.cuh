@@ -97,11 +97,11 @@ __device__ __forceinline__ void fetch_bias(const Epilogue &e, long long J, long 
 }
 
 // 32 rows by 128 bytes of the result from (row0, col0), rows = lanes.  get(c, v) gives the product's
-// columns col0 + c .. + 31, bias their bias in shared memory.  part >= 0 (T float): the
+// columns col0 + c .. + 31, bias their bias in shared memory (NULL: they have it).  part >= 0 (T float): the
 // values as they are, to plane `part`.  ready: the box's last store has read it, and the residual is on
 // its way; phase: of its barrier.  Rows are swizzled in shared memory, so that neither side has bank
-// conflicts; TMA writes whole lines.
-template <class T, class Get>
+// conflicts; TMA writes whole lines.  Bare: the epilogue is empty (the gradients' products).
+template <class T, bool Bare, class Get>
 __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, long long row0, long long col0, int part,
                                            const Box &w, unsigned &phase, bool ready, const T *bias, Get &&get) {
   constexpr bool Fast = sizeof(T) == 2;
@@ -109,10 +109,10 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
   using Un = Unit<T, U>;
   const int lane = threadIdx.x & 31;
   unsigned char *mine = w.at + lane * 128;
-  const bool plain = part >= 0;
+  const bool plain = Bare || part >= 0;
   auto block = [&](int c, float (&v)[32]) {
     get(c, v);
-    if (plain || !e.bias)
+    if (!bias)
       return;
 #pragma unroll
     for (int i = 0; i < 32; i += U) {
@@ -187,7 +187,7 @@ __device__ __forceinline__ void finish_box(const Epilogue &e, const Boxes &m, lo
       *at = o;
     }
   }
-  send(m.y, plain ? part : 0);
+  send(m.y, max(part, 0));
 }
 
 // 32 bytes at once (aligned to 32).
@@ -276,7 +276,7 @@ __device__ __forceinline__ void finish_row(const Epilogue &e, float *part, long 
 // NULL: the float values go to partial[row * J + col] instead.
 template <class T>
 __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
-                                             long long row0, long long col0, const float *v, unsigned char *box) {
+                                             long long row0, long long col0, const float *v, const T *bias, unsigned char *box) {
   constexpr bool Fast = sizeof(T) == 2;
   const int lane = threadIdx.x & 31, rows = int(min(32ll, I - row0));
   float *stage = reinterpret_cast<float *>(box);
@@ -287,7 +287,7 @@ __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, 
   __syncwarp();
   const long long col = col0 + lane;
   if (col < J) {
-    const float bias = e.bias && !partial ? to_float(static_cast<const T *>(e.bias)[col]) : 0.f;
+    const float add = bias ? to_float(bias[lane]) : 0.f;
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += 8) {
       float x[8];
@@ -298,7 +298,7 @@ __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, 
           res[i] = static_cast<const T *>(e.residual)[(row0 + r0 + i) * e.ldr + col];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        x[i] = stage[(r0 + i) * 32 + (lane ^ (r0 + i))] + bias;
+        x[i] = stage[(r0 + i) * 32 + (lane ^ (r0 + i))] + add;
       if (partial) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)

@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
         } else if (g.boxes.on && g.partial) {
 #pragma unroll 1
           for (int c = first; c < end && j * BN + c < g.J; c += 32)
-            finish_box<float>(g.e, g.boxes, row0, j * BN + c, int(s), w, phase, false,
+            finish_box<float, true>(g.e, g.boxes, row0, j * BN + c, int(s), w, phase, false,
                               nullptr, [&](int k, float (&v)[32]) { get(c + k, v); });
         } else if (g.boxes.on) {
           // 64 columns to a box: where the tile has no more, the first of a quarter's two warps has it.
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int x = 0; x < (BN + 127) / 128; ++x) {
             const int c = first * step + 64 * x;
             if (c < end && j * BN + c < g.J)
-              finish_box<T>(g.e, g.boxes, row0, j * BN + c, -1, w, phase, false,
-                            bias + 64 * x, [&](int k, float (&v)[32]) { get(c + k, v); });
+              finish_box<T, QT>(g.e, g.boxes, row0, j * BN + c, -1, w, phase, false,
+                            g.e.bias ? bias + 64 * x : nullptr, [&](int k, float (&v)[32]) { get(c + k, v); });
           }
         } else {
           float *partial = g.partial ? g.partial + s * g.I * g.J : nullptr;
@@ -234,7 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int c = first; c < end && j * BN + c < g.J; c += 32) {
             float v[32];
             get(c, v);
-            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, w.at);
+            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, g.e.bias && !partial ? bias + c - (BN >= 128 ? first : 0) : nullptr,
+                           w.at);
           }
         }
       }

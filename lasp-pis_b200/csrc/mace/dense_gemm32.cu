@@ -20,13 +20,16 @@
 //           of Q per thread; the latencies of a split, not its instructions, take its time, and so
 //           two are under way (gradients of 84613 x 64 -> 1280: 351 -> 291 us).  128-wide ones have
 //           only two stages, which one group uses better (61 us against 67 for 10000 x 512 -> 512):
-//           four warps P, four Q.  The warp that finishes a slab last issues its MMAs.
+//           four warps P, four Q.  The warp that finishes a slab last issues its MMAs, all operands
+//           uniform (84613 x 64 -> 1280: 182 -> 172 us).
 //   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
-//           epilogue.  A slab that has reached TMEM has left its stage: warp 8 then starts the
-//           loads of the slab that takes its place.
-// What bounds it: no unit (gradients of 84613 x 64 -> 1280: issue slots 34% busy, DRAM 33%, tensor pipe
-// 12%), but the chain load, split, multiply, drain of a slab at one CTA per SM; with one slab per
-// tile (84613 x 64 -> 1280: 200 us, 2.3 TB/s) the drain's epilogue.  Measured and not kept: plain loads
+//           epilogue.  A slab that has reached TMEM has left its stage: one of them (in turn) then
+//           starts the loads of the slab that takes its place.
+// What bounds it: no unit (gradients of 84613 x 64 -> 1280, 275 us: issue slots 34% busy, DRAM 33%, tensor
+// pipe 12%), but the chain load, split, multiply, drain of a slab at one CTA per SM (10000 x 512 -> 512: 55
+// us); with one slab per tile (84613 x 64 -> 1280: 172 us, 2.6 TB/s) the drain, by its instructions'
+// latencies: the bias as the sums' first value, prefetched, and scales as whole floats took it from 200 us
+// to 179.  Measured and not kept: plain loads
 // straight into the split's registers (10000 x 512 -> 512: 174 us, then 104 with TMA), P split in place
 // (358 us where TMEM gave 351), L2 prefetches of P (no change), three stages and one box of results for
 // 128-wide tiles (84613 x 64 -> 1280: 245 us), results written from registers by sectors (227 us).
@@ -49,7 +52,7 @@ static_assert(buffers<64>() * 64 + stages<64>() * 64 <= 512 && buffers<128>() * 
 // The split of slab g runs after the MMAs of g - stages, which waited for the drain of the slab
 // `buffers` before that.
 template <int BN> constexpr int slots() { return buffers<BN>() + stages<BN>(); }
-template <int BN> constexpr int slot_bytes() { return 2 * BN + kBM; }
+template <int BN> constexpr int slot_bytes() { return 4 * BN + kBM; }
 template <int BN> constexpr int smem_bytes() {
   return stages<BN>() * stage_bytes<BN>() + 8 * (BN / 64) * kBoxBytes + 8 * (BN / 2) * 4 + slots<BN>() * slot_bytes<BN>() + 512;
 }
@@ -91,7 +94,6 @@ __device__ __forceinline__ void split2(float2 v, float2 scale, uint32_t &hi, uin
 struct Walk {
   unsigned u, tile;
   int k, end, part;
-  Walk() = default;
   __device__ __forceinline__ explicit Walk(const Gemm32 &g) : u(blockIdx.x) { open(g); }
   __device__ __forceinline__ void open(const Gemm32 &g) {
     part = 0;
@@ -110,16 +112,17 @@ struct Walk {
   __device__ __forceinline__ bool next(const Gemm32 &g) {
     if (++k < end)
       return false;
+    skip(g);
+    return true;
+  }
+  __device__ __forceinline__ void skip(const Gemm32 &g) {
     u += gridDim.x;
     open(g);
-    return true;
   }
 };
 
-// The walk's state of the loads, and what the warps share.
+// What the warps share.
 struct Shared {
-  Walk ahead;
-  int i0, j0; // its tile
   uint32_t tmem_base;
   volatile int abort_flag;
   volatile int progress; // of sums that a drain warp adds again
@@ -190,14 +193,11 @@ __device__ __forceinline__ float row_sum(const float (&v)[64]) {
   s[0] = __fadd2_rn(__fadd2_rn(s[0], s[1]), __fadd2_rn(s[2], s[3]));
   return s[0].x + s[0].y;
 }
-// 32 columns of this warp's 32 lanes.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+// 16 columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-               "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-               "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
 // P's row r to TMEM, lane = row: hi in 32 columns from `taddr` (two k each), lo in the next 32.  Returns
@@ -210,12 +210,15 @@ __device__ __forceinline__ unsigned split_p(const unsigned char *base, int r, ui
     *sum += row_sum(v);
   const int e = row_power(v);
   const float2 scale = make_float2(pow2(e), pow2(e));
-  uint32_t h[32], l[32];
 #pragma unroll
-  for (int p = 0; p < 32; ++p)
-    split2(make_float2(v[2 * p], v[2 * p + 1]), scale, h[p], l[p]);
-  tmem_st32(taddr, h);
-  tmem_st32(taddr + 32, l);
+  for (int c = 0; c < 32; c += 16) {
+    uint32_t h[16], l[16];
+#pragma unroll
+    for (int p = 0; p < 16; ++p)
+      split2(make_float2(v[2 * (c + p)], v[2 * (c + p) + 1]), scale, h[p], l[p]);
+    tmem_st16(taddr + c, h);
+    tmem_st16(taddr + 32 + c, l);
+  }
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
   tc_fence_before();
   return unsigned(127 - e);
@@ -241,6 +244,12 @@ template <int ROWS, bool Turned> __device__ __forceinline__ unsigned split_q(uns
     *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
   return unsigned(127 - e);
+}
+// True in one thread of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 // D (TMEM) (+)= A (TMEM) B (shared memory).
 template <bool Add> __device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
@@ -285,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *staging = smem + kStages * kStageBytes; // the drain warps' boxes, then their bias
   float *biases = reinterpret_cast<float *>(staging + 8 * kBoxes * kBoxBytes);
-  // [kSlots][2 BN + kBM]: 2^-e of Q's rows (the upper halves of floats), then 127 - e of P's
+  // [kSlots][4 BN + kBM]: 2^-e of Q's rows (floats), then 127 - e of P's (bytes)
   unsigned char *scales = reinterpret_cast<unsigned char *>(biases + 8 * (BN / 2));
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kSlots * kSlotBytes);
   // full[S] | tfull[B] | tfree[B] | scaled[kSlots] | residual[8 x boxes]
@@ -328,16 +337,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
 
   // P's split slab n: 64 columns behind the accumulators, a place for each stage.
   auto p_columns = [&](int n) { return tmem + uint32_t(kBuffers * BN + n % kStages * 64); };
-  // The MMAs of slab n (one thread).
+  // The MMAs of slab n (one warp, one of its threads: what the warp computes together is uniform, which
+  // the instructions' operands have to be).
   auto multiply = [&](int n) {
     const int b = n % kBuffers;
-    if (n >= kBuffers && !wait_for(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, sh))
+    if (!__all_sync(0xffffffffu, n < kBuffers || wait_for(tfree0 + 8 * b, unsigned(n / kBuffers - 1) & 1, sh)))
       return;
     tc_fence_after();
     // Few instructions per MMA: while one thread issues, its warp's share of the next slab waits.  A
     // 16-wide step is 32 bytes (2 descriptor units) of Q, 8 columns of P.
     const uint64_t qh = smem_desc(smem_u32(smem + n % kStages * kStageBytes) + 2 * kPBytes), ql = qh + (kQBytes >> 4);
     const uint32_t d = tmem + uint32_t(b * BN), ph = p_columns(n), pl = ph + 32, idesc = g.idesc;
+    if (!elect_one())
+      return;
     umma_f16_tmem<false>(d, pl, qh, idesc); // the small terms first
     umma_f16_tmem<true>(d, ph, ql, idesc);
 #pragma unroll
@@ -350,14 +362,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       umma_f16_tmem<true>(d, ph + 8 * m, qh + 2 * m, idesc);
     umma_commit(tfull0 + 8 * b);
   };
-  // The loads of slab n at sh.ahead, which moves on (one thread; the MMAs of slab n - 2 are done).
-  auto open_ahead = [&] {
+  // The loads of slab n at w (one thread; the MMAs of slab n - kStages are done).
+  auto fetch = [&](int n, const Walk &w) {
     long long i, j;
-    g.tiles.at(sh.ahead.tile, i, j);
-    sh.i0 = int(i * kBM), sh.j0 = int(j * BN);
-  };
-  auto fetch = [&](int n) {
-    const int i0 = sh.i0, j0 = sh.j0, k0 = sh.ahead.k * kBK;
+    g.tiles.at(w.tile, i, j);
+    const int i0 = int(i * kBM), j0 = int(j * BN), k0 = w.k * kBK;
     const unsigned base = smem_u32(smem + n % kStages * kStageBytes), full = full0 + 8 * (n % kStages);
     mbar_expect_tx(full, kStageBytes);
     if (PT) {
@@ -376,13 +385,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       tma_load_2d(base + 2 * kPBytes, &g.mq, k0, j0, full);
       tma_load_2d(base + 2 * kPBytes + kQBytes, &g.mq, k0 + 32, j0, full);
     }
-    if (sh.ahead.next(g) && sh.ahead.live(g))
-      open_ahead();
   };
 
-  // Registers: 128 each at launch; 256 threads give 32 to the other 256 (96 + 160 = 2 x 128).
+  // Registers: 128 each at launch; the 256 threads that split give some to the 256 that drain (2 x 128
+  // in all).  84613 x 64 -> 1280 and its gradients with 96: 186 and 292 us, 112: 184 and 275, 128: 191 and 277.
+  constexpr int kSplitRegs = 112;
   if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSplitRegs));
     const int group = warp >> 2, r = threadIdx.x & 127;
     const bool has_p = kInTurn || group == 0, has_q = kInTurn ? r < BN : group == 1;
     bool ok = true; // the same in the whole warp
@@ -398,24 +407,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         } else {
           unsigned char *stage = smem + n % kStages * kStageBytes, *scale = scales + n % kSlots * kSlotBytes;
           if (has_p)
-            scale[2 * BN + r] = static_cast<unsigned char>(
+            scale[4 * BN + r] = static_cast<unsigned char>(
                 split_p<PT>(stage, r, p_columns(n) + (uint32_t(32 * (warp & 3)) << 16), PT && g.sums ? &sum : nullptr));
           if (has_q)
-            reinterpret_cast<unsigned short *>(scale)[r] =
-                static_cast<unsigned short>(split_q<BN, QT>(stage + 2 * kPBytes, r, 1 + group) << 7);
+            reinterpret_cast<unsigned *>(scale)[r] = split_q<BN, QT>(stage + 2 * kPBytes, r, 1 + group) << 23;
           // Each lane's stores, then the warp's, are visible before the warp counts as arrived; the
           // last to arrive sees all of them.
           fence_proxy_async_smem();
           __threadfence_block();
           __syncwarp();
+          int before = 0;
           if (lane == 0) {
             mbar_arrive(scaled0 + 8 * (n % kSlots)); // this warp's scales, for the drain
-            if (atomicAdd(&sh.arrived[n % kSlots], 1) == kSplitWarps - 1) {
+            before = atomicAdd(&sh.arrived[n % kSlots], 1);
+            if (before == kSplitWarps - 1)
               sh.arrived[n % kSlots] = 0;
-              __threadfence_block();
-              fence_proxy_async_smem();
-              multiply(n);
-            }
+            __threadfence_block();
+          }
+          if (__shfl_sync(0xffffffffu, before, 0) == kSplitWarps - 1) {
+            fence_proxy_async_smem();
+            multiply(n);
           }
         }
       }
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(256 - kSplitRegs));
     constexpr int kCols = BN / 2;
     const int quarter = warp & 3, half = (warp - 8) >> 2;
     const int me = warp - 8;
@@ -444,24 +455,59 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       boxes[x] = {staging + (kBoxes * me + x) * kBoxBytes, residual0 + 8 * (kBoxes * me + x)};
     float *bias = biases + me * kCols;
     // A tile's residual is on its way while the tile accumulates (a kept z needs the boxes first).
-    const bool early = g.boxes.on && !g.partial && g.e.residual && !g.e.z;
-    if (me == 0 && lane == 0) {
-      sh.ahead = Walk(g);
-      open_ahead();
-      for (int x = 0; x < kStages && sh.ahead.live(g); ++x)
-        fetch(x);
+    const bool early = !QT && g.boxes.on && !g.partial && g.e.residual && !g.e.z;
+    Walk ahead(g); // of the loads
+    for (int x = 0; x < kStages && ahead.live(g); ++x) {
+      if (me == x && lane == 0)
+        fetch(x, ahead);
+      ahead.next(g);
     }
+    // A unit's tile and its bias are ready before the unit: the drain's latencies are what a unit takes.
+    int next_i = 0, next_j = 0; // its rows' and columns' tile
+    float next_bias[kCols / 32] = {};
+    auto prepare = [&](unsigned tile) {
+      long long i, j;
+      g.tiles.at(tile, i, j);
+      next_i = int(i), next_j = int(j);
+      if (!QT && g.e.bias && !g.partial)
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h)
+          next_bias[h] = static_cast<const float *>(g.e.bias)[min(j * BN + half * kCols + 32 * h + lane, g.J - 1)];
+    };
     float acc[kCols];
     bool ok = true;
     int n = 0;
-    for (Walk w(g); w.live(g);) {
+    Walk w(g);
+    if (w.live(g))
+      prepare(w.tile);
+    while (w.live(g)) {
       const int s = w.part;
-      long long i, j;
-      g.tiles.at(w.tile, i, j);
+      const long long i = next_i, j = next_j;
       const long long row0 = i * kBM + 32 * quarter, row = row0 + lane, cols0 = j * BN + half * kCols;
       const bool any = row0 < g.I && cols0 < g.J;
-      if (!g.partial)
-        fetch_bias<float>(g.e, g.J, cols0, kCols, bias);
+      // The sums start with the bias (the gradients' products have none).
+      if (QT) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          acc[c] = 0.f;
+      } else {
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h)
+          bias[32 * h + lane] = next_bias[h];
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+          const float4 f = *reinterpret_cast<const float4 *>(bias + c);
+          acc[c] = f.x, acc[c + 1] = f.y, acc[c + 2] = f.z, acc[c + 3] = f.w;
+        }
+        __syncwarp();
+      }
+      {
+        Walk after = w;
+        after.skip(g);
+        if (after.live(g))
+          prepare(after.tile);
+      }
       if (early && any && lane == 0) {
         bulk_wait_read();
 #pragma unroll
@@ -469,9 +515,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           if (cols0 + 32 * c < g.J)
             fetch_residual(g.boxes, boxes[c], row0, cols0 + 32 * c);
       }
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        acc[c] = 0.f;
       for (bool same = true; same; same = !w.next(g), ++n) {
         const int b = n % kBuffers;
         ok = ok && wait_for(tfull0 + 8 * b, unsigned(n / kBuffers) & 1, sh) &&
@@ -479,35 +522,34 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         ok = __all_sync(0xffffffffu, ok);
         if (!ok)
           continue;
-        if (me == 0 && lane == 0 && sh.ahead.live(g))
-          fetch(n + kStages);
+        if (me == (n & 7) && lane == 0 && ahead.live(g)) // in turn: no warp falls behind by all of them
+          fetch(n + kStages, ahead);
+        ahead.next(g);
         tc_fence_after();
         const unsigned char *scale = scales + n % kSlots * kSlotBytes;
-        const unsigned char *fq = scale + 2 * (half * kCols);
+        const float *fq = reinterpret_cast<const float *>(scale) + half * kCols;
         // 2^-e of P's row, one ulp more in three slabs of four.
-        const float fp = __uint_as_float((uint32_t(scale[2 * BN + 32 * quarter + lane]) << 23) + ((w.k & 3) != 3));
+        const float fp = __uint_as_float((uint32_t(scale[4 * BN + 32 * quarter + lane]) << 23) + ((w.k & 3) != 3));
         const float2 fp2 = make_float2(fp, fp);
-        uint32_t r[kCols / 32][32];
 #pragma unroll
-        for (int h = 0; h < kCols / 32; ++h)
-          tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + half * kCols + 32 * h), r[h]);
-        tmem_wait_ld();
+        for (int h = 0; h < kCols; h += 32) {
+          uint32_t r[32];
+          tmem_ld32_async(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(b * BN + half * kCols + h), r);
+          tmem_wait_ld();
+          tmem_anchor(r);
+          if (h + 32 == kCols) {
+            tc_fence_before();
+            mbar_arrive(tfree0 + 8 * b);
+          }
 #pragma unroll
-        for (int h = 0; h < kCols / 32; ++h)
-          tmem_anchor(r[h]);
-        tc_fence_before();
-        mbar_arrive(tfree0 + 8 * b);
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
-          const uint2 f = *reinterpret_cast<const uint2 *>(fq + 2 * c);
-          const uint32_t fs[2] = {f.x, f.y};
-#pragma unroll
-          for (int y = 0; y < 2; ++y) { // the two scalings, and the float sum
-            const int x = c + 2 * y;
-            const float2 s = make_float2(__uint_as_float(fs[y] << 16), __uint_as_float(fs[y] & 0xffff0000u));
-            const float2 v = make_float2(__uint_as_float(r[x / 32][x % 32]), __uint_as_float(r[x / 32][x % 32 + 1]));
-            const float2 a = __ffma2_rn(__fmul2_rn(v, s), fp2, make_float2(acc[x], acc[x + 1]));
-            acc[x] = a.x, acc[x + 1] = a.y;
+          for (int c = 0; c < 32; c += 4) { // the two scalings, and the float sum
+            const float4 f = *reinterpret_cast<const float4 *>(fq + h + c);
+            const float2 v = make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            const float2 u = make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+            const int x = h + c;
+            const float2 a = __ffma2_rn(__fmul2_rn(v, make_float2(f.x, f.y)), fp2, make_float2(acc[x], acc[x + 1]));
+            const float2 d = __ffma2_rn(__fmul2_rn(u, make_float2(f.z, f.w)), fp2, make_float2(acc[x + 2], acc[x + 3]));
+            acc[x] = a.x, acc[x + 1] = a.y, acc[x + 2] = d.x, acc[x + 3] = d.y;
           }
         }
       }
@@ -537,10 +579,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         }
         while (const unsigned lanes = __ballot_sync(0xffffffffu, odd != 0)) {
           const int at = __ffs(lanes) - 1, c = __ffs(__shfl_sync(0xffffffffu, odd, at)) - 1;
-          const float x = plain_sum(g.p + (row0 + at) * (PT ? 1 : g.ldp), PT ? g.ldp : 1,
+          float x = plain_sum(g.p + (row0 + at) * (PT ? 1 : g.ldp), PT ? g.ldp : 1,
                                     g.q + (col0 + c) * (QT ? 1 : g.ldq), QT ? g.ldq : 1,
                                     (long long)s * g.slabs / g.parts * kBK,
                                     min(g.K, (s + 1ll) * g.slabs / g.parts * kBK));
+          if (!QT && g.e.bias && !g.partial)
+            x += static_cast<const float *>(g.e.bias)[col0 + c];
           if (lane == 0)
             sh.progress = sh.progress + 1;
           if (lane == at) {
@@ -552,15 +596,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
           }
         }
         if (g.boxes.on)
-          finish_box<float>(
-              g.e, g.boxes, row0, col0, g.partial ? s : -1, boxes[c0 / 32], phase[c0 / 32], early || (c0 && !g.e.z), bias + c0,
+          finish_box<float, QT>(
+              g.e, g.boxes, row0, col0, g.partial ? s : -1, boxes[c0 / 32], phase[c0 / 32], early || (c0 && !g.e.z), nullptr,
               [&](int, float (&v)[32]) {
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
                   v[c] = acc[c0 + c];
               });
         else
-          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, boxes[0].at);
+          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, nullptr, boxes[0].at);
       }
     }
     if (lane == 0)
