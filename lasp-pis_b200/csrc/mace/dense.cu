@@ -105,7 +105,8 @@ void narrow(const Dense &d, cudaStream_t stream) {
 // stream it.  A warp has four rows of W under way, eight 16-byte loads per lane in flight, finds x in
 // L1, and `ks` warps of a block share them along k where there are few outputs.  Float
 // sums: lanes, then the warps in order.  M: d.rows or a little more (rows past the last read it).
-// Turned: the same for a few outputs, with x in W's place and W in x's.
+// Turned: the same for a few outputs, with x in W's place and W in x's.  gridDim.y: further groups of M
+// rows (see is_small).
 constexpr int kFew = 8, kFewOutputs = 4;
 // A unit that is read once, in the order written (all of a step's loads before the first use).
 template <class T, int U> __device__ __forceinline__ Unit<T, U> stream_unit(const T *p) {
@@ -129,6 +130,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
   using Un = Unit<T, U>;
   __shared__ float parts[8][R * M];
   const T *const x = static_cast<const T *>(Turned ? d.weight : d.x);
+  const long long few0 = (long long)blockIdx.y * M;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = warp % ks, slot = warp / ks, slots = 8 / ks;
   // Groups of four outputs go round the blocks first, so that every SM reads as much.
@@ -168,8 +170,8 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
       }
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + at * U);
-        u[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + (at + step) * U);
+        v[m] = *reinterpret_cast<const Un *>(x + min(few0 + m, few - 1) * ldf + at * U);
+        u[m] = *reinterpret_cast<const Un *>(x + min(few0 + m, few - 1) * ldf + (at + step) * U);
       }
       add(a, v);
       add(b, u);
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
         a[r] = stream_unit<T, U>(w[r] + at * U);
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        v[m] = *reinterpret_cast<const Un *>(x + min((long long)m, few - 1) * ldf + at * U);
+        v[m] = *reinterpret_cast<const Un *>(x + min(few0 + m, few - 1) * ldf + at * U);
       add(a, v);
     }
     __syncwarp();
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ D
           mine += parts[warp + s][lane];
       __syncthreads();
     }
-    const long long at_many = n0 + lane / M, at_few = lane % M;
+    const long long at_many = n0 + lane / M, at_few = few0 + lane % M;
     if (!sub && lane < R * M && at_many < many && at_few < few) {
       const Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz};
       finish<T>(e, Turned ? at_many : at_few, Turned ? at_few : at_many, mine);
@@ -224,16 +226,26 @@ bool is_few(const Dense &d) {
 }
 // Few outputs: the tensor cores' tiles would be mostly empty, and x is what streams.
 bool is_few_outputs(const Dense &d) { return d.outputs <= kFew; }
+// Small products whose operands TMA cannot read: every warp forms its 4 x 8 sums, the operands come from
+// L2, and nothing is copied or cut first.  f32 and bf16 393 x 1235 -> 27: 7.5 and 7.7 us here, 19.7 and
+// 16.1 with copies and the tensor cores; but bf16 1000 x 565 -> 110 (62 million products) 18.4 and 13.6, and
+// 10000 x 65 -> 64 (640,000 sums, whose joining over a warp bounds it) 25.8 and 9.5.
+constexpr long long kSmallSums = 1ll << 17, kSmallProducts = 1ll << 25;
+bool is_small(const Dense &d) {
+  return d.rows * d.outputs <= std::min(kSmallSums, kSmallProducts / d.inputs) &&
+         !(tma_ready(d.type, d.x, d.rows, d.ldx) && tma_ready(d.type, d.weight, d.outputs, d.ldw));
+}
 template <class T, int U, int M, bool Turned> void launch_few(const Dense &d, cudaStream_t stream) {
+  const long long rest = ((Turned ? d.outputs : d.rows) + M - 1) / M;
   const long long groups = ((Turned ? d.rows : d.outputs) + kFewOutputs - 1) / kFewOutputs;
   // Warps share a group while there are fewer groups than warps and each keeps two steps of k.
   int ks = 1;
-  while (ks < 8 && groups * ks < 16ll * sm_count() && d.inputs / U >= 128ll * ks)
+  while (ks < 8 && groups * rest * ks < 16ll * sm_count() && d.inputs / U >= 128ll * ks)
     ks *= 2;
   const long long blocks = (groups + 8 / ks - 1) / (8 / ks);
   // As many blocks as fit, so that groups spread evenly over the SMs; fewer where they are not filled.
-  lapis::launch(few_rows_kernel<T, U, M, Turned>, dim3(unsigned(std::min<long long>(blocks, 4ll * sm_count()))), 256, 0,
-                stream, d, ks);
+  lapis::launch(few_rows_kernel<T, U, M, Turned>, dim3(unsigned(std::min<long long>(blocks, 4ll * sm_count())), unsigned(rest)),
+                256, 0, stream, d, ks);
   lapis::check(cudaGetLastError());
 }
 void few_rows(const Dense &d, bool turned, cudaStream_t stream) {
@@ -326,6 +338,146 @@ __global__ void __launch_bounds__(256)
     if (c0 + c < a.outputs)
       partial[blockIdx.y * a.outputs + c0 + c] = s;
   }
+}
+
+// ---------------- small gradients ----------------
+// All gradients of a layer with few weights, any alignment, float arithmetic: a block takes kSmallRows rows
+// or fewer (as shared memory allows) at a time, forms their dz (rounded to the type) beside x and W in
+// shared memory, writes their dx, and adds to dW and db -- x has one more column of ones for db -- in
+// registers.  Many rows: each block writes a partial [outputs][inputs + 1], which a second launch adds.
+// Launches are what bound such calls, one or two here and 4 to 8 with the tensor cores (f32 with SiLU,
+// here and there: 12 x 9 -> 7 4.4 and 22 us, 18081 x 8 -> 24 11.7 and 40, 295 x 338 -> 12 18 and 41; bf16
+// 4096 x 63 -> 64 26 and 29).  What bounds large ones is shared memory, two reads for each product, so
+// steps are short where there are many weights, and blocks many; bf16 1000 x 1000 -> 4, whose steps are
+// short and wide, takes 27 us and 17.
+constexpr int kSmallRows = 64, kSmallWeights = 4096, kSmallWidth = 512, kSmallFloats = 16384;
+constexpr long long kSmallWork = 1ll << 24; // products of a pair of values, for dW
+struct SmallGradients {
+  int rows, blocks; // of a step; of the grid
+  unsigned shared;
+};
+bool is_small(const DenseBackward &d) {
+  return d.outputs + d.inputs < kSmallWidth && d.outputs * (d.inputs + 1) <= kSmallWeights &&
+         d.rows <= kSmallWork / (d.outputs * (d.inputs + 1));
+}
+SmallGradients small_gradients(const DenseBackward &d) {
+  SmallGradients s;
+  const int width = int(d.outputs + d.inputs + 1);
+  s.rows = std::min({kSmallRows, kSmallFloats / width, std::max(8, 32768 / int(d.outputs * (d.inputs + 1)))});
+  s.shared = unsigned(std::max(s.rows * width + int(d.outputs * d.inputs), 256)) * 4u; // (256: the groups' sums)
+  s.blocks = int(std::min<long long>((d.rows + s.rows - 1) / s.rows, std::min(4ll, 200000ll / (s.shared + 1024)) * sm_count()));
+  return s;
+}
+// Value e of [outputs][inputs + 1] (dW, db) to its place.
+template <class T> __device__ __forceinline__ void small_result(const DenseBackward &a, int e, float v) {
+  const int W = int(a.inputs) + 1, o = e / W, i = e - o * W;
+  if (i < W - 1) {
+    if (a.dweight)
+      static_cast<T *>(a.dweight)[o * a.lddw + i] = from_float<T>(v);
+  } else if (a.dbias) {
+    static_cast<T *>(a.dbias)[o] = from_float<T>(v);
+  }
+}
+template <class T>
+__global__ void __launch_bounds__(256)
+    small_gradient_kernel(const __grid_constant__ DenseBackward a, int step, float *partial) {
+  constexpr bool Fast = sizeof(T) == 2;
+  constexpr int kMine = kSmallWeights / 256;
+  extern __shared__ float shared[];
+  const int I = int(a.inputs), O = int(a.outputs), W = I + 1, n = O * W;
+  float *const xs = shared, *const dz = xs + step * W, *const ws = dz + step * O; // [step][W], [step][O], [O][I]
+  const int t = threadIdx.x;
+  if (a.dx)
+    for (int e = t; e < O * I; e += 256)
+      ws[e] = to_float(static_cast<const T *>(a.weight)[(long long)(e / I) * a.ldw + e % I]);
+  // Fewer sums than threads: groups of threads take every groups-th row.
+  const int groups = n < 256 ? 256 / n : 1, group = n < 256 ? t / n : 0, mine = n < 256 ? t % n : t;
+  float acc[kMine] = {};
+  for (long long r0 = (long long)blockIdx.x * step; r0 < a.rows; r0 += (long long)gridDim.x * step) {
+    const int rows = int(min((long long)step, a.rows - r0));
+    __syncthreads();
+    if (a.dweight)
+      for (int e = t; e < rows * I; e += 256) {
+        const int r = e / I, i = e - r * I;
+        xs[r * W + i] = to_float(static_cast<const T *>(a.x)[(r0 + r) * a.ldx + i]);
+      }
+    for (int r = t; r < rows; r += 256)
+      xs[r * W + I] = 1.f;
+    for (int e = t; e < rows * O; e += 256) {
+      const int r = e / O, o = e - r * O;
+      float v = to_float(static_cast<const T *>(a.dy)[(r0 + r) * a.lddy + o]);
+      if (a.activation != None)
+        v *= slope<Fast>(to_float(static_cast<const T *>(a.z)[(r0 + r) * a.ldz + o]), a.activation);
+      dz[e] = to_float(from_float<T>(v)); // (in 16 bits, as for the larger products)
+    }
+    __syncthreads();
+    if (a.dx)
+      for (int e = t; e < rows * I; e += 256) {
+        const int r = e / I, i = e - r * I;
+        float s = 0.f;
+#pragma unroll 4
+        for (int o = 0; o < O; ++o)
+          s = fmaf(dz[r * O + o], ws[o * I + i], s);
+        static_cast<T *>(a.dx)[(r0 + r) * a.lddx + i] = from_float<T>(s);
+      }
+    if ((a.dweight || a.dbias) && group < groups) {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const int e = mine + 256 * k;
+        if (e < n && (k == 0 || groups == 1)) {
+          const int o = e / W;
+          const float *const g = dz + o, *const x = xs + (e - o * W);
+          float s = acc[k];
+          if (a.dweight || e - o * W == I)
+#pragma unroll 4
+            for (int r = group; r < rows; r += groups)
+              s = fmaf(g[r * O], x[r * W], s);
+          acc[k] = s;
+        }
+      }
+    }
+  }
+  if (!a.dweight && !a.dbias)
+    return;
+  if (groups > 1) { // the groups' sums in order
+    __syncthreads();
+    shared[t] = acc[0];
+    __syncthreads();
+    float s = 0.f;
+    if (t < n)
+      for (int k = 0; k < groups; ++k)
+        s += shared[k * n + t];
+    acc[0] = s;
+  }
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int e = t + 256 * k;
+    if (e < n) {
+      if (partial)
+        partial[(long long)blockIdx.x * n + e] = acc[k];
+      else
+        small_result<T>(a, e, acc[k]);
+    }
+  }
+}
+// The partials' sums: 32 values per block, in a fixed order.
+template <class T>
+__global__ void __launch_bounds__(1024)
+    small_sum_kernel(const __grid_constant__ DenseBackward a, const float *partial, int parts) {
+  __shared__ float sum[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n = int(a.outputs * (a.inputs + 1)), e = int(blockIdx.x) * 32 + x;
+  float s = 0.f;
+  if (e < n)
+    for (int p = y; p < parts; p += 32)
+      s += partial[(long long)p * n + e];
+  sum[y][x] = s;
+  __syncthreads();
+  float v = sum[x][y];
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (!x && int(blockIdx.x) * 32 + y < n)
+    small_result<T>(a, int(blockIdx.x) * 32 + y, v);
 }
 
 // Copy of a [rows][cols] array with any row distance and alignment into rows of ldo elements (a multiple
@@ -453,14 +605,14 @@ struct BackwardLayout {
 };
 } // namespace
 
-long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) || is_few_outputs(d) ? 0 : ForwardLayout(d).total; }
+long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) || is_few_outputs(d) || is_small(d) ? 0 : ForwardLayout(d).total; }
 void dense(const Dense &d, void *workspace, cudaStream_t stream) {
   if (is_narrow(d)) {
     narrow(d, stream);
     return;
   }
-  if (is_few(d) || is_few_outputs(d)) {
-    few_rows(d, !is_few(d), stream);
+  if (is_few(d) || is_few_outputs(d) || is_small(d)) {
+    few_rows(d, !is_few(d) && is_few_outputs(d), stream);
     return;
   }
   const ForwardLayout l(d);
@@ -471,7 +623,34 @@ void dense(const Dense &d, void *workspace, cudaStream_t stream) {
   product(p, static_cast<char *>(workspace) + l.product, stream);
 }
 
-long long dense_backward_workspace(const DenseBackward &d) { return BackwardLayout(d).total; }
+long long dense_backward_workspace(const DenseBackward &d) {
+  if (is_small(d)) {
+    const int blocks = small_gradients(d).blocks;
+    return blocks > 1 ? round_up(blocks * d.outputs * (d.inputs + 1) * 4, 16) : 0;
+  }
+  return BackwardLayout(d).total;
+}
+namespace {
+void small_backward(const DenseBackward &d, float *partial, cudaStream_t stream) {
+  const SmallGradients s = small_gradients(d);
+  with_type(d.type, [&](auto tag) {
+    using T = decltype(tag);
+    static thread_local int configured = -1;
+    int device = 0;
+    lapis::check(cudaGetDevice(&device));
+    if (configured != device) {
+      lapis::check(cudaFuncSetAttribute(small_gradient_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (kSmallFloats + kSmallWeights) * 4));
+      configured = device;
+    }
+    const bool sums = s.blocks > 1 && (d.dweight || d.dbias);
+    lapis::launch(small_gradient_kernel<T>, dim3(unsigned(s.blocks)), 256, s.shared, stream, d, s.rows, sums ? partial : nullptr);
+    if (sums)
+      lapis::launch(small_sum_kernel<T>, dim3(unsigned((d.outputs * (d.inputs + 1) + 31) / 32)), 1024, 0, stream, d, partial, s.blocks);
+    lapis::check(cudaGetLastError());
+  });
+}
+} // namespace
 void dense_backward(const DenseBackward &d, void *workspace, cudaStream_t stream) {
   if (!d.rows) { // sums of nothing
     if (d.dweight)
@@ -479,6 +658,11 @@ void dense_backward(const DenseBackward &d, void *workspace, cudaStream_t stream
                                      size_t(d.outputs), stream));
     if (d.dbias)
       lapis::check(cudaMemsetAsync(d.dbias, 0, size_t(d.outputs) * bytes_of(d.type), stream));
+    return;
+  }
+  if (is_small(d)) {
+    if (d.dx || d.dweight || d.dbias)
+      small_backward(d, static_cast<float *>(workspace), stream);
     return;
   }
   const BackwardLayout l(d);

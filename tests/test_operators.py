@@ -214,6 +214,26 @@ def test_dense_few_rows_and_few_outputs(op, rows, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(600, 203, 301), (300, 1003, 130), (130, 65, 1005), (400, 259, 63), (70, 4001, 9),
+                                   (500, 63, 64), (500, 64, 63), (3000, 255, 15), (100003, 3, 5), (65, 1, 1), (64, 31, 1),
+                                   (9, 400, 9), (1001, 11, 370)], ids=lambda s: "x".join(map(str, s)))
+def test_dense_small_and_odd(op, shape, dtype):
+    """Both sides of the limits under which operands of any alignment are read as they are, with
+    rows further apart than they are long, and each gradient alone."""
+    M, K, N = shape
+    dt = dtype_of(dtype)
+    x, w = normal(1, M, K + 3, dtype=dt)[:, 1:K + 1], normal(2, N, K + 2, dtype=dt, scale=K ** -0.5)[:, :K]
+    b, r = normal(3, N, dtype=dt), normal(4, M, N + 5, dtype=dt)[:, 2:N + 2]
+    z = normal(5, M, N + 1, dtype=dt)[:, :N]
+    check_dense(op, x, w, b, "silu", r, True)
+    check_dense(op, x, w, None, None, None, False)
+    for need in ((True, True, True), (True, False, False), (False, True, False), (False, False, True)):
+        check_dense_backward(op, r, x, w, "gelu", z, need)
+    check_dense_backward(op, r, x, w, None, None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_dense_larger(op, dtype):
     """Several tiles per SM with every part of the epilogue; a wide layer of few rows; a long sum."""
     dt = dtype_of(dtype)
@@ -765,7 +785,7 @@ def call_dense(lib, type=0, rows=4, inputs=8, outputs=16, x=0x10000, ldx=8, w=0x
     return code, lib.mace_last_error().decode()
 
 
-def call_dense_backward(lib, type=0, rows=4, inputs=8, outputs=16, dy=0x10000, lddy=16, x=0x20000, ldx=8, w=0x30000,
+def call_dense_backward(lib, type=0, rows=100, inputs=8, outputs=16, dy=0x10000, lddy=16, x=0x20000, ldx=8, w=0x30000,
                         ldw=8, act=0, z=None, ldz=0, dx=0x40000, lddx=8, dw=0x50000, lddw=8, db=0x60000, ws=0x1000000,
                         size=1 << 24):
     code = lib.mace_dense_backward(type, rows, inputs, outputs, dy, lddy, x, ldx, w, ldw, act, z, ldz, dx, lddx, dw,
