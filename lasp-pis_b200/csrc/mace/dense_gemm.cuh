@@ -272,12 +272,13 @@ __device__ __forceinline__ void finish_row(const Epilogue &e, float *part, long 
 }
 
 // A warp's 32 x 32 block where rows allow no boxes: through its box (columns permuted by row), so that
-// neighbouring lanes write neighbouring columns, 8 rows' residuals in flight at once.  partial !=
-// NULL: the float values go to partial[row * J + col] instead.
+// neighbouring lanes write neighbouring columns, with several rows' residuals in flight (as registers
+// allow).  bias: it is added here.  partial != NULL: the float values go to partial[row * J + col] instead.
 template <class T>
 __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, long long I, long long J,
-                                             long long row0, long long col0, const float *v, const T *bias, unsigned char *box) {
+                                             long long row0, long long col0, const float *v, bool bias, unsigned char *box) {
   constexpr bool Fast = sizeof(T) == 2;
+  constexpr int kRows = Fast ? 16 : 8; // at once
   const int lane = threadIdx.x & 31, rows = int(min(32ll, I - row0));
   float *stage = reinterpret_cast<float *>(box);
   __syncwarp();
@@ -287,33 +288,33 @@ __device__ __forceinline__ void finish_block(const Epilogue &e, float *partial, 
   __syncwarp();
   const long long col = col0 + lane;
   if (col < J) {
-    const float add = bias ? to_float(bias[lane]) : 0.f;
+    const float add = bias ? to_float(static_cast<const T *>(e.bias)[col]) : 0.f;
 #pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += 8) {
-      float x[8];
-      T res[8];
+    for (int r0 = 0; r0 < rows; r0 += kRows) {
+      float x[kRows];
+      T res[kRows];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kRows; ++i)
         if (!partial && e.residual && r0 + i < rows)
           res[i] = static_cast<const T *>(e.residual)[(row0 + r0 + i) * e.ldr + col];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kRows; ++i)
         x[i] = stage[(r0 + i) * 32 + (lane ^ (r0 + i))] + add;
       if (partial) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kRows; ++i)
           if (r0 + i < rows)
             partial[(row0 + r0 + i) * J + col] = x[i];
         continue;
       }
       if (e.z)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kRows; ++i)
           if (r0 + i < rows)
             static_cast<T *>(e.z)[(row0 + r0 + i) * e.ldz + col] = from_float<T>(x[i]);
       activate_all<Fast>(x, e.activation);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kRows; ++i)
         if (r0 + i < rows)
           static_cast<T *>(e.out)[(row0 + r0 + i) * e.ldo + col] = from_float<T>(e.residual ? x[i] + to_float(res[i]) : x[i]);
     }

@@ -234,8 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm16_kernel(const __grid_consta
           for (int c = first; c < end && j * BN + c < g.J; c += 32) {
             float v[32];
             get(c, v);
-            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, g.e.bias && !partial ? bias + c - (BN >= 128 ? first : 0) : nullptr,
-                           w.at);
+            finish_block<T>(g.e, partial, g.I, g.J, row0, j * BN + c, v, g.e.bias && !partial, w.at);
           }
         }
       }

@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
                   v[c] = acc[c0 + c];
               });
         else
-          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, nullptr, boxes[0].at);
+          finish_block<float>(g.e, partial, g.I, g.J, row0, col0, acc + c0, false, boxes[0].at);
       }
     }
     if (lane == 0)
