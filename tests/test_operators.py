@@ -216,7 +216,7 @@ def test_dense_few_rows_and_few_outputs(op, rows, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(600, 203, 301), (300, 1003, 130), (130, 65, 1005), (400, 259, 63), (70, 4001, 9),
                                    (500, 63, 64), (500, 64, 63), (3000, 255, 15), (100003, 3, 5), (65, 1, 1), (64, 31, 1),
-                                   (9, 400, 9), (1001, 11, 370)], ids=lambda s: "x".join(map(str, s)))
+                                   (9, 400, 9), (1001, 11, 370), (18, 534, 94), (11, 3001, 96), (2, 9000, 230), (700, 90, 130)], ids=lambda s: "x".join(map(str, s)))
 def test_dense_small_and_odd(op, shape, dtype):
     """Both sides of the limits under which operands of any alignment are read as they are, with
     rows further apart than they are long, and each gradient alone."""
