@@ -49,9 +49,11 @@ template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2;
 template <int BN> constexpr int stages() { return BN == 64 ? 3 : 2; }
 template <int BN> constexpr int buffers() { return BN == 64 ? 4 : 3; }
 static_assert(buffers<64>() * 64 + stages<64>() * 64 <= 512 && buffers<128>() * 128 + stages<128>() * 64 <= 512, "TMEM");
-// The split of slab g runs after the MMAs of g - stages, which waited for the drain of the slab
-// `buffers` before that.
-template <int BN> constexpr int slots() { return buffers<BN>() + stages<BN>(); }
+// Scales of a slab's rows, from its split to its drain.  The split of slab n writes them after the MMAs of
+// n - stages, which wait until every drain warp has read TMEM for n - stages - buffers.  A warp reads
+// the last of that slab's scales after that, but those of the slab before ahead of it: a slot more than
+// buffers + stages.
+template <int BN> constexpr int slots() { return buffers<BN>() + stages<BN>() + 1; }
 template <int BN> constexpr int slot_bytes() { return 4 * BN + kBM; }
 template <int BN> constexpr int smem_bytes() {
   return stages<BN>() * stage_bytes<BN>() + 8 * (BN / 64) * kBoxBytes + 8 * (BN / 2) * 4 + slots<BN>() * slot_bytes<BN>() + 512;

@@ -905,3 +905,38 @@ def test_python_refusals_on_the_gpu(op):
     with pytest.raises(RuntimeError, match="eps"):
         op.layer_norm(x, eps=-1.0)
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- schedules (no GPU needed)
+@pytest.mark.parametrize("width", [64, 128])
+def test_float_product_scales_are_read_before_they_are_written_again(width):
+    """The float product's schedule as a graph of what waits for what: the split of slab n writes the
+    scale slot of slab n - slots, so every drain warp's reads of that slab come before it."""
+    import pathlib
+    import re
+    source = (pathlib.Path(__file__).parent.parent / "lasp-pis_b200/csrc/mace/dense_gemm32.cu").read_text()
+    number = {}
+    for name in ("stages", "buffers", "slots"):
+        body = re.search(rf"constexpr int {name}\(\) {{ return (.*?); }}", source).group(1)
+        body = re.sub(r"BN == 64 \? (\d+) : (\d+)", lambda m: m.group(1 if width == 64 else 2), body)
+        number[name] = eval(re.sub(r"(\w+)<BN>\(\)", lambda m: str(number[m.group(1)]), body))
+    stages, buffers, slots = number["stages"], number["buffers"], number["slots"]
+    warps, slabs = 8, 40
+    after = {}  # event -> events it comes after
+    for n in range(slabs):
+        # Loads of slab n are started by one drain warp, in turn, that has seen the MMAs of n - stages.
+        after["fetch", n] = [("seen", n - stages, (n - stages) & 7)] if n >= stages else []
+        after["split", n] = [("fetch", n)]  # writes the scales
+        after["mma", n] = [("split", n)] + [("freed", n - buffers, w) for w in range(warps) if n >= buffers]
+        for w in range(warps):
+            after["seen", n, w] = [("mma", n)] + [("read", n - 1, w)] * (n > 0)
+            after["freed", n, w] = [("seen", n, w)]  # TMEM is read, the scales may not be
+            after["read", n, w] = [("freed", n, w)]
+    for n in range(slots, slabs):
+        before, todo = set(), [("split", n)]
+        while todo:
+            for e in after[todo.pop()]:
+                if e not in before:
+                    before.add(e)
+                    todo.append(e)
+        assert all(("read", n - slots, w) in before for w in range(warps)), n
