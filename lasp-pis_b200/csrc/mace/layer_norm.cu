@@ -732,7 +732,8 @@ __global__ void __launch_bounds__(Block ? 1024 : 256)
           const float dz = element(r * width + c, c, st.x, st.y, xh);
           sum_gamma[k] = fmaf(dz, xh, sum_gamma[k]);
           sum_beta[k] += dz;
-          out[r * width + c] = from_float<T>(st.y * (dz * gm - fmaf(xh, st.w, st.z)));
+          if (a.dx) // (else nothing may write here: the next span's copies are not ordered after such writes)
+            out[r * width + c] = from_float<T>(st.y * (dz * gm - fmaf(xh, st.w, st.z)));
         }
       }
     }

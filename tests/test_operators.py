@@ -532,6 +532,28 @@ def test_layer_norm_many_rows_and_strides(op, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(40001, 131, 131), (3001, 333, 333), (701, 2053, 2053), (1201, 333, 340),
+                                   (5, 16395, 16395), (3, 40000, 40000), (301, 1024, 1024)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_layer_norm_gradients_left_out(op, shape, dtype):
+    """Each way to leave gradients out, on rows that form spans (several rows, several spans a block; a row
+    a span), on rows too wide for registers and on aligned ones: what is asked for does not change."""
+    import torch
+    dt = dtype_of(dtype)
+    M, n, ld = shape
+    x, dy = normal(1, M, ld, dtype=dt)[:, :n], normal(2, M, ld, dtype=dt)[:, :n]
+    gamma, beta = normal(3, n, dtype=dt), normal(4, n, dtype=dt)
+    mean, rstd = check_norm(op, x, gamma, beta, 1e-5, "silu")
+    check_norm_backward(op, dy, x, mean, rstd, gamma, beta, "silu")
+    full = op.layer_norm_backward(dy, x, mean, rstd, gamma, beta, "silu")
+    for need in ((False, True, True), (False, True, False), (False, False, True), (True, False, False), (True, True, False)):
+        got = op.layer_norm_backward(dy, x, mean, rstd, gamma, beta, "silu", need)
+        for wanted, a, b in zip(need, got, full):
+            assert torch.equal(a, b) if wanted else a is None
+
+
+@gpu
 def test_layer_norm_far_from_zero(op):
     """Rows of mean 1e4 and standard deviation 1: the variance is taken about the row's own mean."""
     import torch
