@@ -10,8 +10,8 @@
 // warp, or a block for wide rows) between its statistics and its result.  HBM bounds it, so what
 // counts is bytes in flight: a warp holds rows of up to 8 KiB, and where a thread's share of a row is
 // small it takes several rows at once, and loads the next ones before the arithmetic of these.  The
-// variance is taken about a first mean and, for floats, corrected for that mean's own rounding, so a
-// row far from zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
+// variance is taken about a first mean and corrected for that mean's own rounding, so a row far from
+// zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
 // parameters' gradients stay in registers too; each block writes one partial row of dgamma and
 // dbeta, and a second launch adds the partial rows in a fixed order.
 //
@@ -20,6 +20,7 @@
 #include "operators.cuh"
 #include "tcgen05.cuh"
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace mace {
@@ -150,6 +151,54 @@ template <int N> __device__ __forceinline__ void fma_all(float *z, const float *
   }
 }
 
+// A row may lie far from zero against its spread, or have none.  The values centred about a first mean have
+// a mean of their own, `fix`, that mean's rounding error; s is the sum of the centred values and that of
+// their squares.  Where fix is not small against the spread (a few steps of the type at most, then),
+// the difference below loses the variance, and the row is centred once more; so where the squares overflow.
+__device__ __forceinline__ float variance(float2 s, float inv_n) {
+  const float fix = s.x * inv_n, w = fmaf(-fix, fix, s.y * inv_n);
+  return w < 0.f ? 0.f : w; // (NaN stays)
+}
+__device__ __forceinline__ bool recentre(float fix, float var) { return !(4.f * fix * fix <= var && var <= FLT_MAX); }
+// Such a row of floats, from memory: its group centres it twice more and writes its result (mine: whether
+// this group's row is one).
+template <bool Warp>
+__device__ __noinline__ void centre_again(const Norm &a, long long row, bool mine, float mean, int G, int t,
+                                          float2 (*shared0)[32], float2 (*shared1)[32]) {
+  const float inv_n = 1.f / float(a.width);
+  mine = mine && row < a.rows;
+  const float *x = static_cast<const float *>(a.x) + (mine ? row : 0) * a.ldx;
+  float fix = 0.f;
+  float2 s[1];
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    s[0] = make_float2(0.f, 0.f);
+    for (long long i = t; mine && i < a.width; i += G) {
+      const float d = x[i] - mean - fix;
+      s[0].x += d;
+      s[0].y = fmaf(d, d, s[0].y);
+    }
+    __syncwarp();
+    group_sum<Warp, 1>(s, G, k ? shared1 : shared0);
+    fix += s[0].x * inv_n;
+  }
+  const float r = 1.f / sqrtf(variance(s[0], inv_n) + a.eps);
+  if (!mine)
+    return;
+  if (a.mean && !t) {
+    a.mean[row] = mean + fix;
+    a.rstd[row] = r;
+  }
+  for (long long i = t; i < a.width; i += G) {
+    float z = (x[i] - mean - fix) * r;
+    if (a.gamma)
+      z *= static_cast<const float *>(a.gamma)[i];
+    if (a.beta)
+      z += static_cast<const float *>(a.beta)[i];
+    static_cast<float *>(a.y)[row * a.ldy + i] = activate<false>(z, a.activation);
+  }
+}
+
 // T elements in units of U, C units per thread (columns (c G + t) U ...), a row per group of G threads
 // -- G lanes of a warp (Threads = kWarpBlock), or a block of at most Threads -- and R rows per group
 // at once.  Instructions come next after bytes: at 6.5 TB/s an SM has 22 issue slots for each 16-bit
@@ -160,7 +209,7 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
   constexpr bool Fast = sizeof(T) == 2, Ahead = C * R <= 4, Warp = Threads == kWarpBlock,
                  Shared = Warp && C >= kSharedChunks;
   using Un = Unit<T, U>;
-  __shared__ float2 shared[2][R][32];
+  __shared__ float2 shared[Fast ? 2 : 4][R][32];
   extern __shared__ __align__(16) unsigned char parameters[]; // [2][32 C] units (Shared)
   Un *const common = reinterpret_cast<Un *>(parameters);
   const int G = Warp ? lanes : blockDim.x, t = Warp ? threadIdx.x & (G - 1) : threadIdx.x;
@@ -185,12 +234,19 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
       own[1][c] = parameter_unit<T, U>(a.beta, col(c), width, 0.f);
     }
   }
+  float count = 0.f; // of this thread's elements of a row
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    count += Fast && col(c) < width ? float(U) : 0.f;
   Un next[R][C];
+  T next_first[R];
   auto load = [&](long long from) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = from + r * per_block + group;
       const T *p = x + min(row, a.rows - 1) * a.ldx;
+      if (Fast)
+        next_first[r] = *p;
 #pragma unroll
       for (int c = 0; c < C; ++c)
         next[r][c] = load_unit<T, U>(p, col(c) < width, min(col(c), width - U));
@@ -201,22 +257,28 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
   for (; base < a.rows; base += step) {
     if (!Ahead)
       load(base);
-    float v[R][C * U];
+    float v[R][C * U], pivot[R];
     float2 s[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         unpack<T, U>(next[r][c], v[r] + c * U);
-      s[r] = make_float2(sum_of<C * U>(v[r]), 0.f);
+      pivot[r] = Fast ? to_float(next_first[r]) : 0.f;
+      const float sum = sum_of<C * U>(v[r]);
+      s[r] = make_float2(Fast ? fmaf(-count, pivot[r], sum) : sum, 0.f);
     }
     if (Ahead)
       load(base + step);
     group_sum<Warp, R>(s, G, shared[0]);
-    float mean[R], rs[R];
+    float mean[R], rs[R], rest[R], shift[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      mean[r] = s[r].x * inv_n;
+      // 16-bit values: the sums' distance from the first value's, which is exact where values are near
+      // each other, so that what the mean's rounding leaves is known.
+      const float d = s[r].x * inv_n;
+      mean[r] = Fast ? pivot[r] + d : d;
+      rest[r] = Fast ? (pivot[r] - mean[r]) + d : 0.f;
       scale_shift<C * U>(v[r], 1.f, -mean[r]);
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -224,23 +286,22 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
 #pragma unroll
           for (int u = 0; u < U; ++u)
             v[r][c * U + u] = 0.f;
-      // Floats may lie far from zero against their spread: the centred values' own mean is the first
-      // mean's rounding error.  16-bit values with such a mean are coarser than that error.
       s[r] = make_float2(Fast ? 0.f : sum_of<C * U>(v[r]), dot_of<C * U>(v[r], v[r], 0.f));
     }
     group_sum<Warp, R>(s, G, shared[1]);
+    unsigned again = 0; // rows
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float fix = s[r].x * inv_n;
-      const float w = fmaf(-fix, fix, s[r].y * inv_n), var = w < 0.f ? 0.f : w; // (NaN stays)
+      const float fix = Fast ? rest[r] : s[r].x * inv_n, w = fmaf(-fix, fix, s[r].y * inv_n), var = w < 0.f ? 0.f : w;
+      const bool later = !Fast && recentre(fix, var);
+      again |= unsigned(later) << r;
       rs[r] = Fast ? rsqrtf(var + a.eps) : 1.f / sqrtf(var + a.eps);
       const long long row = base + r * per_block + group;
-      if (a.mean && !t && row < a.rows) {
+      if (a.mean && !t && row < a.rows && !later) {
         a.mean[row] = mean[r] + fix;
         a.rstd[row] = Fast ? 1.f / sqrtf(var + a.eps) : rs[r];
       }
-      if (!Fast)
-        scale_shift<C * U>(v[r], 1.f, -fix);
+      shift[r] = -fix * rs[r]; // (v - fix) rs in one instruction
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -254,13 +315,18 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
 #pragma unroll
         for (int u = 0; u < U; ++u)
           z[u] = v[r][c * U + u];
-        scale_shift<U>(z, rs[r], 0.f);
+        scale_shift<U>(z, rs[r], shift[r]);
         fma_all<U>(z, gamma, beta);
         activate_all<Fast>(z, a.activation);
-        if (row < a.rows && col(c) < width)
+        if (row < a.rows && col(c) < width && !(again >> r & 1))
           *reinterpret_cast<Un *>(y + row * a.ldy + col(c)) = pack<T, U>(z);
       }
     }
+    if constexpr (!Fast)
+      if (Warp ? __any_sync(0xffffffffu, again) : again)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          centre_again<Warp>(a, base + r * per_block + group, again >> r & 1, mean[r], G, t, shared[2], shared[3]);
   }
 }
 
@@ -427,7 +493,7 @@ __global__ void __launch_bounds__(Threads)
 constexpr int kWideThreads = 1024;
 template <class T> __global__ void __launch_bounds__(kWideThreads) wide_norm_kernel(const __grid_constant__ Norm a) {
   constexpr bool Fast = sizeof(T) == 2;
-  __shared__ float2 shared[2][1][32];
+  __shared__ float2 shared[3][1][32];
   const float inv_n = 1.f / float(a.width);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(a.x) + row * a.ldx;
@@ -444,8 +510,18 @@ template <class T> __global__ void __launch_bounds__(kWideThreads) wide_norm_ker
       s[0].y = fmaf(d, d, s[0].y);
     }
     group_sum<false, 1>(s, 0, shared[1]);
-    const float fix = s[0].x * inv_n;
-    const float v = fmaf(-fix, fix, s[0].y * inv_n), var = v < 0.f ? 0.f : v;
+    float fix = s[0].x * inv_n, var = variance(s[0], inv_n);
+    if (recentre(fix, var)) { // (the same for all threads)
+      s[0] = make_float2(0.f, 0.f);
+      for (long long i = threadIdx.x; i < a.width; i += kWideThreads) {
+        float d = to_float(x[i]) - m1 - fix;
+        s[0].x += d;
+        s[0].y = fmaf(d, d, s[0].y);
+      }
+      group_sum<false, 1>(s, 0, shared[2]);
+      fix += s[0].x * inv_n;
+      var = variance(s[0], inv_n);
+    }
     const float r = 1.f / sqrtf(var + a.eps);
     if (a.mean && !threadIdx.x) {
       a.mean[row] = m1 + fix;
@@ -612,7 +688,7 @@ __global__ void __launch_bounds__(Block ? 1024 : 256) span_norm_kernel(const __g
   constexpr bool Fast = sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char parameters[];
   __shared__ uint64_t bar;
-  __shared__ float2 shared[2][1][32];
+  __shared__ float2 shared[3][1][32];
   T *gamma = reinterpret_cast<T *>(parameters + span.bytes), *beta = gamma + a.width;
   const int width = int(a.width), warp = threadIdx.x >> 5, t = Team<Block>::first(), stride = Team<Block>::stride();
   const float inv_n = 1.f / float(width);
@@ -643,7 +719,18 @@ __global__ void __launch_bounds__(Block ? 1024 : 256) span_norm_kernel(const __g
         s.y = fmaf(d, d, s.y);
       }
       s = Team<Block>::sum(s, shared[1]);
-      const float fix = s.x * inv_n, v = fmaf(-fix, fix, s.y * inv_n), var = v < 0.f ? 0.f : v;
+      float fix = s.x * inv_n, var = variance(s, inv_n);
+      if (recentre(fix, var)) { // (the same for the whole team)
+        s = make_float2(0.f, 0.f);
+        for (int c = t; c < width; c += stride) {
+          const float d = to_float(row[c]) - m1 - fix;
+          s.x += d;
+          s.y = fmaf(d, d, s.y);
+        }
+        s = Team<Block>::sum(s, shared[2]);
+        fix += s.x * inv_n;
+        var = variance(s, inv_n);
+      }
       // A wait that ran out shows as NaN.
       const float rs = there ? 1.f / sqrtf(var + a.eps) : __uint_as_float(0x7fc00000u);
       if (a.mean && !t) {

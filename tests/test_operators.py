@@ -564,6 +564,26 @@ def test_layer_norm_far_from_zero(op):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [8, 56, 127, 504, 896, 1000, 3584, 7160, 16392])
+def test_layer_norm_rows_with_little_spread(op, n, dtype):
+    """Constant rows far from zero, and rows of which one element is a step away: where rows start, and
+    with them the kernel, makes no difference."""
+    import torch
+    dt = dtype_of(dtype)
+    values = [0.1, -1536.0, 7168.0, 30000.0, 49152.0] + [2031616.0] * (dt != torch.float16)
+    x = torch.tensor(values + values, device="cuda").to(dt)[:, None].repeat(1, n)
+    for k in range(len(values)):
+        x[k, n // 3] = torch.nextafter(x[k, 0], torch.tensor(math.inf, dtype=dt, device="cuda"))
+    gamma, beta = normal(1, n, dtype=dt, scale=0.2, shift=1.0), normal(2, n, dtype=dt)
+    anywhere = torch.empty(x.shape[0], n + 1, dtype=dt, device="cuda")[:, 1:]
+    for rows in (x, anywhere.copy_(x)):
+        mean, rstd = check_norm(op, rows, None, None, 1e-5, None)
+        assert torch.equal(mean[len(values):], x[len(values):, 0].float())
+        check_norm(op, rows, gamma, beta, 1e-5, "silu")
+
+
+@gpu
 @pytest.mark.parametrize("n", [64, 2053, 40000])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layer_norm_special_rows(op, dtype, n):
