@@ -50,7 +50,8 @@ MACE_EXPORT long long mace_dense_workspace(int type, long long rows, long long i
  * column sums of dz; each of dx, dweight and dbias may be NULL and is then not computed (x is
  * read for dweight only, weight for dx only).  z may be NULL where activation is none.  The
  * residual's gradient is dy.  With rows = 0, dweight and dbias are zero.  In 16-bit types, dz is
- * rounded to the type before the products, as a tensor between two layers would be. */
+ * rounded to the type before the products of layers that run on the tensor cores, as a tensor
+ * between two layers would be; dbias sums the float values. */
 MACE_EXPORT int mace_dense_backward(int type, long long rows, long long inputs, long long outputs, const void *dy,
                                     long long lddy, const void *x, long long ldx, const void *weight,
                                     long long ldw, int activation, const void *z, long long ldz, void *dx,

@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(256)
 
 // ---------------- small gradients ----------------
 // All gradients of a layer with few weights, any alignment, float arithmetic: a block takes kSmallRows rows
-// or fewer (as shared memory allows) at a time, forms their dz (rounded to the type) beside x and W in
+// or fewer (as shared memory allows) at a time, forms their dz (in float, not rounded) beside x and W in
 // shared memory, writes their dx, and adds to dW and db -- x has one more column of ones for db -- in
 // registers.  Many rows: each block writes a partial [outputs][inputs + 1], which a second launch adds.
 // Launches are what bound such calls, one or two here and 4 to 8 with the tensor cores (f32 with SiLU,
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(256)
       float v = to_float(static_cast<const T *>(a.dy)[(r0 + r) * a.lddy + o]);
       if (a.activation != None)
         v *= slope<Fast>(to_float(static_cast<const T *>(a.z)[(r0 + r) * a.ldz + o]), a.activation);
-      dz[e] = to_float(from_float<T>(v)); // (in 16 bits, as for the larger products)
+      dz[e] = v;
     }
     __syncthreads();
     if (a.dx)

@@ -175,6 +175,27 @@ def test_dense_backward_many_rows(op, dtype):
         check_dense_backward(op, dy, x, w, "silu", z, need)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(12, 9, 7), (3001, 63, 64), (20011, 24, 40), (3000, 200, 136)], ids=lambda s: "x".join(map(str, s)))
+def test_dense_bias_gradient_sums_floats(op, shape, dtype):
+    """dbias is a sum of floats, rounded once, whatever the layer's size: values of dz that the type rounds
+    to nothing count, and none is rounded on its way (no u |dz| in the bound)."""
+    M, K, N = shape
+    dt = dtype_of(dtype)
+    x, w = normal(1, M, K, dtype=dt), normal(2, N, K, dtype=dt)
+    z = normal(4, M, N, dtype=dt)
+    for dy in (normal(3, M, N, dtype=dt, scale=0.1, shift=1.0), normal(3, M, N, dtype=dt, scale=0.0, shift=2.0 ** -24)):
+        for act, zs in (("silu", z), ("silu", z - 5), ("gelu", z)):
+            _, _, db = op.dense_backward(dy, x, w, act, zs)
+            d64 = dy.double()
+            g64 = d64 * slope64(zs.double(), act)
+            want, S = g64.sum(0), g64.abs().sum(0)
+            # Slopes are off by at most 2^-20 of 1.13; fewer than M / 32 + 64 additions in sequence.
+            bound = (1.13 * 2.0 ** -20 * d64.abs()).sum(0) + (M / 32 + 64) * 2.0 ** -24 * S
+            close(db, want, bound + half_step(dt) * (want.abs() + bound) + tiny(dt) / 2, "dbias")
+
+
 def spread(rng, low, high):
     return min(high, max(low, round(math.exp(rng.uniform(math.log(low), math.log(high))))))
 
