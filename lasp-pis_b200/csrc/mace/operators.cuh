@@ -68,11 +68,12 @@ template <class T, int U> __device__ __forceinline__ Unit<T, U> pack(const float
   return u;
 }
 
-// 1 + exp(-z).  16-bit results take the fast exponential (2^-21 of the value and a little more for
-// large |z|, far below their own rounding).  The quotients below take the fast division (2 ulp): the
-// exact one branches for every value.
-template <bool Fast> __device__ __forceinline__ float exp_plus_one(float z) {
-  return 1.f + (Fast ? __expf(-z) : expf(-z));
+// exp(-|z|): SiLU and its slope by quotients over 1 + exp(-|z|), in [1, 2], where nothing overflows and the
+// fast division (2 ulp; the exact one branches for every value) has no range in which it gives 0.  16-bit
+// results take the fast exponential (2^-21 of the value and a little more for large |z|, far below
+// their own rounding).
+template <bool Fast> __device__ __forceinline__ float exp_minus_abs(float z) {
+  return Fast ? __expf(-fabsf(z)) : expf(-fabsf(z));
 }
 // Phi(-m) for m >= 0, as exp(-m^2 / 2) g(m): g, a scaled complementary error function, is a polynomial
 // in t = 1 / (1 + 0.32 m), fitted here for the least relative error (4.4e-7).  e: the exponential.
@@ -91,8 +92,10 @@ __device__ __forceinline__ float normal_tail(float m, float &e) {
   return q * t * e;
 }
 template <bool Fast> __device__ __forceinline__ float activate(float z, int act) {
-  if (act == Silu)
-    return __fdividef(z, exp_plus_one<Fast>(z));
+  if (act == Silu) {
+    const float e = exp_minus_abs<Fast>(z);
+    return __fdividef(z < 0.f ? z * e : z, 1.f + e);
+  }
   if (act == Gelu && Fast) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the tail is 0 from 40 on, NaN stays
     const float m = fmaxf(-z, fminf(z, 40.f)); // |z|; the formula's NaN for -infinity, but not for infinity
     float e;
@@ -123,7 +126,7 @@ template <bool Fast, int N> __device__ __forceinline__ void activate_all(float (
 // d act / dz
 template <bool Fast> __device__ __forceinline__ float slope(float z, int act) {
   if (act == Silu) {
-    float s = __fdividef(1.f, exp_plus_one<Fast>(z));
+    const float e = exp_minus_abs<Fast>(z), s = __fdividef(z < 0.f ? e : 1.f, 1.f + e);
     return s * (1.f + z * (1.f - s));
   }
   if (act == Gelu && Fast) {

@@ -403,6 +403,28 @@ def test_activations_of_special_values(op, dtype, act):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu_far_below_zero(op, dtype):
+    """SiLU and its slope relative to their own size, down to where they leave the type: z enters as the bias
+    of a product of zeros."""
+    import torch
+    dt, u = dtype_of(dtype), half_step(dtype_of(dtype))
+    z = torch.linspace(-104, 20, 2048, device="cuda").to(dt)
+    x, w = torch.zeros(16, 8, dtype=dt, device="cuda"), torch.zeros(2048, 8, dtype=dt, device="cuda")
+    y = op.dense(x, w, z, "silu")
+    _, _, db = op.dense_backward(torch.ones(1, 2048, dtype=dt, device="cuda"), x[:1], w, "silu", z[None])
+    z64 = z.double()
+    # The exponential: 2 ulp in f32, |z| 2^-23 of its value in 16 bits; subnormal, it has steps of 2^-149.
+    # Quotient and products: 6 ulp; the slope's 1 + z (1 - s) cancels near z = -1.28 only, to 2^-22.
+    rel = 2.0 ** -20 + (z64.abs() * 2.0 ** -23 if dt != torch.float32 else 0)
+    low = (z64.abs() + 1) * 2.0 ** -147 + tiny(dt)
+    want = act64(z64, "silu")
+    close(y, want.expand(16, 2048), (rel + u) * want.abs() + low, "silu")
+    want = slope64(z64, "silu")
+    close(db, want, (rel + u) * want.abs() + 2.0 ** -21 * ((z64 + 1.2785).abs() < 0.5) + low, "slope")
+
+
+@gpu
 def test_dense_f32_rows_of_any_magnitude(op):
     """Rows from 1e-25 to 1e25, and weights whose rows differ as much: the error stays relative to
     each row's own products."""
