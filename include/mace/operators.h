@@ -35,7 +35,7 @@ enum { MACE_ACT_NONE = 0, MACE_ACT_SILU = 1, MACE_ACT_GELU = 2, MACE_ACT_RELU = 
  * residual may be y itself (same address and ld).
  * float products run on the tensor cores as split fp16 pairs (but for up to 8 rows or outputs, or
  * few inputs: plain float arithmetic): per row and 64 consecutive inputs the largest magnitude sets
- * the scale, values down to 2^-18 of it keep 22 bits, and smaller ones are held to 2^-40 of it.
+ * the scale, values down to 2^-29 of it keep 22 bits, and smaller ones are held to 2^-52 of it.
  * Infinities and NaN give what the sum gives (such results are summed again, which is slow where
  * there are many). */
 MACE_EXPORT int mace_dense(int type, long long rows, long long inputs, long long outputs, const void *x,

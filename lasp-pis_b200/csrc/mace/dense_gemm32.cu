@@ -1,16 +1,18 @@
-// The dense layer's matrix products of floats on the tensor cores (tcgen05, kind::f16), with the
-// error of float arithmetic.
+// The dense layer's matrix products of floats on the tensor cores (tcgen05, kind::f16), with an error
+// like that of float arithmetic.
 //
 //   out(i, j) = sum_k P(i, k) Q(j, k)
 //
 // Both operands are split on the way to the tensor cores: per row and 64-wide slab of k, with 2^e the
-// power of two that brings the largest magnitude into [2^14, 2^15), v 2^e = hi + lo, both fp16
-// rounded to nearest (22 significant bits for values down to 2^-18 of the largest).  A slab's
-// products lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22) accumulate fresh in TMEM, are scaled back
-// by the two exact powers of two and added to float registers: the tensor pipe truncates, which
-// must not add up over long k.  A slab's result comes out 8.7e-8 too small in the mean (tc_gemm.cu),
-// so three slabs of four are scaled by 1 + 2^-23: 8.9e-8.  2-norm errors against 64 bits: 0.8e-7 to
-// 2.2e-7, where float sums in order have 1.4e-7 to 1.4e-6.
+// power of two that brings the largest magnitude into [2^14, 2^15), v 2^e = hi + 2^-12 lo, both fp16
+// rounded to nearest.  Scaled so, lo is as large as hi, and values down to 2^-29 of the largest keep 22
+// bits (2^-23 of themselves), smaller ones 2^-52 of the largest.  A slab's products lo*hi + hi*lo
+// accumulate fresh in TMEM, the first product of hi*hi scales them by 2^-12 (lo*lo is below 2^-22), and
+// the sum is scaled back by the two exact powers of two and added to float registers: the tensor pipe
+// truncates, which must not add up over long k.  A slab's result comes out too small by that, 9e-8 in the
+// mean for values of both signs, 2e-7 for values of one; no factor makes up for it, since sums that are
+// exact in floats (small integers, one product) come out exact.  2-norm errors against 64 bits: 1.3e-7
+// to 2.1e-7, where float sums in order have 1.2e-7 to 1.6e-6.
 //
 // TMA brings the slab's floats into shared memory, whichever index is contiguous; the split reads a row
 // per thread.  P's rows go to TMEM, the first operand's other place; Q's over their floats, k-major
@@ -43,6 +45,7 @@ namespace {
 using namespace tc;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kThreads = 512, kDrainThreads = 256;
+constexpr int kLoBits = 12; // lo halves hold (v 2^e - hi) 2^12: up to 2^15, as hi
 template <int BN> constexpr int stage_bytes() { return 2 * (kBM + BN) * kBK * 2; }
 // 64-wide tiles: three stages, and a box of results per drain warp; 128-wide ones: two and two.  TMEM
 // holds P's split slabs, 64 columns for each stage, and as many accumulators as then fit.
@@ -82,11 +85,13 @@ __device__ __forceinline__ int split_power(uint32_t bits) {
   return min(max(e, -126), 126);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
-// Two neighbouring values: hi and lo halves (the remainder v 2^e - hi is exact).
+// Two neighbouring values: hi and lo halves (the remainder v 2^e - hi is exact; its half is scaled by 2^kLoBits).
 __device__ __forceinline__ void split2(float2 v, float2 scale, uint32_t &hi, uint32_t &lo) {
+  constexpr float kUp = float(1 << kLoBits);
   const float2 x = __fmul2_rn(v, scale);
   const __half2 h = __float22half2_rn(x);
-  const __half2 l = __float22half2_rn(__ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x));
+  const float2 rest = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x);
+  const __half2 l = __float22half2_rn(__fmul2_rn(rest, make_float2(kUp, kUp)));
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }
@@ -253,12 +258,19 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
-// D (TMEM) (+)= A (TMEM) B (shared memory).
-template <bool Add> __device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
-  asm volatile("{\n\t.reg .pred p;\n\t"
-               "setp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-               "r"(a), "l"(b), "r"(idesc), "n"(int(Add)));
+// D (TMEM) = A (TMEM) B (shared memory) + 2^-Down D, D's old value where Add.
+template <bool Add, int Down = 0>
+__device__ __forceinline__ void umma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  if constexpr (Down == 0)
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "n"(int(Add)));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %5;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "n"(int(Add)), "n"(Down));
 }
 
 // sum_k P(i, k) Q(j, k) for k in [k0, k1) by a whole warp, one product at a time, 8 per lane under way;
@@ -359,8 +371,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
       umma_f16_tmem<true>(d, pl + 8 * m, qh + 2 * m, idesc);
       umma_f16_tmem<true>(d, ph + 8 * m, ql + 2 * m, idesc);
     }
+    umma_f16_tmem<true, kLoBits>(d, ph, qh, idesc); // scales them back
 #pragma unroll
-    for (int m = 0; m < kBK / 16; ++m)
+    for (int m = 1; m < kBK / 16; ++m)
       umma_f16_tmem<true>(d, ph + 8 * m, qh + 2 * m, idesc);
     umma_commit(tfull0 + 8 * b);
   };
@@ -533,8 +546,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm32_kernel(const __grid_consta
         tc_fence_after();
         const unsigned char *scale = scales + n % kSlots * kSlotBytes;
         const float *fq = reinterpret_cast<const float *>(scale) + half * kCols;
-        // 2^-e of P's row, one ulp more in three slabs of four.
-        const float fp = __uint_as_float((uint32_t(scale[4 * BN + 32 * quarter + lane]) << 23) + ((w.k & 3) != 3));
+        // 2^-e of P's row.
+        const float fp = __uint_as_float(uint32_t(scale[4 * BN + 32 * quarter + lane]) << 23);
         const float2 fp2 = make_float2(fp, fp);
 #pragma unroll
         for (int h = 0; h < kCols; h += 32) {

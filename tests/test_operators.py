@@ -439,6 +439,44 @@ def test_dense_f32_rows_of_any_magnitude(op):
                          need=(False, True, True))
 
 
+@gpu
+@pytest.mark.parametrize("big", [1e3, 1e6, 1e8])
+def test_dense_f32_values_beside_much_larger_ones(op, big):
+    """A large value that meets a weight of zero: the others' products keep their bits, in the result and in
+    both gradients (the bounds are relative to the products that are there)."""
+    M, K, N = 300, 256, 200
+    f32 = dtype_of("f32")
+    x, w, dy = normal(1, M, K, dtype=f32), normal(2, N, K, dtype=f32), normal(3, M, N, dtype=f32)
+    x[:, 70], w[:, 70] = big, 0.0
+    check_dense(op, x, w, None, None, None, False)
+    x, w = normal(1, M, K, dtype=f32), normal(2, N, K, dtype=f32)
+    w[:, 30], x[:, 30] = big, 0.0
+    check_dense(op, x, w, None, None, None, False)
+    dy[:, 11], w[11], w[:, 30] = big, 0.0, 1.0
+    check_dense_backward(op, dy, x, w, None, None, need=(True, False, False))
+    dy[:, 11] = 1.0
+    dy[40], x[40] = big, 0.0
+    check_dense_backward(op, dy, x, w, None, None, need=(False, True, False))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(300, 64, 70), (300, 512, 200), (5000, 200, 40)], ids=lambda s: "x".join(map(str, s)))
+def test_dense_f32_exact_sums_are_exact(op, shape):
+    """Small integers: every partial sum is exact in floats, and so is the result.  A weight of ones on the
+    diagonal returns x to the bits that the operands keep."""
+    import torch
+    M, K, N = shape
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w, dy = (torch.randint(-8, 9, s, device="cuda", generator=g).float() for s in ((M, K), (N, K), (M, N)))
+    assert torch.equal(op.dense(x, w).double(), x.double() @ w.double().t())
+    dx, dw, db = op.dense_backward(dy, x, w)
+    assert torch.equal(dx.double(), dy.double() @ w.double()) and torch.equal(dw.double(), dy.double().t() @ x.double())
+    assert torch.equal(db.double(), dy.double().sum(0))
+    x = normal(2, M, K, dtype=torch.float32)
+    y = op.dense(x, torch.eye(K, device="cuda"))
+    assert ((y - x).abs() <= 2.0 ** -23 * x.abs()).all()
+
+
 # ---------------------------------------------------------------- layer norm
 def check_norm(op, x, gamma, beta, eps, act):
     import torch
