@@ -918,6 +918,7 @@ template <auto Kernel> int resident_blocks(int threads, int shared = 0) {
 // Upper bound of a backward pass's partial rows (its grid): 148 SMs hold at most 8 blocks of 256
 // threads each; other devices may hold more blocks, the grid is cut at this number.
 constexpr int kMostParts = 1184;
+constexpr int kSpanColumns = 12; // of a thread, backward
 int wide_parts(long long rows) { return int(std::min<long long>(rows, 32)); }
 // Whether spans are used, for rows that allow no wide loads: from 128 elements on, as far as their
 // place (and gamma and beta) fits in shared memory.  Rows that lie without gaps form spans of up to 64
@@ -934,7 +935,7 @@ bool span_of(int type, long long rows, long long width, bool contiguous, int arr
   const long long place = (s.rows * row + 31) / 16 * 16, all = place * arrays + 2 * row;
   s.bytes = int(std::min(place, 1ll << 30));
   shared = int(std::min(all, 1ll << 30));
-  return all <= 216 * 1024 && (arrays == 1 || width <= 12 * (block ? 1024 : 256));
+  return all <= 216 * 1024 && (arrays == 1 || width <= kSpanColumns * (block ? 1024 : 256));
 }
 template <auto Kernel> int span_blocks(int shared, int threads) {
   static thread_local int device = -1;
@@ -987,9 +988,11 @@ void layer_norm(const Norm &a, cudaStream_t stream) {
   });
 }
 
-long long layer_norm_backward_workspace(int, long long rows, long long width) {
-  // Partial rows: never more than one per row of x, nor than a grid's blocks.
-  return std::min<long long>(rows, kMostParts) * 2 * width * 4;
+long long layer_norm_backward_workspace(int type, long long rows, long long width) {
+  // Partial rows: never more than one per row of x, nor than a grid's blocks.  Rows longer than registers
+  // (2048 units) and spans (12 columns a thread) hold, whatever their alignment, have few.
+  const bool wide = width > std::max(2048 * (16 / bytes_of(type)), kSpanColumns * 1024);
+  return (wide ? wide_parts(rows) : std::min<long long>(rows, kMostParts)) * 2 * width * 4;
 }
 
 void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t stream) {
@@ -1022,9 +1025,9 @@ void layer_norm_backward(const NormBackward &a, void *workspace, cudaStream_t st
         using std::integral_constant;
         const bool narrow = a.width <= 4 * (block ? 512 : 256);
         if (block)
-          narrow ? go(integral_constant<int, 4>{}, std::true_type{}) : go(integral_constant<int, 12>{}, std::true_type{});
+          narrow ? go(integral_constant<int, 4>{}, std::true_type{}) : go(integral_constant<int, kSpanColumns>{}, std::true_type{});
         else
-          narrow ? go(integral_constant<int, 4>{}, std::false_type{}) : go(integral_constant<int, 12>{}, std::false_type{});
+          narrow ? go(integral_constant<int, 4>{}, std::false_type{}) : go(integral_constant<int, kSpanColumns>{}, std::false_type{});
       } else if (s.wide) {
         if (a.dx) {
           int grid = int(std::min<long long>(a.rows, resident_blocks<wide_norm_backward_kernel<T>>(kWideThreads)));

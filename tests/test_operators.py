@@ -684,6 +684,17 @@ def test_layer_norm_special_rows(op, dtype, n):
 
 
 @gpu
+@pytest.mark.parametrize("n", [8192, 8196, 12287, 12288, 12289, 16384, 16385, 16392])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_many_wide_rows(op, dtype, n):
+    """Both sides of the lengths at which rows stop being held, with more rows than partial sums."""
+    dt = dtype_of(dtype)
+    x, dy, gamma = normal(1, 200, n, dtype=dt), normal(2, 200, n, dtype=dt), normal(3, n, dtype=dt)
+    mean, rstd = check_norm(op, x, gamma, None, 1e-5, None)
+    check_norm_backward(op, dy, x, mean, rstd, gamma, None, None)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layer_norm_empty(op, dtype):
     import torch
@@ -981,6 +992,15 @@ def test_refusals(op, call, wrong, message):
     lib = op._library()[0]
     code, error = call(lib, **wrong)
     assert code == -1 and message in error, error
+
+
+@pytest.mark.parametrize("type,held", [(0, 12288), (1, 16384), (2, 16384)])
+def test_workspace_of_wide_rows(op, type, held):
+    """Rows longer than any kernel holds at once have at most 32 partial sums of the parameters' gradients."""
+    size = op._library()[0].mace_layer_norm_backward_workspace
+    assert size(type, 2000, held) == 1184 * 2 * held * 4
+    assert size(type, 2000, held + 1) == 32 * 2 * (held + 1) * 4
+    assert size(type, 3, 1 << 20) == 3 * 2 * (1 << 20) * 4
 
 
 def test_no_rows_is_no_work(op):
