@@ -13,13 +13,16 @@ All tensors of a call have one type (float32, bfloat16 or float16) and one devic
 are float32.  A leading tensor is (..., features); tensors whose last index is not contiguous, or
 whose leading indices do not collapse into rows, are copied first.  Work is queued on torch's
 current stream of the tensors' device, and outputs are new contiguous tensors.  The calls record
-no autograd graph: the backward calls give the gradients.  Wrong arguments raise ValueError (or
-TypeError), a failed call RuntimeError.
+no autograd graph: the backward calls give the gradients.  Where autograd is on and an argument of
+a forward call requires a gradient, a UserWarning says so (torch.no_grad() or detach() around such
+calls keeps it away).  Wrong arguments raise ValueError (or TypeError); what the library itself
+refuses (an empty last index, a negative eps) and a failed call raise RuntimeError.
 """
 from __future__ import annotations
 
 import ctypes as ct
 import math
+import warnings
 
 from .native import _error, load
 
@@ -85,6 +88,11 @@ def _like(t, name, torch, shape, dtype, device):
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
     return t
+
+
+def _warn_of_autograd(name):
+    warnings.warn(f"{name} records no autograd graph, and an argument requires a gradient: its result has none "
+                  f"(the gradients come from {name}_backward)", UserWarning, stacklevel=3)
 
 
 def _rows(t):
@@ -159,6 +167,9 @@ def dense(x, weight, bias=None, activation=None, residual=None, keep=False):
     pr, ldr = None, 0
     if residual is not None:
         residual, pr, ldr = _rows(_like(residual, "residual", torch, shape, dtype, device))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        _warn_of_autograd("dense")
     x, px, ldx = _rows(x)
     weight, pw, ldw = _rows(weight)
     y = x.new_empty(shape)
@@ -223,6 +234,9 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, activation=None, keep=False):
         gamma = _flat(_like(gamma, "gamma", torch, (width,), dtype, device))
     if beta is not None:
         beta = _flat(_like(beta, "beta", torch, (width,), dtype, device))
+    if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad)
+                                    or (beta is not None and beta.requires_grad)):
+        _warn_of_autograd("layer_norm")
     x, px, ldx = _rows(x)
     y = _new_like(x, torch) if x.dim() == len(shape) else x.new_empty(shape)
     mean = rstd = None

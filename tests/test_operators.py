@@ -1050,6 +1050,29 @@ def test_python_refusals_on_the_gpu(op):
     torch.cuda.synchronize()
 
 
+@gpu
+def test_results_without_history_are_announced(op):
+    """A forward call on tensors that require gradients, with autograd on, warns; the values are the same, and
+    without autograd, or on detached tensors, and in the backward calls, nothing is said."""
+    import warnings
+
+    import torch
+    x, w = normal(1, 20, 16, dtype=torch.float32), normal(2, 24, 16, dtype=torch.float32)
+    p, g = torch.nn.Parameter(w), torch.nn.Parameter(x[0].clone())
+    for call, plain in ((lambda: op.dense(x, p), lambda: op.dense(x, w)),
+                        (lambda: op.dense(x.clone().requires_grad_(), w), lambda: op.dense(x, w)),
+                        (lambda: op.layer_norm(x, g), lambda: op.layer_norm(x, g.detach()))):
+        with pytest.warns(UserWarning, match="no autograd graph"):
+            y = call()
+        assert not y.requires_grad
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            assert torch.equal(y, plain())
+            with torch.no_grad():
+                assert torch.equal(y, call())
+            op.dense_backward(normal(3, 20, 24, dtype=torch.float32), x, p)
+
+
 # ---------------------------------------------------------------- schedules (no GPU needed)
 @pytest.mark.parametrize("width", [64, 128])
 def test_float_product_scales_are_read_before_they_are_written_again(width):
