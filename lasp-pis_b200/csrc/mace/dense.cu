@@ -277,6 +277,89 @@ void few_rows(const Dense &d, bool turned, cudaStream_t stream) {
   });
 }
 
+// ---------------- up to 16 outputs, many rows that TMA cannot read ----------------
+// Floats, rows of x that start anywhere: copying x for the tensor cores moves it three times, where the
+// call's floor is to read it once.  A block has 64 rows and all outputs; a slab of 32 k comes by single
+// loads (a warp a row: 128 bytes at any offset), on its way in registers while the slab before it is
+// summed from shared memory, 4 rows by 2 outputs a thread, in floats, a slab at a time.  Rows of shared memory
+// are 36 floats apart, so that its 16-byte reads have no bank conflicts; these reads bound it.  With
+// few rows the blocks do not fill the device.  Here, with a copy and the tensor cores, and as a plain
+// product (us): 80000 x 301 -> 16 53, 85, 67; 80000 x 33 -> 16 16, 32, 27; 57901 x 911 -> 10 115, 169, 121;
+// 20000 x 1001 -> 12 64, 85, 66; but 9472 x 1237 -> 16 55 and 45.  With more outputs shared memory is read
+// more often (20000 x 1001 -> 48: 128, and 87 with a copy).  4-byte asynchronous copies: 74 at 1001 -> 12.
+constexpr int kOddOutputs = 16, kOddRows = 64, kOddSlab = 32, kOddPitch = 36, kOddThreads = 128;
+__global__ void __launch_bounds__(kOddThreads, 5) odd_rows_kernel(const __grid_constant__ Dense d) {
+  constexpr int N = kOddOutputs, kWarps = kOddThreads / 32, R = 4, C = 2, kAcross = N / C, kHigh = kOddRows / R;
+  static_assert(kAcross * kHigh == kOddThreads, "a thread has R rows and C outputs");
+  constexpr int kMine = kOddRows / kWarps, kMineW = N / kWarps; // rows of x and W that a warp brings
+  __shared__ __align__(16) float slabs[2][kOddRows + N][kOddPitch];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cx = threadIdx.x % kAcross, ry = threadIdx.x / kAcross;
+  const long long row0 = (long long)blockIdx.x * kOddRows;
+  const float *const x = static_cast<const float *>(d.x), *const w = static_cast<const float *>(d.weight);
+  const long long count = (d.inputs + kOddSlab - 1) / kOddSlab;
+  float next[kMine + kMineW];
+  auto load = [&](long long slab) { // columns and rows past the end: the last ones (as zeros; not written)
+    const long long in = min(slab * kOddSlab + lane, d.inputs - 1);
+#pragma unroll
+    for (int r = 0; r < kMine; ++r)
+      next[r] = x[min(row0 + warp + kWarps * r, d.rows - 1) * d.ldx + in];
+#pragma unroll
+    for (int n = 0; n < kMineW; ++n)
+      next[kMine + n] = w[min((long long)(warp + kWarps * n), d.outputs - 1) * d.ldw + in];
+  };
+  float sum[R][C] = {};
+  load(0);
+  for (long long slab = 0; slab < count; ++slab) {
+    float(*const at)[kOddPitch] = slabs[slab & 1];
+    const bool there = slab * kOddSlab + lane < d.inputs;
+#pragma unroll
+    for (int r = 0; r < kMine + kMineW; ++r)
+      at[r < kMine ? warp + kWarps * r : kOddRows + warp + kWarps * (r - kMine)][lane] = there ? next[r] : 0.f;
+    __syncthreads(); // (who writes this place next has passed the next barrier, and with it all of its readers)
+    load(min(slab + 1, count - 1));
+    const float *const xs = at[ry], *const ws = at[kOddRows + cx];
+    float part[R][C] = {};
+#pragma unroll
+    for (int k = 0; k < kOddSlab; k += 4) {
+      float4 a[R], b[C];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        a[i] = *reinterpret_cast<const float4 *>(xs + i * kHigh * kOddPitch + k);
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        b[j] = *reinterpret_cast<const float4 *>(ws + j * kAcross * kOddPitch + k);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          part[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, part[i][j]))));
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        sum[i][j] += part[i][j];
+  }
+  const Epilogue e{d.bias, d.activation, d.residual, d.ldr, d.y, d.ldy, d.z, d.ldz};
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const long long row = row0 + ry + i * kHigh;
+      const int col = cx + j * kAcross;
+      if (row < d.rows && col < d.outputs)
+        finish<float>(e, row, col, sum[i][j]);
+    }
+}
+bool is_odd(const Dense &d) {
+  return d.type == F32 && d.outputs > kFew && d.outputs <= kOddOutputs && d.inputs > 12 && d.rows >= 128ll * sm_count() &&
+         !tma_ready(d.type, d.x, d.rows, d.ldx);
+}
+void odd(const Dense &d, cudaStream_t stream) {
+  lapis::launch(odd_rows_kernel, dim3(unsigned((d.rows + kOddRows - 1) / kOddRows)), kOddThreads, 0, stream, d);
+  lapis::check(cudaGetLastError());
+}
+
 // ---------------- one pass over dy ----------------
 // A block is `lanes` columns units wide (a power of two up to 32) and 256 / lanes rows high; it walks
 // rows by gridDim.y blocks' heights, writes dz = dy act'(z) (dz NULL: not wanted) and adds its columns:
@@ -605,8 +688,14 @@ struct BackwardLayout {
 };
 } // namespace
 
-long long dense_workspace(const Dense &d) { return is_narrow(d) || is_few(d) || is_few_outputs(d) || is_small(d) ? 0 : ForwardLayout(d).total; }
+long long dense_workspace(const Dense &d) {
+  return is_narrow(d) || is_few(d) || is_few_outputs(d) || is_small(d) || is_odd(d) ? 0 : ForwardLayout(d).total;
+}
 void dense(const Dense &d, void *workspace, cudaStream_t stream) {
+  if (is_odd(d)) {
+    odd(d, stream);
+    return;
+  }
   if (is_narrow(d)) {
     narrow(d, stream);
     return;

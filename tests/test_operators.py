@@ -254,6 +254,30 @@ def test_dense_small_and_odd(op, shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(18943, 255, 16), (18944, 35, 9), (19001, 33, 16), (20001, 130, 17), (20001, 1001, 12),
+                                   (40007, 13, 10), (40007, 12, 10), (30001, 31, 8), (90001, 41, 11), (19072, 98, 15)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_dense_many_odd_rows_and_few_outputs(op, shape):
+    """Rows of floats that start anywhere, on both sides of the limits within which they are read as they
+    are; infinities and NaN stay in their rows."""
+    import torch
+    M, K, N = shape
+    f32 = dtype_of("f32")
+    x, w = normal(1, M, K + 3, dtype=f32)[:, 1:K + 1], normal(2, N, K + 2, dtype=f32, scale=K ** -0.5)[:, :K]
+    b, r = normal(3, N, dtype=f32), normal(4, M, N + 5, dtype=f32)[:, 2:N + 2]
+    check_dense(op, x, w, b, "gelu", r, True)
+    clean, _ = check_dense(op, x.contiguous(), w, None, None, None, False)
+    assert torch.equal(op.dense(x, w), clean)
+    bad = x.contiguous()
+    bad[5, K - 1], bad[M - 1, 0], bad[70, 3] = math.inf, math.nan, -math.inf
+    y = op.dense(bad, w)
+    same = torch.ones(M, dtype=torch.bool, device="cuda")
+    same[[5, 70, M - 1]] = False
+    assert torch.equal(y[same], clean[same]) and y[M - 1].isnan().all()
+    assert torch.equal(y[5].sign(), w[:, K - 1].sign()) and y[[5, 70]].isinf().all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_dense_larger(op, dtype):
     """Several tiles per SM with every part of the epilogue; a wide layer of few rows; a long sum."""
