@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
         unpack<T, U>(next[r][c], v[r] + c * U);
       pivot[r] = Fast ? to_float(next_first[r]) : 0.f;
       const float sum = sum_of<C * U>(v[r]);
-      s[r] = make_float2(Fast ? fmaf(-count, pivot[r], sum) : sum, 0.f);
+      s[r] = Fast ? make_float2(fmaf(-count, pivot[r], sum), sum) : make_float2(sum, 0.f);
     }
     if (Ahead)
       load(base + step);
@@ -274,11 +274,13 @@ __global__ void __launch_bounds__(Threads) layer_norm_kernel(const __grid_consta
     float mean[R], rs[R], rest[R], shift[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      // 16-bit values: the sums' distance from the first value's, which is exact where values are near
-      // each other, so that what the mean's rounding leaves is known.
+      // 16-bit values: the sums' distance from the first value's is exact where values are near each other,
+      // so that what the mean's rounding leaves is known.  Where that distance is the larger sum (the
+      // first value lies far from the rest), the plain sum has the smaller error.
       const float d = s[r].x * inv_n;
-      mean[r] = Fast ? pivot[r] + d : d;
-      rest[r] = Fast ? (pivot[r] - mean[r]) + d : 0.f;
+      const bool near = Fast && fabsf(s[r].x) <= fabsf(s[r].y);
+      mean[r] = near ? pivot[r] + d : Fast ? s[r].y * inv_n : d;
+      rest[r] = near ? (pivot[r] - mean[r]) + d : 0.f;
       scale_shift<C * U>(v[r], 1.f, -mean[r]);
 #pragma unroll
       for (int c = 0; c < C; ++c)

@@ -689,6 +689,19 @@ def test_layer_norm_rows_with_little_spread(op, n, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n", [56, 1000, 4096, 16384, 32768])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_rows_that_begin_far_from_the_rest(op, n, dtype):
+    """One value decides a row's mean and spread, in the first place, behind it, and in the last."""
+    dt = dtype_of(dtype)
+    x = normal(1, 12, n, dtype=dt)
+    for k, at in enumerate((0, 1, n // 2, n - 1)):
+        x[3 * k, at], x[3 * k + 1, at], x[3 * k + 2, at] = 60000.0, -300.0, 20.0
+    mean, rstd = check_norm(op, x, None, None, 1e-5, None)
+    check_norm_backward(op, normal(2, 12, n, dtype=dt), x, mean, rstd, None, None, None)
+
+
+@gpu
 @pytest.mark.parametrize("n", [64, 2053, 40000])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layer_norm_special_rows(op, dtype, n):
