@@ -33,8 +33,8 @@ enum { MACE_ACT_NONE = 0, MACE_ACT_SILU = 1, MACE_ACT_GELU = 2, MACE_ACT_RELU = 
  * [outputs][inputs], bias [outputs] (or NULL), residual, y and z [rows][outputs] (residual or
  * z NULL: left out).  z, kept for mace_dense_backward, is written before the activation.
  * residual may be y itself (same address and ld).
- * float products run on the tensor cores as split fp16 pairs (but for up to 8 rows or outputs, or
- * few inputs: plain float arithmetic): per row and 64 consecutive inputs the largest magnitude sets
+ * float products run on the tensor cores as split fp16 pairs (but for up to 8 rows or outputs, few
+ * inputs, and some unaligned rows: plain float arithmetic): per row and 64 consecutive inputs the largest magnitude sets
  * the scale, values down to 2^-29 of it keep 22 bits, and smaller ones are held to 2^-52 of it.
  * Infinities and NaN give what the sum gives (such results are summed again, which is slow where
  * there are many). */

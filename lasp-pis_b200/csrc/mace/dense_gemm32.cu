@@ -27,9 +27,9 @@
 //   8..15   drain: lane = output row, two warps per TMEM lane quadrant, BN / 2 columns each, and the
 //           epilogue.  A slab that has reached TMEM has left its stage: one of them (in turn) then
 //           starts the loads of the slab that takes its place.
-// What bounds it: no unit (gradients of 84613 x 64 -> 1280, 268 us: issue slots 34% busy, DRAM 33%, tensor
-// pipe 12%), but the chain load, split, multiply, drain of a slab at one CTA per SM (10000 x 512 -> 512: 55
-// us); with one slab per tile (84613 x 64 -> 1280: 156 us, 2.9 TB/s) the drain, by its instructions'
+// What bounds it: no unit (gradients of 84613 x 64 -> 1280, 284 us: issue slots 47% busy, DRAM 41%, tensor
+// pipe 17%), but the chain load, split, multiply, drain of a slab at one CTA per SM (10000 x 512 -> 512: 57
+// us); with one slab per tile (84613 x 64 -> 1280: 155 us, 2.9 TB/s) the drain, by its instructions'
 // latencies: the bias as the sums' first value, prefetched, and scales as whole floats took it from 200 us
 // to 179.  Measured and not kept: plain loads
 // straight into the split's registers (10000 x 512 -> 512: 174 us, then 104 with TMA), P split in place

@@ -8,14 +8,15 @@
 //
 // One pass over the data: a row stays in the registers of its group of threads (part of a warp, a
 // warp, or a block for wide rows) between its statistics and its result.  HBM bounds it, so what
-// counts is bytes in flight: a warp holds rows of up to 8 KiB, and where a thread's share of a row is
-// small it takes several rows at once, and loads the next ones before the arithmetic of these.  The
+// counts is bytes in flight: a warp holds rows of up to 4 KiB (backward 1 KiB), a block wider ones, and
+// where a thread's share of a row is small it takes several rows at once, and loads the next ones
+// before the arithmetic of these.  The
 // variance is taken about a first mean and corrected for that mean's own rounding, so a row far from
 // zero loses nothing.  A group walks the rows with a fixed set of columns per thread, so the
 // parameters' gradients stay in registers too; each block writes one partial row of dgamma and
 // dbeta, and a second launch adds the partial rows in a fixed order.
 //
-// bf16 16384 x 4096 forward: 57 us, 4.7 TB/s (0.72 of the measured copy rate); f16 8191 x 2048: 18 us
+// bf16 16384 x 4096 forward: 60 us, 4.4 TB/s (0.68 of the measured copy rate); f16 8191 x 2048: 18 us
 // forward, 29 backward (3.5 TB/s); f32 84613 x 64 with SiLU: 11.5 and 17.8.
 #include "operators.cuh"
 #include "tcgen05.cuh"
